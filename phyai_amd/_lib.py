@@ -56,6 +56,23 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "phyai_fp8_debug_mfma_rate": (_int, [_int, _int, _vp, _vp, _vp]),
 }
 
+# the same library's second interface; mirrors include/phyai_layer.h one to one
+LAYER_ABI_VERSION = 1
+_f32 = ctypes.c_float
+LAYER_SIGNATURES: dict[str, tuple[object, list[object]]] = {
+    "phyai_layer_abi_version": (_int, []),
+    "phyai_layer_last_error": (ctypes.c_char_p, []),
+    "phyai_layer_block_quant": (_int, [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp]),
+    "phyai_layer_block_gemm": (_int, [_vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp]),
+    "phyai_layer_block_linear_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "phyai_layer_block_linear": (_int, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
+    "phyai_layer_head_rope": (_int, [_vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
+                                     _i64, _i64, _f32, _int, _int, _int, _vp]),
+    "phyai_layer_paged_attention_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "phyai_layer_paged_attention": (_int, [_vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
+                                           _i64, _f32, _int, _i64, _int, _vp, _sz, _vp]),
+}
+
 
 class Fp8LibraryError(RuntimeError):
     """The native library is missing, stale, or a call into it failed."""
@@ -79,7 +96,7 @@ def open_library(path: str) -> ctypes.CDLL:
             "(or phyai_amd._lib.build()); there is no non-HIP fallback"
         )
     lib = ctypes.CDLL(path)
-    for name, (res, args) in SIGNATURES.items():
+    for name, (res, args) in (SIGNATURES | LAYER_SIGNATURES).items():
         try:
             fn = getattr(lib, name)
         except AttributeError as e:
@@ -89,6 +106,9 @@ def open_library(path: str) -> ctypes.CDLL:
     got = lib.phyai_fp8_abi_version()
     if got != ABI_VERSION:
         raise Fp8LibraryError(f"{path} has ABI version {got}, expected {ABI_VERSION}; rebuild it")
+    got = lib.phyai_layer_abi_version()
+    if got != LAYER_ABI_VERSION:
+        raise Fp8LibraryError(f"{path} has layer ABI version {got}, expected {LAYER_ABI_VERSION}; rebuild it")
     return lib
 
 
@@ -120,4 +140,10 @@ def open_host_extension():
 def check(rc: int, what: str) -> None:
     if rc != 0:
         msg = load().phyai_fp8_last_error()
+        raise Fp8LibraryError(f"{what} failed (rc={rc}): {msg.decode() if msg else ''}")
+
+
+def check_layer(rc: int, what: str) -> None:
+    if rc != 0:
+        msg = load().phyai_layer_last_error()
         raise Fp8LibraryError(f"{what} failed (rc={rc}): {msg.decode() if msg else ''}")

@@ -669,6 +669,297 @@ def fp8_mlp(x: torch.Tensor, weight1: torch.Tensor, weight1_scale: torch.Tensor,
     return out
 
 
+# ---- linear with a scale for each block of 128 ----------------------------------------------------
+
+BLOCK = 128   # elements per scale, along K and (of weights) along N
+
+
+def _device_of(op: str, device: torch.device):
+    """Context in which ``device`` is the current one: kernels are launched on its current stream."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _same_device(op: str, device: torch.device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and (not isinstance(t, torch.Tensor) or t.device != device):
+            raise _err(op, f"{name} must be a tensor on {device}, got {t.device if isinstance(t, torch.Tensor) else type(t)!r}")
+
+
+def fp8_block_quant(x: torch.Tensor, *, out: torch.Tensor | None = None,
+                    scale_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """e4m3fn quantization of bf16 ``x[..., K]`` with one scale per 128 elements of a row:
+    ``scale = max(amax, 1e-12) / 448`` in fp32, ``codes = e4m3fn(x / scale)``; the last block of a row may be
+    shorter.  Returns ``(codes[..., K] float8_e4m3fn, scale[..., ceil(K / 128)] float32)``."""
+    op = "fp8_block_quant"
+    x2 = _as_rows(op, x, "x", torch.bfloat16)
+    M, K = x2.shape
+    if K == 0 or K % 8 != 0:
+        raise _err(op, f"last dim {K} must be a positive multiple of 8")
+    blocks = -(-K // BLOCK)
+    if out is None:
+        out = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    elif out.shape != x.shape or out.dtype != torch.float8_e4m3fn or not out.is_contiguous() or out.device != x.device:
+        raise _err(op, "out must be a contiguous float8_e4m3fn tensor shaped like x")
+    sshape = (*x.shape[:-1], blocks)
+    if scale_out is None:
+        scale_out = torch.empty(sshape, dtype=torch.float32, device=x.device)
+    elif scale_out.shape != sshape or scale_out.dtype != torch.float32 or not scale_out.is_contiguous() or scale_out.device != x.device:
+        raise _err(op, f"scale_out must be a contiguous float32 tensor of shape {sshape}")
+    if M == 0:
+        return out, scale_out
+    with _device_of(op, x.device):
+        rc = _lib.load().phyai_layer_block_quant(x2.data_ptr(), x2.stride(0) if M > 1 else K, M, K, out.data_ptr(),
+                                                 scale_out.data_ptr(), blocks, 1, _stream_ptr())
+    _lib.check_layer(rc, op)
+    return out, scale_out
+
+
+def _check_block_weight(op: str, weight, weight_scale, bias, K: int, device) -> int:
+    _same_device(op, device, weight=weight, weight_scale=weight_scale, bias=bias)
+    if weight is None or weight.dim() != 2 or weight.dtype not in (torch.float8_e4m3fn, torch.uint8) or not weight.is_contiguous():
+        raise _err(op, "weight must be a contiguous 2-D float8_e4m3fn GPU tensor (N, K)")
+    N, Kw = weight.shape
+    if Kw != K:
+        raise _err(op, f"weight K={Kw} does not match activation K={K}")
+    if N == 0 or K == 0 or K % 16 != 0 or N % 16 != 0:
+        raise _err(op, f"K={K} and N={N} must be positive multiples of 16")
+    want = (-(-N // BLOCK), -(-K // BLOCK))
+    if weight_scale is None or weight_scale.dtype != torch.float32 or tuple(weight_scale.shape) != want or not weight_scale.is_contiguous():
+        raise _err(op, f"weight_scale must be a contiguous float32 GPU tensor of shape {want}")
+    _check_bias(op, bias, N)
+    return N
+
+
+def fp8_block_gemm(xq: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+                   bias: torch.Tensor | None = None, *, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``bf16(sum over blocks g of 128 along K: x_scale[m, g] * weight_scale[n // 128, g] * (xq @ weight.T over g) + bias)``
+    on quantized activations ``xq[..., K]``.
+
+    ``x_scale``: ``[..., ceil(K / 128)]`` as :func:`fp8_block_quant` returns it, or ``[..., 1]``: one scale per token
+    row (what the per-token quantizers and the norms fused with them return)."""
+    op = "fp8_block_gemm"
+    if not (isinstance(xq, torch.Tensor) and xq.is_cuda and xq.dim() >= 1 and xq.dtype in (torch.float8_e4m3fn, torch.uint8)):
+        raise _err(op, "xq must be a float8_e4m3fn GPU tensor")
+    x2 = xq.reshape(-1, xq.shape[-1])
+    if not x2.is_contiguous() or x2.data_ptr() % 16 != 0:
+        x2 = x2.contiguous() if not x2.is_contiguous() else x2.clone()
+    M, K = x2.shape
+    N = _check_block_weight(op, weight, weight_scale, bias, K, xq.device)
+    blocks = -(-K // BLOCK)
+    _same_device(op, xq.device, x_scale=x_scale, out=out)
+    if x_scale is None or x_scale.dtype != torch.float32 or x_scale.dim() < 1 or x_scale.shape[:-1] != xq.shape[:-1] \
+            or x_scale.shape[-1] not in (1, blocks) or not x_scale.is_contiguous():
+        raise _err(op, f"x_scale must be a contiguous float32 GPU tensor of shape {(*xq.shape[:-1], blocks)} or {(*xq.shape[:-1], 1)}")
+    out = _out_for(op, tuple(xq.shape[:-1]), N, out, xq.device)
+    if M == 0:
+        return out
+    per_row = x_scale.shape[-1]
+    with _device_of(op, xq.device):
+        rc = _lib.load().phyai_layer_block_gemm(x2.data_ptr(), x_scale.data_ptr(), per_row, 1 if per_row == blocks else 0, weight.data_ptr(),
+                                                weight_scale.data_ptr(), bias.data_ptr() if bias is not None else None, out.data_ptr(), N,
+                                                M, N, K, _stream_ptr())
+    _lib.check_layer(rc, op)
+    return out
+
+
+def fp8_block_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: torch.Tensor | None = None, *,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """The W8A8 linear of a checkpoint whose weights have one scale per block of 128 x 128 (``weight_block_size:
+    [128, 128]``): :func:`fp8_block_quant` of bf16 ``x[..., K]`` and :func:`fp8_block_gemm` as one call, bf16 out.  Few
+    token rows are one kernel, which quantizes the rows it multiplies (same codes).
+
+    ``weight``: ``[N, K]`` e4m3fn; ``weight_scale``: ``[ceil(N / 128), ceil(K / 128)]`` fp32, what a code is multiplied
+    with (called ``weight_scale_inv`` in some checkpoints); N and K are multiples of 16."""
+    op = "fp8_block_linear"
+    x2 = _as_rows(op, x, "x", torch.bfloat16)
+    M, K = x2.shape
+    N = _check_block_weight(op, weight, weight_scale, bias, K, x.device)
+    _same_device(op, x.device, out=out)
+    out = _out_for(op, tuple(x.shape[:-1]), N, out, x.device)
+    if M == 0:
+        return out
+    lib = _lib.load()
+    with _device_of(op, x.device):
+        need = lib.phyai_layer_block_linear_workspace_bytes(M, N, K)
+        ws = reserve_workspace(need, x.device) if need else None
+        rc = lib.phyai_layer_block_linear(x2.data_ptr(), x2.stride(0) if M > 1 else K, weight.data_ptr(), weight_scale.data_ptr(),
+                                          bias.data_ptr() if bias is not None else None, out.data_ptr(), N, M, N, K,
+                                          ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, _stream_ptr())
+    _lib.check_layer(rc, op)
+    return out
+
+
+# ---- around attention: head norms with rotation and cache write, attention over pages ---------------------
+
+_HEAD_TYPES = {torch.bfloat16: 0, torch.float16: 1}
+
+
+def rope_table(positions: int, rot: int, base: float = 10000.0, *, device=None) -> torch.Tensor:
+    """``[positions, rot]`` fp32 table of :func:`qk_norm_rope`: row t holds ``cos(t * base ** (-2 i / rot))`` for i < rot / 2,
+    then the sines.  Angles are computed in 64 bits (a far position times a frequency has few bits left in 32)."""
+    inv = float(base) ** (-torch.arange(0, rot, 2, dtype=torch.float64) / rot)
+    angle = torch.arange(positions, dtype=torch.float64)[:, None] * inv
+    return torch.cat([angle.cos(), angle.sin()], dim=1).float().to(device=device if device is not None else "cuda").contiguous()
+
+
+def _page_strides(t: torch.Tensor) -> tuple[int, ...]:
+    """Elements between pages, tokens and heads (0 where there is only one: what torch says there means nothing)."""
+    return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3]))
+
+
+def _check_pages(op: str, k_pages, v_pages, dtype, head_dim: int, device) -> None:
+    _same_device(op, device, k_pages=k_pages, v_pages=v_pages)
+    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+        if t is None or t.dim() != 4 or t.dtype != dtype or t.shape[3] != head_dim:
+            raise _err(op, f"{name} must be a {dtype} GPU tensor of shape (pages, page_size, kv_heads, {head_dim})")
+        if t.numel() and (t.stride(3) != 1 or any(s % 8 for s in _page_strides(t)) or t.data_ptr() % 16):
+            raise _err(op, f"{name} needs head_dim innermost, other strides that are multiples of 8 and a 16-byte aligned base")
+    if k_pages.shape != v_pages.shape:
+        raise _err(op, f"k_pages and v_pages must have one shape, got {tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
+    if k_pages.shape[1] == 0 or k_pages.shape[2] == 0:
+        raise _err(op, "a page must hold at least one token and one head")
+
+
+def _vector(op: str, name: str, t, dtype, n: int, device) -> int:
+    if not isinstance(t, torch.Tensor) or t.device != device or t.dtype != dtype or t.shape != (n,) or not t.is_contiguous():
+        raise _err(op, f"{name} must be a contiguous {dtype} tensor of {n} elements on {device}")
+    return t.data_ptr()
+
+
+def qk_norm_rope(qkv: torch.Tensor, cos_sin: torch.Tensor, positions: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int, *,
+                 q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6, gemma: bool = False,
+                 interleaved: bool = False, k_pages: torch.Tensor | None = None, v_pages: torch.Tensor | None = None,
+                 slots: torch.Tensor | None = None, out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Norms of the query and key heads of a fused projection, the position rotation, and the write of keys and values
+    into a paged cache, in one pass (bf16 or fp16, fp32 inside, one rounding).
+
+    ``qkv``: ``[T, (num_heads + 2 num_kv_heads) * head_dim]`` = q | k | v as ``QKVParallelLinear`` returns it.  ``q_weight`` /
+    ``k_weight`` (``[head_dim]``, both or neither): RMSNorm of every head with that weight (``1 + weight`` with ``gemma``).
+    ``cos_sin``: ``[table, rot]`` fp32 (:func:`rope_table`), the angles of the first ``rot`` elements of a head at each
+    position; pairs are ``(i, i + rot / 2)`` or, ``interleaved``, ``(2 i, 2 i + 1)``.  ``positions``: ``[T]`` int64; one
+    outside the table turns its token into NaNs.
+
+    With ``k_pages`` / ``v_pages`` (``[pages, page_size, num_kv_heads, head_dim]``) and ``slots`` (``[T]`` int64, page *
+    page_size + place) keys and values go into the cache and ``(q, None)`` is returned; a slot outside the cache (-1: padding)
+    is not written, and slots must differ from each other.  Without pages the result is ``(q, k)``; values stay in ``qkv``.
+    ``out``: where q ``[T, num_heads, head_dim]`` goes."""
+    op = "qk_norm_rope"
+    if not (isinstance(qkv, torch.Tensor) and qkv.is_cuda and qkv.dim() == 2 and qkv.dtype in _HEAD_TYPES):
+        raise _err(op, "qkv must be a 2-D bfloat16 or float16 GPU tensor")
+    H, KV, D = int(num_heads), int(num_kv_heads), int(head_dim)
+    if H <= 0 or KV <= 0 or D <= 0 or D % 8 != 0 or D > 512:
+        raise _err(op, f"bad heads: num_heads={H}, num_kv_heads={KV}, head_dim={D} (a multiple of 8 up to 512)")
+    T, dev, dtype = qkv.shape[0], qkv.device, qkv.dtype
+    width = (H + 2 * KV) * D
+    if qkv.shape[1] != width:
+        raise _err(op, f"qkv must have {width} columns for {H} + 2 * {KV} heads of {D}, got {qkv.shape[1]}")
+    if qkv.stride(1) != 1 or (T > 1 and (qkv.stride(0) % 8 != 0 or qkv.stride(0) < width)) or qkv.data_ptr() % 16 != 0:
+        qkv = qkv.contiguous() if not qkv.is_contiguous() else qkv.clone()
+    if not (isinstance(cos_sin, torch.Tensor) and cos_sin.device == dev and cos_sin.dtype == torch.float32 and cos_sin.dim() == 2
+            and cos_sin.is_contiguous() and cos_sin.data_ptr() % 16 == 0 and cos_sin.shape[0] > 0):
+        raise _err(op, f"cos_sin must be a contiguous 2-D float32 tensor on {dev} with at least one row")
+    rot = cos_sin.shape[1]
+    if rot > D or rot % 8 != 0:
+        raise _err(op, f"cos_sin has {rot} columns; needs a multiple of 8 up to head_dim={D}")
+    pos = _vector(op, "positions", positions, torch.int64, T, dev)
+    if (q_weight is None) != (k_weight is None):
+        raise _err(op, "q_weight and k_weight go together")
+    weights = [None, None]
+    if q_weight is not None:
+        weights = [_vector(op, name, w, dtype, D, dev) for name, w in (("q_weight", q_weight), ("k_weight", k_weight))]
+        if any(w % 16 for w in weights):
+            raise _err(op, "q_weight and k_weight must be 16-byte aligned")
+    if out is None:
+        out = torch.empty(T, H, D, dtype=dtype, device=dev)
+    elif tuple(out.shape) != (T, H, D) or out.dtype != dtype or out.device != dev or not out.is_contiguous() or out.data_ptr() % 16:
+        raise _err(op, f"out must be a contiguous {dtype} tensor of shape {(T, H, D)} on {dev}, 16-byte aligned")
+    paged = k_pages is not None or v_pages is not None or slots is not None
+    k = ks = vs = slot_ptr = None
+    n_pages = page_size = 0
+    if paged:
+        import ctypes
+
+        _check_pages(op, k_pages, v_pages, dtype, D, dev)
+        if k_pages.shape[2] != KV:
+            raise _err(op, f"pages have {k_pages.shape[2]} heads, num_kv_heads is {KV}")
+        slot_ptr = _vector(op, "slots", slots, torch.int64, T, dev)
+        n_pages, page_size = k_pages.shape[:2]
+        ks, vs = ((ctypes.c_int64 * 3)(*_page_strides(t)) for t in (k_pages, v_pages))
+    else:
+        k = torch.empty(T, KV, D, dtype=dtype, device=dev)
+    if T == 0:
+        return out, k
+    with _device_of(op, dev):
+        rc = _lib.load().phyai_layer_head_rope(
+            qkv.data_ptr(), qkv.stride(0) if T > 1 else width, *weights, cos_sin.data_ptr(), cos_sin.shape[0], pos, out.data_ptr(),
+            k.data_ptr() if k is not None else None, k_pages.data_ptr() if paged else None, v_pages.data_ptr() if paged else None, ks, vs,
+            slot_ptr, n_pages, page_size, T, H, KV, D, rot, float(eps), 1 if gemma else 0, 1 if interleaved else 0, _HEAD_TYPES[dtype],
+            _stream_ptr())
+    _lib.check_layer(rc, op)
+    return out, k
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, q_offsets: torch.Tensor,
+                    kv_lens: torch.Tensor, *, scale: float | None = None, causal: bool = True, window: int | None = None,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of each sequence's new tokens - one, or a chunk - over its pages of a cache that holds their keys and
+    values already.
+
+    ``q``: ``[T, heads, head_dim]`` bf16 or fp16; sequence b's tokens are rows ``q_offsets[b]`` to ``q_offsets[b + 1]``
+    (``[B + 1]`` int32).  ``k_pages`` / ``v_pages``: ``[pages, page_size, kv_heads, head_dim]`` with equal strides; key j of
+    sequence b is token ``j % page_size`` of page ``page_table[b, j // page_size]`` (``[B, width]`` int32), ``kv_lens[b]``
+    (``[B]`` int32) of them.  The new tokens are the last of these: token i stands at ``kv_lens[b] - tokens + i`` and sees
+    keys up to its own (``causal``), or all, and with ``window`` none that lie ``window`` or more before it.  Query head h
+    reads key head ``h // (heads // kv_heads)``.  ``scale`` defaults to ``head_dim ** -0.5``.
+
+    Returns ``[T, heads, head_dim]``; a row that sees nothing is zero, rows outside every sequence are left as they were
+    (of a fresh result: undefined), and rows that see keys of a page that does not exist are NaN."""
+    op = "paged_attention"
+    if not (isinstance(q, torch.Tensor) and q.is_cuda and q.dim() == 3 and q.dtype in _HEAD_TYPES):
+        raise _err(op, "q must be a 3-D bfloat16 or float16 GPU tensor (tokens, heads, head_dim)")
+    T, H, D = q.shape
+    dev, dtype = q.device, q.dtype
+    if H == 0 or D == 0 or D % 8 != 0 or D > 256:
+        raise _err(op, f"needs at least one head and head_dim a multiple of 8 up to 256, got {H} heads of {D}")
+    if q.numel() and (q.stride(2) != 1 or q.stride(0) % 8 != 0 or q.stride(1) % 8 != 0 or q.data_ptr() % 16 != 0):
+        q = q.contiguous() if not q.is_contiguous() else q.clone()
+    _check_pages(op, k_pages, v_pages, dtype, D, dev)
+    if k_pages.numel() and _page_strides(k_pages) != _page_strides(v_pages):
+        raise _err(op, f"k_pages and v_pages must have the same strides, got {k_pages.stride()} and {v_pages.stride()}")
+    n_pages, page_size, KV, _ = k_pages.shape
+    if H % KV != 0:
+        raise _err(op, f"{H} query heads are not a multiple of {KV} key heads")
+    if not (isinstance(page_table, torch.Tensor) and page_table.device == dev and page_table.dtype == torch.int32 and page_table.dim() == 2
+            and (page_table.numel() == 0 or page_table.stride(1) == 1)):
+        raise _err(op, f"page_table must be a 2-D int32 tensor on {dev} with contiguous rows")
+    B, W = page_table.shape
+    offsets, lens = _vector(op, "q_offsets", q_offsets, torch.int32, B + 1, dev), _vector(op, "kv_lens", kv_lens, torch.int32, B, dev)
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise _err(op, f"scale must be a positive number, got {scale}")
+    if window is not None and window < 1:
+        raise _err(op, f"window must be at least 1, got {window}")
+    if out is None:
+        out = torch.empty(T, H, D, dtype=dtype, device=dev)
+    elif tuple(out.shape) != (T, H, D) or out.dtype != dtype or out.device != dev or not out.is_contiguous() or out.data_ptr() % 16:
+        raise _err(op, f"out must be a contiguous {dtype} tensor of shape {(T, H, D)} on {dev}, 16-byte aligned")
+    if T == 0 or B == 0:
+        return out
+    import ctypes
+
+    lib = _lib.load()
+    with _device_of(op, dev):
+        need = lib.phyai_layer_paged_attention_workspace_bytes(T, B, H, KV, D, W * page_size)
+        ws = reserve_workspace(need, dev) if need else None
+        rc = lib.phyai_layer_paged_attention(
+            q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), v_pages.data_ptr(), (ctypes.c_int64 * 3)(*_page_strides(k_pages)), n_pages,
+            page_size, page_table.data_ptr(), page_table.stride(0), W, offsets, lens, out.data_ptr(), T, B, H, KV, D, scale, 1 if causal else 0,
+            min(int(window), (1 << 31) - 1) if window is not None else 0, _HEAD_TYPES[dtype], ws.data_ptr() if ws is not None else None,
+            ws.numel() if ws is not None else 0, _stream_ptr())
+    _lib.check_layer(rc, op)
+    return out
+
+
 STAMP_WORDS = 12
 
 
