@@ -15,6 +15,8 @@
 
 #include <dlfcn.h>
 
+#include <cmath>
+
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
@@ -23,6 +25,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/phyai_fp8.h"
+#include "../../include/phyai_layer.h"
 #include "host_entry.h"
 
 namespace {
@@ -46,6 +49,11 @@ struct Lib {
     decltype(&phyai_fp8_linear_per_tensor) per_tensor;
     decltype(&phyai_fp8_rmsnorm_quant) rmsnorm;
     decltype(&phyai_fp8_adarmsnorm_quant) adarmsnorm;
+    decltype(&phyai_layer_block_linear) block_linear;
+    decltype(&phyai_layer_block_linear_workspace_bytes) block_linear_ws;
+    decltype(&phyai_layer_head_rope) head_rope;
+    decltype(&phyai_layer_paged_attention) attention;
+    decltype(&phyai_layer_paged_attention_workspace_bytes) attention_ws;
 } lib = {};
 
 struct Py {
@@ -792,6 +800,154 @@ PyObject* py_adarmsnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- around attention (phyai_layer.h) -------------------------------------------------------------------------------
+bool on(const at::Tensor* t, const at::Device& dev) { return t && t->is_cuda() && t->device() == dev; }
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool vector_on(const at::Tensor* t, at::ScalarType dtype, int64_t n, const at::Device& dev) {
+    return on(t, dev) && t->dim() == 1 && vector_of(t, dtype, n);
+}
+int head_type(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 ? PHYAI_LAYER_BF16 : t.scalar_type() == at::kHalf ? PHYAI_LAYER_F16 : -1; }
+at::Tensor fresh3(int64_t a, int64_t b, int64_t c, at::ScalarType dtype, const at::Device& dev) {
+    return at::Tensor(at::detail::empty_cuda({a, b, c}, dtype, dev, std::nullopt));
+}
+// Pages [pages, page_size, heads, D]: strides (0 along an axis of one), false unless the kernels can read them as they lie.
+bool pages_of(const at::Tensor* t, at::ScalarType dtype, int64_t D, const at::Device& dev, int64_t* strides) {
+    if (!on(t, dev) || t->dim() != 4 || t->scalar_type() != dtype || t->size(3) != D || t->numel() == 0 || t->stride(3) != 1 || !aligned16(t->const_data_ptr()))
+        return false;
+    for (int i = 0; i < 3; ++i) {
+        strides[i] = t->size(i) > 1 ? t->stride(i) : 0;
+        if (strides[i] < 0 || strides[i] % 8 != 0) return false;
+    }
+    return true;
+}
+bool integer(PyObject* o, int64_t* v) {
+    if (!PyLong_CheckExact(o)) return false;
+    *v = PyLong_AsLongLong(o);
+    return !(*v == -1 && PyErr_Occurred());
+}
+
+// block_linear(x, weight, weight_scale, bias, out)
+PyObject* py_block_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const at::Tensor *x = n == 5 ? tensor(a[0]) : nullptr, *w = n == 5 ? tensor(a[1]) : nullptr, *s = n == 5 ? tensor(a[2]) : nullptr;
+    Rows r;
+    Where at_;
+    if (!x || !w || !s || !rows_of(*x, at::kBFloat16, &r) || !where(*x, &at_)) return declined();
+    const at::Tensor* b = tensor(a[3]);
+    if (!on(w, at_.dev) || !on(s, at_.dev) || (a[3] != Py_None && !on(b, at_.dev)) || w->dim() != 2 || !codes_dtype(*w) || !w->is_contiguous() ||
+        w->size(1) != r.K)
+        return declined();
+    const int64_t N = w->size(0);
+    if (N == 0 || N % 16 != 0 || r.K % 16 != 0 || s->dim() != 2 || s->scalar_type() != at::kFloat || s->size(0) != (N + 127) / 128 ||
+        s->size(1) != (r.K + 127) / 128 || !s->is_contiguous() || (b && !vector_of(b, at::kBFloat16, N)))
+        return declined();
+    at::Tensor y;
+    if (a[4] != Py_None) {
+        const at::Tensor* o = tensor(a[4]);
+        if (!shaped(o, *x, N, at::kBFloat16) || !on(o, at_.dev)) return declined();
+        y = *o;
+    } else y = fresh(*x, N, at::kBFloat16, at_.dev);
+    Scratch ws = {nullptr, 0};
+    const size_t need = lib.block_linear_ws(r.M, N, r.K);
+    if (need > 0 && !workspace(need, at_, &ws)) return declined();
+    if (lib.block_linear(r.p, r.ld, w->const_data_ptr(), s->const_data_ptr<float>(), b ? b->const_data_ptr() : nullptr, y.mutable_data_ptr(), N, r.M, N, r.K,
+                         ws.p, ws.n, at_.stream) != 0)
+        return declined();
+    return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
+// qk_norm_rope(qkv, cos_sin, positions, heads, kv_heads, head_dim, q_weight, k_weight, eps, gemma, interleaved, k_pages, v_pages,
+// slots, out) -> (q, k or None)
+PyObject* py_qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const at::Tensor *x = n == 15 ? tensor(a[0]) : nullptr, *cs = n == 15 ? tensor(a[1]) : nullptr;
+    Where at_;
+    int64_t H, KV, D;
+    if (!x || !cs || x->dim() != 2 || x->numel() == 0 || !where(*x, &at_) || head_type(*x) < 0 || !integer(a[3], &H) || !integer(a[4], &KV) ||
+        !integer(a[5], &D))
+        return declined();
+    const int64_t T = x->size(0), most = 1 << 16;
+    if (H <= 0 || KV <= 0 || D <= 0 || H > most || KV > most || D > 512 || D % 8 != 0 || x->size(1) != (H + 2 * KV) * D || x->stride(1) != 1) return declined();
+    const int64_t ld = T > 1 ? x->stride(0) : x->size(1);
+    if (ld % 8 != 0 || ld < x->size(1) || !aligned16(x->const_data_ptr())) return declined();
+    if (!on(cs, at_.dev) || cs->dim() != 2 || cs->scalar_type() != at::kFloat || !cs->is_contiguous() || cs->size(0) == 0 || cs->size(1) % 8 != 0 ||
+        cs->size(1) > D || !aligned16(cs->const_data_ptr()) || !vector_on(tensor(a[2]), at::kLong, T, at_.dev))
+        return declined();
+    const auto dtype = x->scalar_type();
+    const at::Tensor *qw = tensor(a[6]), *kw = tensor(a[7]);
+    if (a[6] != Py_None || a[7] != Py_None)
+        if (!vector_on(qw, dtype, D, at_.dev) || !vector_on(kw, dtype, D, at_.dev) || !aligned16(qw->const_data_ptr()) || !aligned16(kw->const_data_ptr()))
+            return declined();
+    const double eps = PyFloat_AsDouble(a[8]);
+    if (eps == -1.0 && PyErr_Occurred()) return declined();
+    const int gemma = PyObject_IsTrue(a[9]), inter = PyObject_IsTrue(a[10]);
+    if (gemma < 0 || inter < 0) return declined();
+    const at::Tensor *kp = tensor(a[11]), *vp = tensor(a[12]), *slots = tensor(a[13]);
+    const bool paged = a[11] != Py_None || a[12] != Py_None || a[13] != Py_None;
+    int64_t ks[3], vs[3];
+    if (paged && (!pages_of(kp, dtype, D, at_.dev, ks) || !pages_of(vp, dtype, D, at_.dev, vs) || kp->sizes() != vp->sizes() || kp->size(2) != KV ||
+                  !vector_on(slots, at::kLong, T, at_.dev)))
+        return declined();
+    at::Tensor q, k;
+    if (a[14] != Py_None) {
+        const at::Tensor* o = tensor(a[14]);
+        if (!on(o, at_.dev) || o->dim() != 3 || o->scalar_type() != dtype || !o->is_contiguous() || o->size(0) != T || o->size(1) != H || o->size(2) != D ||
+            !aligned16(o->const_data_ptr()))
+            return declined();
+        q = *o;
+    } else q = fresh3(T, H, D, dtype, at_.dev);
+    if (!paged) k = fresh3(T, KV, D, dtype, at_.dev);
+    if (lib.head_rope(x->const_data_ptr(), ld, qw ? qw->const_data_ptr() : nullptr, kw ? kw->const_data_ptr() : nullptr, cs->const_data_ptr<float>(), cs->size(0),
+                      tensor(a[2])->const_data_ptr<int64_t>(), q.mutable_data_ptr(), paged ? nullptr : k.mutable_data_ptr(),
+                      paged ? kp->mutable_data_ptr() : nullptr, paged ? vp->mutable_data_ptr() : nullptr, ks, vs,
+                      paged ? slots->const_data_ptr<int64_t>() : nullptr, paged ? kp->size(0) : 0, paged ? kp->size(1) : 0, T, H, KV, D, cs->size(1), (float)eps,
+                      gemma, inter, head_type(*x), at_.stream) != 0)
+        return declined();
+    return Py_BuildValue("NN", THPVariable_Wrap(std::move(q)), wrap_or_none(k));
+    END_HANDLE_TH_ERRORS
+}
+
+// paged_attention(q, k_pages, v_pages, page_table, q_offsets, kv_lens, scale, causal, window, out)
+PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const at::Tensor *q = n == 10 ? tensor(a[0]) : nullptr, *kp = n == 10 ? tensor(a[1]) : nullptr, *vp = n == 10 ? tensor(a[2]) : nullptr,
+                     *table = n == 10 ? tensor(a[3]) : nullptr;
+    Where at_;
+    if (!q || !kp || !vp || !table || q->dim() != 3 || q->numel() == 0 || !where(*q, &at_) || head_type(*q) < 0) return declined();
+    const int64_t T = q->size(0), H = q->size(1), D = q->size(2);
+    if (D % 8 != 0 || D > 256 || q->stride(2) != 1 || q->stride(0) % 8 != 0 || q->stride(1) % 8 != 0 || !aligned16(q->const_data_ptr())) return declined();
+    const auto dtype = q->scalar_type();
+    int64_t ks[3], vs[3];
+    if (!pages_of(kp, dtype, D, at_.dev, ks) || !pages_of(vp, dtype, D, at_.dev, vs) || kp->sizes() != vp->sizes() || ks[0] != vs[0] || ks[1] != vs[1] ||
+        ks[2] != vs[2] || H % kp->size(2) != 0)
+        return declined();
+    if (!on(table, at_.dev) || table->dim() != 2 || table->scalar_type() != at::kInt || table->numel() == 0 || table->stride(1) != 1) return declined();
+    const int64_t B = table->size(0), W = table->size(1);
+    const at::Tensor *offsets = tensor(a[4]), *lens = tensor(a[5]);
+    if (!vector_on(offsets, at::kInt, B + 1, at_.dev) || !vector_on(lens, at::kInt, B, at_.dev)) return declined();
+    const double scale = a[6] == Py_None ? 1.0 / std::sqrt((double)D) : PyFloat_AsDouble(a[6]);
+    if (scale == -1.0 && PyErr_Occurred()) return declined();
+    const int causal = PyObject_IsTrue(a[7]);
+    int64_t window = 0;
+    if (causal < 0 || !(scale > 0.0) || (a[8] != Py_None && (!integer(a[8], &window) || window < 1 || window > 0x7FFFFFFF))) return declined();
+    at::Tensor o;
+    if (a[9] != Py_None) {
+        const at::Tensor* t = tensor(a[9]);
+        if (!on(t, at_.dev) || t->scalar_type() != dtype || t->sizes() != q->sizes() || !t->is_contiguous() || !aligned16(t->const_data_ptr())) return declined();
+        o = *t;
+    } else o = fresh3(T, H, D, dtype, at_.dev);
+    Scratch ws = {nullptr, 0};
+    const size_t need = lib.attention_ws(T, B, H, kp->size(2), D, W * kp->size(1));
+    if (need > 0 && !workspace(need, at_, &ws)) return declined();
+    if (lib.attention(q->const_data_ptr(), q->stride(0), q->stride(1), kp->const_data_ptr(), vp->const_data_ptr(), ks, kp->size(0), kp->size(1),
+                      table->const_data_ptr<int32_t>(), table->stride(0), W, offsets->const_data_ptr<int32_t>(), lens->const_data_ptr<int32_t>(),
+                      o.mutable_data_ptr(), T, B, H, kp->size(2), D, (float)scale, causal, window, head_type(*q), ws.p, ws.n, at_.stream) != 0)
+        return declined();
+    return THPVariable_Wrap(std::move(o));
+    END_HANDLE_TH_ERRORS
+}
+
 // ---- module --------------------------------------------------------------------------------------------------------
 // bind(library path, workspaces, owner variable, reserve, epilogues, layouts, ActivationView, PER_CHANNEL, PER_TENSOR)
 PyObject* py_bind(PyObject*, PyObject* args) {
@@ -825,6 +981,11 @@ PyObject* py_bind(PyObject*, PyObject* args) {
     get(l.per_tensor, "phyai_fp8_linear_per_tensor");
     get(l.rmsnorm, "phyai_fp8_rmsnorm_quant");
     get(l.adarmsnorm, "phyai_fp8_adarmsnorm_quant");
+    get(l.block_linear, "phyai_layer_block_linear");
+    get(l.block_linear_ws, "phyai_layer_block_linear_workspace_bytes");
+    get(l.head_rope, "phyai_layer_head_rope");
+    get(l.attention, "phyai_layer_paged_attention");
+    get(l.attention_ws, "phyai_layer_paged_attention_workspace_bytes");
     if (!ok) return PyErr_Format(PyExc_RuntimeError, "%s lacks an entry point this extension binds", path);
     for (PyObject* o : {p.workspaces, p.owner, p.reserve, p.epilogues, p.layouts, p.view_type, p.per_channel, p.per_tensor}) Py_INCREF(o);
     lib = l;
@@ -889,6 +1050,9 @@ PyMethodDef methods[] = {
     PHYAI_FAST("quant_rowwise", py_quant_rowwise),
     PHYAI_FAST("rmsnorm", py_rmsnorm),
     PHYAI_FAST("adarmsnorm", py_adarmsnorm),
+    PHYAI_FAST("block_linear", py_block_linear),
+    PHYAI_FAST("qk_norm_rope", py_qk_norm_rope),
+    PHYAI_FAST("paged_attention", py_paged_attention),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_phyai_host", "Eager call path of phyai_amd.ops and of the fp8 layers.", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

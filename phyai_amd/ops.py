@@ -771,6 +771,9 @@ def fp8_block_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.
     ``weight``: ``[N, K]`` e4m3fn; ``weight_scale``: ``[ceil(N / 128), ceil(K / 128)]`` fp32, what a code is multiplied
     with (called ``weight_scale_inv`` in some checkpoints); N and K are multiples of 16."""
     op = "fp8_block_linear"
+    y = _native().block_linear(x, weight, weight_scale, bias, out)
+    if y is not None:
+        return y
     x2 = _as_rows(op, x, "x", torch.bfloat16)
     M, K = x2.shape
     N = _check_block_weight(op, weight, weight_scale, bias, K, x.device)
@@ -844,6 +847,10 @@ def qk_norm_rope(qkv: torch.Tensor, cos_sin: torch.Tensor, positions: torch.Tens
     is not written, and slots must differ from each other.  Without pages the result is ``(q, k)``; values stay in ``qkv``.
     ``out``: where q ``[T, num_heads, head_dim]`` goes."""
     op = "qk_norm_rope"
+    got = _native().qk_norm_rope(qkv, cos_sin, positions, num_heads, num_kv_heads, head_dim, q_weight, k_weight, eps, gemma, interleaved,
+                                 k_pages, v_pages, slots, out)
+    if got is not None:
+        return got
     if not (isinstance(qkv, torch.Tensor) and qkv.is_cuda and qkv.dim() == 2 and qkv.dtype in _HEAD_TYPES):
         raise _err(op, "qkv must be a 2-D bfloat16 or float16 GPU tensor")
     H, KV, D = int(num_heads), int(num_kv_heads), int(head_dim)
@@ -915,6 +922,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     Returns ``[T, heads, head_dim]``; a row that sees nothing is zero, rows outside every sequence are left as they were
     (of a fresh result: undefined), and rows that see keys of a page that does not exist are NaN."""
     op = "paged_attention"
+    got = _native().paged_attention(q, k_pages, v_pages, page_table, q_offsets, kv_lens, scale, causal, window, out)
+    if got is not None:
+        return got
     if not (isinstance(q, torch.Tensor) and q.is_cuda and q.dim() == 3 and q.dtype in _HEAD_TYPES):
         raise _err(op, "q must be a 3-D bfloat16 or float16 GPU tensor (tokens, heads, head_dim)")
     T, H, D = q.shape
