@@ -46,6 +46,17 @@ __device__ __forceinline__ float to_f32(uint32_t h) {
     if constexpr (TYPE == HEAD_BF16) return __uint_as_float(h << 16);
     else return (float)__builtin_bit_cast(_Float16, (uint16_t)h);
 }
+// sum + both halves of w, one instruction
+template <int TYPE>
+__device__ __forceinline__ float add_pair(uint32_t w, float sum) {
+    if constexpr (TYPE == HEAD_BF16) {
+        typedef __bf16 pair __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pair, w), __builtin_bit_cast(pair, 0x3F803F80u), sum, false);
+    } else {
+        typedef _Float16 pair __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(pair, w), __builtin_bit_cast(pair, 0x3C003C00u), sum, false);
+    }
+}
 // the value of the lane 32 away, and this lane's: both orders are fine for max and sum
 __device__ __forceinline__ float other_half_max(float v) {
     auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -68,8 +79,9 @@ __device__ __forceinline__ bool locate(const PagedAttention& p, int group, int r
     int before = 0;
     for (int base = 0; base < p.B; base += 64) {
         const int b = base + lane;
-        int q0 = 0, q1 = 0;
+        int q0 = 0, q1 = 0, kv = 0;
         if (b < p.B) {
+            kv = p.kv_lens[b];
             q0 = clamp_i(p.q_offsets[b], 0, p.T);
             q1 = clamp_i(p.q_offsets[b + 1], q0, p.T);
         }
@@ -89,9 +101,8 @@ __device__ __forceinline__ bool locate(const PagedAttention& p, int group, int r
             o.rows = o.q_len * group;
             o.row0 = (tile - before - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(tiles, l))) * rows_per_tile;
             const int64_t most = (int64_t)p.table_width * p.page_size;
-            const int kv = p.kv_lens[o.b];
+            kv = __builtin_amdgcn_readlane(kv, l);
             o.kv_len = kv < 0 ? 0 : kv > most ? (int)most : kv;
-            o.kv_len = __builtin_amdgcn_readfirstlane(o.kv_len);
             return true;
         }
         before += __builtin_amdgcn_readlane(upto, 63);
@@ -160,7 +171,7 @@ __device__ __forceinline__ void copy_keys(const Pool& s, int page, int j0, int r
         return;
     }
     const int lo = (int)(uint32_t)off, hi = (int)(off >> 32), kind = !there ? 1 : !good ? 2 : 0;
-#pragma unroll
+#pragma unroll 1   // (code that a cold instruction cache does not have to bring: most calls come here once)
     for (int t = 0; t < COPIES; ++t) {
         const int from = t * S::PER_COPY + (int)lr;
         const uint32_t r = (uint32_t)(row + from);
@@ -276,26 +287,30 @@ __device__ __forceinline__ void attend_block(State<DP>& st, const v4i* qf, const
     if (__any(mx > st.m + kRescaleAt)) {
         const float m = __builtin_fmaxf(st.m, mx);
         const float a = m == kNone ? 1.0f : __builtin_amdgcn_exp2f(st.m - m);
+        if (__any(st.m != kNone)) {   // (else O and l are zero)
+            st.l *= a;
+#pragma unroll
+            for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) st.o[b][i] *= a;
+        }
         st.m = m;
-        st.l *= a;
-#pragma unroll
-        for (int b = 0; b < DP / 32; ++b)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) st.o[b][i] *= a;
     }
     const float base = st.m == kNone ? 0.f : st.m;
-    float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -base));
-        sum += s[i];
-    }
-    st.l += sum;
+    for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -base));
+    // the sum is of the rounded probabilities, those that the second product uses: their common error cancels
     v4i pf[2];
+    float sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pf[e][i] = (int)pack2<TYPE>(s[8 * e + 2 * i], s[8 * e + 2 * i + 1]);
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t w = pack2<TYPE>(s[8 * e + 2 * i], s[8 * e + 2 * i + 1]);
+            pf[e][i] = (int)w;
+            sum[e] = add_pair<TYPE>(w, sum[e]);
+        }
+    st.l += sum[0] + sum[1];
     // V^T: lane (16 g + t) asks for key 4 half + t / 4 of a run of eight and dims 16 (g & 1) + 4 (t & 3) .. of a block of 32
     const uint32_t key0 = (uint32_t)(4 * half + ((lane & 15) >> 2)), chunk0 = (uint32_t)((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
     const uint32_t v0 = key0 * S::ROW + ((chunk0 ^ v_swizzle<DP>(key0)) << 4) + (lane & 1) * 8;
@@ -423,13 +438,7 @@ __global__ __launch_bounds__(SplitShape<DP>::WAVES * 64, 1) void attend_split_ke
         load_q<DP>(p, row, qf);
         volatile uint32_t* my_id = &ids[wave][lane];
         copy_page_id(pool, table, p.table_width, begin * 32 + (lane & 31), idp);
-        wait_copies<0>();
-        copy_keys<DP, 32>(pool, (int)*my_id, begin * 32, 0, base, base + 32 * S::ROW);
-        if (begin + 1 < end) {
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            copy_page_id(pool, table, p.table_width, begin * 32 + 32 + (lane & 31), idp);
-        }
-        for (int blk = begin; blk < end; ++blk) {
+        for (int blk = begin - 1; blk < end; ++blk) {
             const int cur = (blk - begin) & 1;
             // this stage and the next one's page numbers have landed; the other stage has been read
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -442,6 +451,7 @@ __global__ __launch_bounds__(SplitShape<DP>::WAVES * 64, 1) void attend_split_ke
                     copy_page_id(pool, table, p.table_width, (blk + 2) * 32 + (lane & 31), idp);
                 }
             }
+            if (blk < begin) continue;
             uint8_t* k = mine + cur * X::STAGE;
             const int j0 = blk * 32;
             if (j0 < all_lo || j0 + 32 > all_hi) special |= clean_values<DP, TYPE, 32>(k + 32 * S::ROW);
@@ -573,20 +583,13 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
     const uint32_t base = (uint32_t)(uintptr_t)lds, idp = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)ids[wave]);
     volatile uint32_t* my_id = &ids[wave][lane];
     const int ahead = wave * MINE + (lane & (MINE - 1));   // the key of a tile whose page this lane looks up
-    if (begin < end) {
-        copy_page_id(pool, table, p.table_width, begin * X::KEYS + ahead, idp);
-        wait_copies<0>();
-        copy_keys<DP, MINE>(pool, (int)*my_id, begin * X::KEYS + wave * MINE, wave * MINE, base, base + X::KEYS * S::ROW);
-        if (begin + 1 < end) {
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            copy_page_id(pool, table, p.table_width, (begin + 1) * X::KEYS + ahead, idp);
-        }
-    }
+    if (begin < end) copy_page_id(pool, table, p.table_width, begin * X::KEYS + ahead, idp);
     bool special = false;
-    for (int blk = begin; blk < end; ++blk) {
+    for (int blk = begin - 1; blk < end; ++blk) {
         const int cur = (blk - begin) & 1;
+        // this tile and the next one's page numbers have landed; behind the barrier the other stage has been read
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        if (blk * X::KEYS < all_lo || (blk + 1) * X::KEYS > all_hi)
+        if (blk >= begin && (blk * X::KEYS < all_lo || (blk + 1) * X::KEYS > all_hi))
             special |= clean_values<DP, TYPE, MINE>(lds + cur * X::STAGE + (X::KEYS + wave * MINE) * S::ROW);
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (blk + 1 < end) {
@@ -598,6 +601,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
                 copy_page_id(pool, table, p.table_width, (blk + 2) * X::KEYS + ahead, idp);
             }
         }
+        if (blk < begin) continue;
         const uint8_t* k = lds + cur * X::STAGE;
 #pragma unroll
         for (int x = 0; x < X::KEYS / 32; ++x) {
