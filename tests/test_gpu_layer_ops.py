@@ -74,15 +74,18 @@ def test_block_quant_special_values_stay_in_their_block(dev, value):
     assert torch.equal(codes[rest], clean.float()[rest]) and torch.equal(scale[1], clean_scale[1])
 
 
-SHAPES = [(1, 16, 16), (1, 256, 128), (3, 144, 272), (16, 128, 1024), (17, 2560, 1024), (33, 272, 4304), (50, 1024, 512), (64, 160, 1168),
+SHAPES = [(1, 16, 16), (2, 144, 4224), (8, 272, 8304), (4, 64, 1072), (1, 256, 128), (3, 144, 272), (16, 128, 1024), (17, 2560, 1024), (33, 272, 4304), (50, 1024, 512), (64, 160, 1168),
           (65, 144, 144), (100, 400, 256), (129, 272, 1040), (200, 528, 2064), (300, 256, 128), (257, 784, 384)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
-@pytest.mark.parametrize("shape", [None, "0", "1", "2", "3"])
+@pytest.mark.parametrize("shape", [None, "few 1", "few 2", "few 4", "few 11", "few 12", "few 14", "1", "2", "3", "4"])
 def test_block_linear(dev, monkeypatch, m, n, k, shape):
     if shape is not None:
-        monkeypatch.setenv("PHYAI_LAYER_BLOCK", shape)
+        few, _, small = shape.partition(" ")
+        monkeypatch.setenv("PHYAI_LAYER_BLOCK", "0" if small else few)
+        if small:
+            monkeypatch.setenv("PHYAI_LAYER_SMALL", small)
     x = seeded((m, k), m + n, 1.0)
     x[:, :: max(1, k // 7)] *= 20
     w, ws = oracle.block_weight(n, k, gen(k))
