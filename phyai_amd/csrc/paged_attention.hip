@@ -69,12 +69,24 @@ __device__ __forceinline__ float other_half_sum(float v) {
 
 __device__ __forceinline__ int clamp_i(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
 
+// j / d for 0 <= j < 2^31 and a d known on the host: one high product (magic 0: d = 1).
+struct Division {
+    uint32_t magic, shift;
+};
+__device__ __forceinline__ int divide(int j, Division d) { return d.magic == 0 ? j : (int)(__umulhi((uint32_t)j, d.magic) >> d.shift); }
+
+// What the host works out once per call.
+struct Plan {
+    Division page, group, workers;
+    int group_size, tiles, splits, many;
+};
+
 // Where a tile of `rows_per_tile` packed rows lies: the tiles of the sequences are numbered one sequence after another.
 // Every wavefront finds it by itself, 64 sequences at a time.
 struct Tile {
     int b, row0, rows, q_begin, q_len, kv_len;
 };
-__device__ __forceinline__ bool locate(const PagedAttention& p, int group, int rows_per_tile, int tile, Tile& o) {
+__device__ __forceinline__ bool locate(const PagedAttention& p, int group, int rows_per_tile, int tile, Tile& o) {   // (rows_per_tile: a power of two)
     const int lane = threadIdx.x & 63;
     int before = 0;
     for (int base = 0; base < p.B; base += 64) {
@@ -132,11 +144,11 @@ struct Pool {
     const uint8_t *zero, *nan;
     int64_t page_bytes, token_bytes;
     int n_pages, page_size, kv_len;
-    uint32_t magic, shift;             // j / page_size = mulhi(j, magic) >> shift, or j
+    Division by_page;
     int d_chunks;                      // 16-byte chunks of a key that exist
     bool neat;                         // whole keys of a copy instruction are neighbours in a page
 };
-__device__ __forceinline__ int page_of(const Pool& s, int j) { return s.magic == 0 ? j : (int)(__umulhi((uint32_t)j, s.magic) >> s.shift); }
+__device__ __forceinline__ int page_of(const Pool& s, int j) { return divide(j, s.by_page); }
 
 // The page number of key j for every lane, into `slot` (256 bytes of LDS): issued with the copies and counted with them.
 __device__ __forceinline__ void copy_page_id(const Pool& s, const int32_t* table_row, int width, int j, uint32_t slot) {
@@ -158,15 +170,15 @@ __device__ __forceinline__ void copy_keys(const Pool& s, int page, int j0, int r
     const int64_t off = (int64_t)page * s.page_bytes + (int64_t)(j - first) * s.token_bytes;
     const uint32_t lr = (uint32_t)lane / S::CHUNKS, lc = (uint32_t)lane % S::CHUNKS;
     if (s.neat && __all(there && good)) {
-        const uint32_t run = lr * (uint32_t)s.token_bytes;
+        // the swizzles of copy t are those of copy 0 with the bits of t's first key flipped
+        const uint32_t run = lr * (uint32_t)s.token_bytes, kc = (lc ^ k_swizzle<DP>((uint32_t)row + lr)) << 4, vc = (lc ^ v_swizzle<DP>((uint32_t)row + lr)) << 4;
 #pragma unroll
         for (int t = 0; t < COPIES; ++t) {
-            const uint32_t r = (uint32_t)row + t * S::PER_COPY + lr;
-            const int64_t at = (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)off, t * S::PER_COPY) |
-                               (int64_t)__builtin_amdgcn_readlane((int)(off >> 32), t * S::PER_COPY) << 32;
             const uint32_t to = (uint32_t)(row + t * S::PER_COPY) * S::ROW;
-            copy16_to_lds<kBaseSettles>(s.k + at, run + ((lc ^ k_swizzle<DP>(r)) << 4), __builtin_amdgcn_readfirstlane(k_lds + to));
-            copy16_to_lds<kBaseSettles>(s.v + at, run + ((lc ^ v_swizzle<DP>(r)) << 4), __builtin_amdgcn_readfirstlane(v_lds + to));
+            const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)off, t * S::PER_COPY) |
+                                (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(off >> 32), t * S::PER_COPY) << 32;
+            copy16_to_lds<kBaseSettles>(s.k + at, (kc ^ k_swizzle<DP>(t * S::PER_COPY) << 4) + run, __builtin_amdgcn_readfirstlane(k_lds + to));
+            copy16_to_lds<kBaseSettles>(s.v + at, (vc ^ v_swizzle<DP>(t * S::PER_COPY) << 4) + run, __builtin_amdgcn_readfirstlane(v_lds + to));
         }
         return;
     }
@@ -336,20 +348,20 @@ struct Row {
     int token, head, lo, hi;
     bool valid;
 };
-__device__ __forceinline__ Row row_of(const PagedAttention& p, const Tile& t, int group, int kv_head, int row) {
+__device__ __forceinline__ Row row_of(const PagedAttention& p, const Tile& t, const Plan& g, int kv_head, int row) {
     Row r;
     r.valid = row < t.rows;
-    const int i = r.valid ? (int)((uint32_t)row / (uint32_t)group) : 0;
+    const int i = r.valid ? divide(row, g.group) : 0;
     r.token = t.q_begin + i;
-    r.head = kv_head * group + (r.valid ? row - i * group : 0);
+    r.head = kv_head * g.group_size + (r.valid ? row - i * g.group_size : 0);
     const int position = t.kv_len - t.q_len + i;
     r.hi = !r.valid ? 0 : p.causal ? clamp_i(position + 1, 0, t.kv_len) : t.kv_len;
     r.lo = p.window > 0 && position >= p.window ? position - p.window + 1 : 0;
     return r;
 }
 // First and last + 1 key that any of the rows row0 .. row1 sees, and that all of them see.
-__device__ __forceinline__ void span_of(const PagedAttention& p, const Tile& t, int group, int row0, int row1, int& lo, int& hi, int& all_lo, int& all_hi) {
-    const int i0 = (int)((uint32_t)row0 / (uint32_t)group), i1 = (int)((uint32_t)row1 / (uint32_t)group);
+__device__ __forceinline__ void span_of(const PagedAttention& p, const Tile& t, const Plan& g, int row0, int row1, int& lo, int& hi, int& all_lo, int& all_hi) {
+    const int i0 = divide(row0, g.group), i1 = divide(row1, g.group);
     const int position0 = t.kv_len - t.q_len + i0, position1 = t.kv_len - t.q_len + i1;
     lo = p.window > 0 && position0 >= p.window ? position0 - p.window + 1 : 0;
     hi = p.causal ? clamp_i(position1 + 1, 0, t.kv_len) : t.kv_len;
@@ -372,7 +384,7 @@ __device__ __forceinline__ void load_q(const PagedAttention& p, const Row& r, v4
 }
 
 template <int DP, int TYPE>
-__device__ __forceinline__ Pool make_pool(const PagedAttention& p, const Tile& t, int kv_head, uint32_t magic, uint32_t shift) {
+__device__ __forceinline__ Pool make_pool(const PagedAttention& p, const Tile& t, int kv_head, const Plan& g) {
     Pool s;
     s.k = reinterpret_cast<const uint8_t*>(p.k_pages + kv_head * p.kv_stride[2]);
     s.v = reinterpret_cast<const uint8_t*>(p.v_pages + kv_head * p.kv_stride[2]);
@@ -383,43 +395,46 @@ __device__ __forceinline__ Pool make_pool(const PagedAttention& p, const Tile& t
     s.n_pages = (int)p.n_pages;
     s.page_size = p.page_size;
     s.kv_len = t.kv_len;
-    s.magic = magic;
-    s.shift = shift;
+    s.by_page = g.page;
     s.d_chunks = p.D / 8;
     s.neat = p.D == DP && p.page_size % Shape<DP>::PER_COPY == 0;
     return s;
 }
 
 // ---- few rows: the wavefronts of a workgroup, and several workgroups, share the keys of 32 rows --------------------------
-// Each wavefront has two stages of 32 keys in LDS to itself and waits for nobody until the end, where the workgroup's
-// states meet in LDS; with more than one workgroup per tile they leave unnormalised sums for attend_join_kernel.
+// Each wavefront has 32 keys in LDS to itself and waits for nobody until the end: it copies a block, waits, multiplies,
+// copies the next; the others' copies are under way meanwhile (twice as many wavefronts beat two stages for each).  Then the
+// workgroup's states meet in LDS; with more than one workgroup per tile they leave unnormalised sums for
+// attend_join_kernel.
 template <int DP>
 struct SplitShape {
-    static constexpr int WAVES = DP == 256 ? 2 : 4;
+    static constexpr int WAVES = DP == 256 ? 4 : 8;
     static constexpr int STAGE = 2 * 32 * Shape<DP>::ROW;
     static constexpr int OLD = DP + 4;                            // floats of a row of O in LDS
-    static constexpr int WAVE_BYTES = 2 * STAGE > 32 * OLD * 4 ? 2 * STAGE : 32 * OLD * 4;
+    static constexpr int WAVE_BYTES = STAGE > 32 * OLD * 4 ? STAGE : 32 * OLD * 4;
 };
+// How much of a state with maximum m belongs into one with the larger maximum `all` (m = -inf: it has seen nothing, or NaN).
+__device__ __forceinline__ float share(float m, float l, float all) { return m == kNone ? (l != l ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(m - all); }
 
 template <int DP, int TYPE>
-__global__ __launch_bounds__(SplitShape<DP>::WAVES * 64, 1) void attend_split_kernel(const PagedAttention p, int group, uint32_t magic, uint32_t shift,
-                                                                                  float* __restrict__ part, int tiles) {
+__global__ __launch_bounds__(SplitShape<DP>::WAVES * 64, 1) void attend_split_kernel(const PagedAttention p, const Plan g, float* __restrict__ part) {
     using S = Shape<DP>;
     using X = SplitShape<DP>;
     __shared__ __align__(16) uint8_t lds[X::WAVES * X::WAVE_BYTES];
     __shared__ uint32_t ids[X::WAVES][64];
-    __shared__ float ml[X::WAVES][32][2];
+    __shared__ float ml[X::WAVES][32][2], weight[X::WAVES][32];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int tile = blockIdx.x, kv_head = blockIdx.y, z = blockIdx.z, splits = gridDim.z;
+    const int tile = blockIdx.x, kv_head = blockIdx.y, z = blockIdx.z;
     Tile t;
-    if (!locate(p, group, ROWS, tile, t)) return;   // (the same for the whole workgroup)
-    const Row row = row_of(p, t, group, kv_head, t.row0 + (lane & 31));
+    if (!locate(p, g.group_size, ROWS, tile, t)) return;   // (the same for the whole workgroup)
+    const Row row = row_of(p, t, g, kv_head, t.row0 + (lane & 31));
     int lo, hi, all_lo, all_hi;
-    span_of(p, t, group, t.row0, t.row0 + ROWS < t.rows ? t.row0 + ROWS - 1 : t.rows - 1, lo, hi, all_lo, all_hi);
+    span_of(p, t, g, t.row0, t.row0 + ROWS < t.rows ? t.row0 + ROWS - 1 : t.rows - 1, lo, hi, all_lo, all_hi);
     const int b0 = lo / 32, n = (hi + 31) / 32 - b0;   // blocks of 32 keys (none: hi = lo = 0)
-    const int workers = splits * X::WAVES, me = z * X::WAVES + wave;
-    const int begin = b0 + (int)((int64_t)n * me / workers), end = b0 + (int)((int64_t)n * (me + 1) / workers);
-    const Pool pool = make_pool<DP, TYPE>(p, t, kv_head, magic, shift);
+    // even shares, the first ones a block larger
+    const int me = z * X::WAVES + wave, each = divide(n, g.workers), rest = n - each * g.splits * X::WAVES;
+    const int begin = b0 + me * each + (me < rest ? me : rest), end = begin + each + (me < rest ? 1 : 0);
+    const Pool pool = make_pool<DP, TYPE>(p, t, kv_head, g);
     const int32_t* table = p.table + (int64_t)t.b * p.table_ld;
     const float c = p.scale * 1.4426950408889634f;
 
@@ -434,29 +449,24 @@ __global__ __launch_bounds__(SplitShape<DP>::WAVES * 64, 1) void attend_split_ke
     bool special = false;
     if (begin < end) {
         const uint32_t base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)mine), idp = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)ids[wave]);
-        v4i qf[DP / 16];
-        load_q<DP>(p, row, qf);
         volatile uint32_t* my_id = &ids[wave][lane];
         copy_page_id(pool, table, p.table_width, begin * 32 + (lane & 31), idp);
-        for (int blk = begin - 1; blk < end; ++blk) {
-            const int cur = (blk - begin) & 1;
-            // this stage and the next one's page numbers have landed; the other stage has been read
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        v4i qf[DP / 16];
+        load_q<DP>(p, row, qf);
+#pragma unroll 1
+        for (int blk = begin; blk < end; ++blk) {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // the page numbers are there, the block before has been read
+            const int page = (int)*my_id;
+            copy_keys<DP, 32>(pool, page, blk * 32, 0, base, base + 32 * S::ROW);
             if (blk + 1 < end) {
-                const int page = (int)*my_id;
-                const uint32_t to = base + (cur ^ 1) * X::STAGE;
-                copy_keys<DP, 32>(pool, page, (blk + 1) * 32, 0, to, to + 32 * S::ROW);
-                if (blk + 2 < end) {
-                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                    copy_page_id(pool, table, p.table_width, (blk + 2) * 32 + (lane & 31), idp);
-                }
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                copy_page_id(pool, table, p.table_width, (blk + 1) * 32 + (lane & 31), idp);
             }
-            if (blk < begin) continue;
-            uint8_t* k = mine + cur * X::STAGE;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             const int j0 = blk * 32;
-            if (j0 < all_lo || j0 + 32 > all_hi) special |= clean_values<DP, TYPE, 32>(k + 32 * S::ROW);
+            if (j0 < all_lo || j0 + 32 > all_hi) special |= clean_values<DP, TYPE, 32>(mine + 32 * S::ROW);
             const bool whole = !row.valid || (j0 >= row.lo && j0 + 32 <= row.hi);
-            attend_block<DP, TYPE>(st, qf, k, k + 32 * S::ROW, 0, j0, row.lo, row.hi, c, !__all(whole));
+            attend_block<DP, TYPE>(st, qf, mine, mine + 32 * S::ROW, 0, j0, row.lo, row.hi, c, !__all(whole));
         }
     }
     if (special) {
@@ -482,67 +492,96 @@ __global__ __launch_bounds__(SplitShape<DP>::WAVES * 64, 1) void attend_split_ke
         ml[wave][lane][1] = l;
     }
     __syncthreads();
-    const int rows = t.rows - t.row0 < ROWS ? t.rows - t.row0 : ROWS;
-    const int quads = p.D / 4;
-    float* part_o = part + (((int64_t)z * gridDim.y + kv_head) * tiles + tile) * (ROWS * (DP + 2));
-    for (int x = threadIdx.x; x < rows * quads; x += X::WAVES * 64) {
-        const int r = x / quads, d = (x - r * quads) * 4;
-        float m = ml[0][r][0];
+    float* part_o = part + (((int64_t)z * gridDim.y + kv_head) * g.tiles + tile) * (ROWS * (DP + 2));
+    if (threadIdx.x < 32) {
+        // every wavefront's share of a row; divided by the row's sum where nothing else is to be added
+        float m = kNone, sum = 0.f, a[X::WAVES];
 #pragma unroll
-        for (int w = 1; w < X::WAVES; ++w) m = __builtin_fmaxf(m, ml[w][r][0]);
-        float sum = 0.f;
+        for (int w = 0; w < X::WAVES; ++w) m = __builtin_fmaxf(m, ml[w][lane][0]);
+#pragma unroll
+        for (int w = 0; w < X::WAVES; ++w) {
+            a[w] = share(ml[w][lane][0], ml[w][lane][1], m);
+            sum = __builtin_fmaf(ml[w][lane][1], a[w], sum);
+        }
+        const float by = g.splits > 1 ? 1.0f : sum == 0.f ? 0.f : 1.0f / sum;
+#pragma unroll
+        for (int w = 0; w < X::WAVES; ++w) weight[w][lane] = a[w] * by;
+        if (g.splits > 1) {
+            part_o[ROWS * DP + 2 * lane] = m;
+            part_o[ROWS * DP + 2 * lane + 1] = sum;
+        }
+    }
+    __syncthreads();
+    const int rows = t.rows - t.row0 < ROWS ? t.rows - t.row0 : ROWS;
+    for (int x = threadIdx.x; x < rows * (DP / 4); x += X::WAVES * 64) {
+        const int r = x / (DP / 4), d = x % (DP / 4) * 4;
+        if (d >= p.D) continue;
         v4f v = {0, 0, 0, 0};
 #pragma unroll
         for (int w = 0; w < X::WAVES; ++w) {
-            const float mw = ml[w][r][0], a = mw == kNone ? (ml[w][r][1] != ml[w][r][1] ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(mw - m);
+            const float a = weight[w][r];
             const v4f ow = *reinterpret_cast<const v4f*>(reinterpret_cast<const float*>(lds + w * X::WAVE_BYTES) + r * X::OLD + d);
-            sum = __builtin_fmaf(ml[w][r][1], a, sum);
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(ow[e], a, v[e]);
         }
-        if (splits == 1) {
-            const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-            const Row w = row_of(p, t, group, kv_head, t.row0 + r);
-            *reinterpret_cast<uint2*>(p.out + ((int64_t)w.token * p.H + w.head) * p.D + d) =
-                make_uint2(pack2<TYPE>(v[0] * inv, v[1] * inv), pack2<TYPE>(v[2] * inv, v[3] * inv));
-        } else {
+        if (g.splits > 1) {
             *reinterpret_cast<v4f*>(part_o + r * DP + d) = v;
-            if (d == 0) {
-                part_o[ROWS * DP + 2 * r] = m;
-                part_o[ROWS * DP + 2 * r + 1] = sum;
-            }
+        } else {
+            const Row w = row_of(p, t, g, kv_head, t.row0 + r);
+            *reinterpret_cast<uint2*>(p.out + ((int64_t)w.token * p.H + w.head) * p.D + d) = make_uint2(pack2<TYPE>(v[0], v[1]), pack2<TYPE>(v[2], v[3]));
         }
     }
 }
 
-// The workgroups' sums of a tile's rows joined, in the order of the splits.  One lane per four value dims.
+// The workgroups' sums of a tile's rows joined, in the order of the splits.  One lane per four value dims of a row; what each
+// split's share is, the lanes of a wavefront work out one split each.
+constexpr int MAX_SPLITS = 64;
 template <int DP, int TYPE>
-__global__ __launch_bounds__(256) void attend_join_kernel(const PagedAttention p, int group, const float* __restrict__ part, int tiles, int splits) {
+__global__ __launch_bounds__(256) void attend_join_kernel(const PagedAttention p, const Plan g, const float* __restrict__ part) {
     constexpr int QUADS = DP / 4, PER = 256 / QUADS;   // rows of a workgroup
+    __shared__ float weight[PER][MAX_SPLITS];
     const int tile = blockIdx.x, kv_head = blockIdx.y;
     Tile t;
-    if (!locate(p, group, ROWS, tile, t)) return;
-    const int r = blockIdx.z * PER + threadIdx.x / QUADS, d = (threadIdx.x % QUADS) * 4;
-    if (t.row0 + r >= t.rows || d >= p.D) return;
-    const float* all = part + ((int64_t)kv_head * tiles + tile) * (ROWS * (DP + 2));
-    const int64_t step = (int64_t)p.KV * tiles * (ROWS * (DP + 2));
-    float m = kNone, sum = 0.f;
-    v4f v = {0, 0, 0, 0};
-    for (int z = 0; z < splits; ++z) {
-        const float* one = all + z * step;
-        const float mz = one[ROWS * DP + 2 * r], lz = one[ROWS * DP + 2 * r + 1];
-        const v4f oz = *reinterpret_cast<const v4f*>(one + r * DP + d);
-        const float mm = __builtin_fmaxf(m, mz);
-        const float a = m == kNone ? (sum != sum ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(m - mm), b = mz == kNone ? (lz != lz ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(mz - mm);
-        sum = sum * a + lz * b;
+    if (!locate(p, g.group_size, ROWS, tile, t)) return;
+    const int r0 = blockIdx.z * PER, rows = t.rows - t.row0;
+    if (r0 >= rows) return;   // (the whole workgroup)
+    const float* all = part + ((int64_t)kv_head * g.tiles + tile) * (ROWS * (DP + 2));
+    const int64_t step = (int64_t)p.KV * g.tiles * (ROWS * (DP + 2));
+    const int lane = threadIdx.x & 63;
+    for (int i = threadIdx.x >> 6; i < PER; i += 4) {
+        float m = kNone, l = 0.f;
+        if (lane < g.splits && r0 + i < rows) {
+            const float* one = all + lane * step + ROWS * DP + 2 * (r0 + i);
+            m = one[0];
+            l = one[1];
+        }
+        float top = m;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = v[e] * a + oz[e] * b;
-        m = mm;
+        for (int s = 1; s < 64; s <<= 1) top = __builtin_fmaxf(top, __shfl_xor(top, s));
+        const float a = share(m, l, top);
+        float sum = wave_sum_f32(l * a);
+        weight[i][lane] = a * (sum == 0.f ? 0.f : 1.0f / sum);
     }
-    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-    const Row w = row_of(p, t, group, kv_head, t.row0 + r);
-    *reinterpret_cast<uint2*>(p.out + ((int64_t)w.token * p.H + w.head) * p.D + d) =
-        make_uint2(pack2<TYPE>(v[0] * inv, v[1] * inv), pack2<TYPE>(v[2] * inv, v[3] * inv));
+    __syncthreads();
+    const int i = threadIdx.x / QUADS, r = r0 + i, d = (threadIdx.x % QUADS) * 4;
+    if (r >= rows || d >= p.D) return;
+    v4f v = {0, 0, 0, 0};
+    const float* one = all + r * DP + d;
+    for (int z = 0; z < g.splits; z += 8) {
+        v4f o[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o[k] = *reinterpret_cast<const v4f*>(one + (z + k < g.splits ? z + k : z) * step);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float a = z + k < g.splits ? weight[i][z + k] : 0.f;
+            if (a != 0.f) {   // (a split that has seen nothing may have left anything)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(o[k][e], a, v[e]);
+            }
+        }
+    }
+    const Row w = row_of(p, t, g, kv_head, t.row0 + r);
+    *reinterpret_cast<uint2*>(p.out + ((int64_t)w.token * p.H + w.head) * p.D + d) = make_uint2(pack2<TYPE>(v[0], v[1]), pack2<TYPE>(v[2], v[3]));
 }
 
 // ---- many rows: four wavefronts of 32 rows each go through the same keys ----------------------------------------------
@@ -553,7 +592,7 @@ struct ManyShape {
 };
 
 template <int DP, int TYPE>
-__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(const PagedAttention p, int group, uint32_t magic, uint32_t shift) {
+__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(const PagedAttention p, const Plan g) {
     using S = Shape<DP>;
     using X = ManyShape<DP>;
     constexpr int MINE = X::KEYS / X::WAVES;
@@ -563,12 +602,12 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kv_head = blockIdx.y;
     Tile t;
-    if (!locate(p, group, ROWS * X::WAVES, blockIdx.x, t)) return;
-    const Row row = row_of(p, t, group, kv_head, t.row0 + wave * ROWS + (lane & 31));
+    if (!locate(p, g.group_size, ROWS * X::WAVES, blockIdx.x, t)) return;
+    const Row row = row_of(p, t, g, kv_head, t.row0 + wave * ROWS + (lane & 31));
     int lo, hi, all_lo, all_hi;
-    span_of(p, t, group, t.row0, t.row0 + ROWS * X::WAVES < t.rows ? t.row0 + ROWS * X::WAVES - 1 : t.rows - 1, lo, hi, all_lo, all_hi);
+    span_of(p, t, g, t.row0, t.row0 + ROWS * X::WAVES < t.rows ? t.row0 + ROWS * X::WAVES - 1 : t.rows - 1, lo, hi, all_lo, all_hi);
     const int begin = lo / X::KEYS, end = (hi + X::KEYS - 1) / X::KEYS;
-    const Pool pool = make_pool<DP, TYPE>(p, t, kv_head, magic, shift);
+    const Pool pool = make_pool<DP, TYPE>(p, t, kv_head, g);
     const int32_t* table = p.table + (int64_t)t.b * p.table_ld;
     const float c = p.scale * 1.4426950408889634f;
     State<DP> st;
@@ -634,58 +673,48 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
         }
 }
 
-// j / d for 0 <= j < 2^31 by one high product: magic = ceil(2^(31 + l) / d), l = ceil(log2 d) (magic 0: d = 1).
-void division(uint32_t d, uint32_t* magic, uint32_t* shift) {
-    if (d == 1) { *magic = 0; *shift = 0; return; }
+// magic = ceil(2^(31 + l) / d), l = ceil(log2 d)
+Division division(uint32_t d) {
+    if (d == 1) return {0, 0};
     uint32_t l = 1;
     while ((1ull << l) < d) ++l;
-    *magic = (uint32_t)(((1ull << (31 + l)) + d - 1) / d);
-    *shift = l - 1;
+    return {(uint32_t)(((1ull << (31 + l)) + d - 1) / d), l - 1};
 }
 
-struct Plan {
-    bool many;
-    int tiles, splits;
-};
 int padded_dim(int64_t D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 int64_t tiles_bound(int64_t T, int64_t B, int64_t group, int64_t rows) {
     return T * group / rows + (B < T ? B : T);   // every sequence with tokens adds less than one tile of its own
 }
-Plan make_plan(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int64_t max_kv) {
+Plan make_plan(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int64_t max_kv, int64_t page_size) {
     Plan r;
     const int64_t group = H / KV;
+    r.group_size = (int)group;
+    r.page = division((uint32_t)page_size);
+    r.group = division((uint32_t)group);
     const int64_t many = tiles_bound(T, B, group, 128) * KV;
-    r.many = many >= 256 && T * group >= 64 * B;
     const char* forced = tuning_env("PHYAI_LAYER_ATTEND");   // 0: many rows; n: few rows, n splits
-    if (forced != nullptr) r.many = atoi(forced) == 0;
-    if (r.many) {
-        r.tiles = (int)tiles_bound(T, B, group, 128);
-        r.splits = 1;
-        return r;
+    r.many = forced != nullptr ? atoi(forced) == 0 : many >= 256 && T * group >= 64 * B;
+    r.tiles = (int)tiles_bound(T, B, group, r.many ? 128 : ROWS);
+    r.splits = 1;
+    const int waves = padded_dim(D) == 256 ? 4 : 8;
+    if (!r.many) {
+        const int64_t most = (max_kv + 32 * waves - 1) / (32 * waves);
+        int64_t s = (512 + r.tiles * KV - 1) / (r.tiles * KV);
+        s = s < most ? s : most;
+        if (forced != nullptr) s = atoi(forced);
+        r.splits = (int)(s < 1 ? 1 : s < MAX_SPLITS ? s : MAX_SPLITS);
     }
-    r.tiles = (int)tiles_bound(T, B, group, ROWS);
-    const int waves = padded_dim(D) == 256 ? 2 : 4;
-    const int64_t most = (max_kv + 32 * waves - 1) / (32 * waves);
-    int64_t s = (512 + r.tiles * KV - 1) / (r.tiles * KV);
-    s = s < most ? s : most;
-    s = s < 64 ? s : 64;
-    if (forced != nullptr) s = atoi(forced);
-    r.splits = (int)(s < 1 ? 1 : s);
+    r.workers = division((uint32_t)(r.splits * waves));
     return r;
 }
 
 template <int DP, int TYPE>
 hipError_t launch(const PagedAttention& p, const Plan& plan, hipStream_t stream) {
-    uint32_t magic, shift;
-    division((uint32_t)p.page_size, &magic, &shift);
-    const int group = p.H / p.KV;
-    if (plan.many) return enqueue(attend_many_kernel<DP, TYPE>, dim3(plan.tiles, p.KV), dim3(256), stream, p, group, magic, shift);
+    if (plan.many) return enqueue(attend_many_kernel<DP, TYPE>, dim3(plan.tiles, p.KV), dim3(256), stream, p, plan);
     float* part = static_cast<float*>(p.workspace);
-    const hipError_t e = enqueue(attend_split_kernel<DP, TYPE>, dim3(plan.tiles, p.KV, plan.splits), dim3(SplitShape<DP>::WAVES * 64), stream, p, group, magic,
-                       shift, part, plan.tiles);
+    const hipError_t e = enqueue(attend_split_kernel<DP, TYPE>, dim3(plan.tiles, p.KV, plan.splits), dim3(SplitShape<DP>::WAVES * 64), stream, p, plan, part);
     if (e != hipSuccess || plan.splits == 1) return e;
-    return enqueue(attend_join_kernel<DP, TYPE>, dim3(plan.tiles, p.KV, ROWS / (256 / (DP / 4))), dim3(256), stream, p, group, part, plan.tiles,
-                           plan.splits);
+    return enqueue(attend_join_kernel<DP, TYPE>, dim3(plan.tiles, p.KV, ROWS / (256 / (DP / 4))), dim3(256), stream, p, plan, (const float*)part);
 }
 template <int TYPE>
 hipError_t launch_d(const PagedAttention& p, const Plan& plan, hipStream_t stream) {
@@ -700,13 +729,13 @@ hipError_t launch_d(const PagedAttention& p, const Plan& plan, hipStream_t strea
 
 size_t paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int64_t max_kv) {
     if (T <= 0 || B <= 0) return 0;
-    const Plan plan = make_plan(T, B, H, KV, D, max_kv);
+    const Plan plan = make_plan(T, B, H, KV, D, max_kv, 1);
     if (plan.many || plan.splits == 1) return 0;
     return (size_t)plan.splits * KV * plan.tiles * (ROWS * (padded_dim(D) + 2)) * sizeof(float);
 }
 
 hipError_t launch_paged_attention(const PagedAttention& p, hipStream_t stream) {
-    const Plan plan = make_plan(p.T, p.B, p.H, p.KV, p.D, (int64_t)p.table_width * p.page_size);
+    const Plan plan = make_plan(p.T, p.B, p.H, p.KV, p.D, (int64_t)p.table_width * p.page_size, p.page_size);
     return p.type == HEAD_BF16 ? launch_d<HEAD_BF16>(p, plan, stream) : launch_d<HEAD_F16>(p, plan, stream);
 }
 
