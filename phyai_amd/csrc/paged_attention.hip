@@ -20,6 +20,7 @@ namespace {
 
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4s lds_v4s;
+typedef __attribute__((address_space(3))) uint32_t lds_u32;   // (through a generic pointer an access would count as one to memory too)
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v8hf __attribute__((ext_vector_type(8)));
 
@@ -138,66 +139,96 @@ __device__ __forceinline__ void copy16_from(const uint8_t* at, uint32_t lds_wave
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(at), "s"(lds_wave_base) : "memory", "m0");
 }
 
-// What a wavefront needs to bring N keys of a tile (its share): the place of key `row` + lane % N in the pool.
+// Where keys come from, for one sequence and key head.
 struct Pool {
     const uint8_t *k, *v;              // the key head's first element in page 0
     const uint8_t *zero, *nan;
+    const int32_t* table;              // the sequence's pages
     int64_t page_bytes, token_bytes;
-    int n_pages, page_size, kv_len;
+    int n_pages, page_size, kv_len, table_width;
     Division by_page;
     int d_chunks;                      // 16-byte chunks of a key that exist
     bool neat;                         // whole keys of a copy instruction are neighbours in a page
 };
-__device__ __forceinline__ int page_of(const Pool& s, int j) { return divide(j, s.by_page); }
 
-// The page number of key j for every lane, into `slot` (256 bytes of LDS): issued with the copies and counted with them.
-__device__ __forceinline__ void copy_page_id(const Pool& s, const int32_t* table_row, int width, int j, uint32_t slot) {
-    int page = page_of(s, j);
-    page = page < width ? page : width - 1;
-    copy4_to_lds<kBaseSettles>(reinterpret_cast<const uint8_t*>(table_row), (uint32_t)page * 4u, slot);
-}
+// A wavefront's part of bringing blocks `begin`, begin + 1, ... of STEP keys into LDS: N keys of each, from key `row` of the
+// block on.  Its lanes look the places of 64 such keys up at once, those of 64 / N blocks - page number, 64-bit offset,
+// whether it is there at all - so that a block's copies cost little more than themselves (looked up for every block:
+// 1000 cycles where the block's arithmetic takes 1500).  Page numbers go through LDS like the keys, asked for a turn ahead:
+// a load of the compiler's own would wait for all copies in flight.
+template <int DP, int STEP, int N>
+struct Feeder {
+    static constexpr int BLOCKS = 64 / N, PER_COPY = Shape<DP>::PER_COPY, COPIES = N / PER_COPY, ROW = Shape<DP>::ROW;
+    const Pool& s;
+    const int begin, row;
+    lds_u32* const ids;                // two times 64 words of LDS, this wavefront's
+    int lo, hi, kind;                  // of the lane's key: offset, and 0, 1 (beyond the last) or 2 (its page does not exist)
+    uint64_t odd;                      // lanes whose kind is not 0
+    uint32_t k_at, v_at;               // the lane's part of an address: of K and V, copy 0
 
-// Copies keys j0 .. j0 + N - 1 of K and V to rows `row` .. of the tile's buffers; `page` is the number of the page that
-// key j0 + lane % N lies in.
-template <int DP, int N>
-__device__ __forceinline__ void copy_keys(const Pool& s, int page, int j0, int row, uint32_t k_lds, uint32_t v_lds) {
-    using S = Shape<DP>;
-    constexpr int COPIES = N / S::PER_COPY;
-    const int lane = threadIdx.x & 63;
-    const int j = j0 + (lane & (N - 1));
-    const int first = page_of(s, j) * s.page_size;
-    const bool there = j < s.kv_len, good = page >= 0 && page < s.n_pages;
-    const int64_t off = (int64_t)page * s.page_bytes + (int64_t)(j - first) * s.token_bytes;
-    const uint32_t lr = (uint32_t)lane / S::CHUNKS, lc = (uint32_t)lane % S::CHUNKS;
-    if (s.neat && __all(there && good)) {
-        // the swizzles of copy t are those of copy 0 with the bits of t's first key flipped
-        const uint32_t run = lr * (uint32_t)s.token_bytes, kc = (lc ^ k_swizzle<DP>((uint32_t)row + lr)) << 4, vc = (lc ^ v_swizzle<DP>((uint32_t)row + lr)) << 4;
+    __device__ __forceinline__ Feeder(const Pool& pool, int first, int first_row, uint32_t* words)
+        : s(pool), begin(first), row(first_row), ids((lds_u32*)words), lo(0), hi(0), kind(0), odd(0) {
+        const uint32_t lane = threadIdx.x & 63, lr = lane / Shape<DP>::CHUNKS, lc = lane % Shape<DP>::CHUNKS;
+        k_at = (lc ^ k_swizzle<DP>((uint32_t)row + lr)) << 4;
+        v_at = (lc ^ v_swizzle<DP>((uint32_t)row + lr)) << 4;
+    }
+    __device__ __forceinline__ int key(int turn) const {
+        const int lane = threadIdx.x & 63;
+        return (begin + turn * BLOCKS + lane / N) * STEP + row + lane % N;
+    }
+    // The page numbers of a turn of BLOCKS blocks; to be waited for before look().
+    __device__ __forceinline__ void ask(int turn) {
+        int page = divide(key(turn), s.by_page);
+        page = page < s.table_width ? page : s.table_width - 1;
+        copy4_to_lds<kBaseSettles>(reinterpret_cast<const uint8_t*>(s.table), (uint32_t)page * 4u,
+                                   __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(ids + (turn & 1) * 64)));
+    }
+    __device__ __forceinline__ void look(int turn) {
+        const int page = (int)((volatile lds_u32*)ids)[(turn & 1) * 64 + (threadIdx.x & 63)];
+        const int j = key(turn);
+        kind = j >= s.kv_len ? 1 : page < 0 || page >= s.n_pages ? 2 : 0;
+        const int64_t off = (int64_t)page * s.page_bytes + (int64_t)(j - divide(j, s.by_page) * s.page_size) * s.token_bytes;
+        lo = (int)(uint32_t)off;
+        hi = (int)(off >> 32);
+        odd = __ballot(kind != 0);
+    }
+    // Block `blk`, whose turn has been looked up, to the buffers at k_lds and v_lds: 2 COPIES copies.
+    __device__ __forceinline__ void copy(int blk, uint32_t k_lds, uint32_t v_lds) {
+        const int from = ((blk - begin) % BLOCKS) * N;   // the block's first lane
+        if (s.neat && ((odd >> from) & (N == 64 ? ~0ull : (1ull << (N & 63)) - 1)) == 0) {
+            const uint32_t run = ((threadIdx.x & 63) / Shape<DP>::CHUNKS) * (uint32_t)s.token_bytes;
 #pragma unroll
-        for (int t = 0; t < COPIES; ++t) {
-            const uint32_t to = (uint32_t)(row + t * S::PER_COPY) * S::ROW;
-            const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)off, t * S::PER_COPY) |
-                                (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(off >> 32), t * S::PER_COPY) << 32;
-            copy16_to_lds<kBaseSettles>(s.k + at, (kc ^ k_swizzle<DP>(t * S::PER_COPY) << 4) + run, __builtin_amdgcn_readfirstlane(k_lds + to));
-            copy16_to_lds<kBaseSettles>(s.v + at, (vc ^ v_swizzle<DP>(t * S::PER_COPY) << 4) + run, __builtin_amdgcn_readfirstlane(v_lds + to));
+            for (int t = 0; t < COPIES; ++t) {
+                const uint32_t to = (uint32_t)(row + t * PER_COPY) * ROW;
+                const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(lo, from + t * PER_COPY) |
+                                    (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, from + t * PER_COPY) << 32;
+                // (the swizzles of copy t are those of copy 0 with the bits of t's first key flipped)
+                copy16_to_lds<kBaseSettles>(s.k + at, (k_at ^ k_swizzle<DP>(t * PER_COPY) << 4) + run, __builtin_amdgcn_readfirstlane(k_lds + to));
+                copy16_to_lds<kBaseSettles>(s.v + at, (v_at ^ v_swizzle<DP>(t * PER_COPY) << 4) + run, __builtin_amdgcn_readfirstlane(v_lds + to));
+            }
+            return;
         }
-        return;
-    }
-    const int lo = (int)(uint32_t)off, hi = (int)(off >> 32), kind = !there ? 1 : !good ? 2 : 0;
 #pragma unroll 1   // (code that a cold instruction cache does not have to bring: most calls come here once)
-    for (int t = 0; t < COPIES; ++t) {
-        const int from = t * S::PER_COPY + (int)lr;
-        const uint32_t r = (uint32_t)(row + from);
-        const int64_t at = (int64_t)(uint32_t)__shfl(lo, from) | (int64_t)__shfl(hi, from) << 32;
-        const int what = __shfl(kind, from);
-        const uint32_t kc = lc ^ k_swizzle<DP>(r), vc = lc ^ v_swizzle<DP>(r);
-        const uint8_t* fill = what == 2 ? s.nan : s.zero;
-        const uint8_t* ka = what != 0 ? fill : (int)kc < s.d_chunks ? s.k + at + kc * 16 : s.zero;
-        const uint8_t* va = what != 0 ? fill : (int)vc < s.d_chunks ? s.v + at + vc * 16 : s.zero;
-        const uint32_t to = (uint32_t)(row + t * S::PER_COPY) * S::ROW;
-        copy16_from(ka, __builtin_amdgcn_readfirstlane(k_lds + to));
-        copy16_from(va, __builtin_amdgcn_readfirstlane(v_lds + to));
+        for (int t = 0; t < COPIES; ++t) {
+            const int lane = from + t * PER_COPY + (int)(threadIdx.x & 63) / Shape<DP>::CHUNKS;
+            const int64_t at = (int64_t)(uint32_t)__shfl(lo, lane) | (int64_t)__shfl(hi, lane) << 32;
+            const int what = __shfl(kind, lane);
+            const uint32_t kc = k_at ^ k_swizzle<DP>(t * PER_COPY) << 4, vc = v_at ^ v_swizzle<DP>(t * PER_COPY) << 4;
+            const uint8_t* fill = what == 2 ? s.nan : s.zero;
+            const uint8_t* ka = what != 0 ? fill : (int)(kc >> 4) < s.d_chunks ? s.k + at + kc : s.zero;
+            const uint8_t* va = what != 0 ? fill : (int)(vc >> 4) < s.d_chunks ? s.v + at + vc : s.zero;
+            const uint32_t to = (uint32_t)(row + t * PER_COPY) * ROW;
+            copy16_from(ka, __builtin_amdgcn_readfirstlane(k_lds + to));
+            copy16_from(va, __builtin_amdgcn_readfirstlane(v_lds + to));
+        }
     }
-}
+};
+
+// A row of the tile: which token and head it is and which keys it sees.
+struct Row {
+    int token, head, lo, hi;
+    bool valid;
+};
 
 // ---- one block of 32 keys against 32 rows ----------------------------------------------------------------------------
 template <int DP>
@@ -240,12 +271,12 @@ __device__ __forceinline__ bool clean_values(uint8_t* v) {
 }
 // Keys first .. last - 1, from their pages.  (A page that does not exist has made its scores NaN already.)
 template <int DP, int TYPE>
-__device__ __forceinline__ void add_special(State<DP>& st, const Pool& s, const int32_t* table, int first, int last, int d_end, int lo, int hi) {
+__device__ __forceinline__ void add_special(State<DP>& st, const Pool& s, int first, int last, int d_end, int lo, int hi) {
     const int half = (threadIdx.x & 63) >> 5;
     last = last < s.kv_len ? last : s.kv_len;
 #pragma unroll 1
     for (int j = first; j < last; ++j) {
-        const int at = page_of(s, j), page = table[at];
+        const int at = divide(j, s.by_page), page = s.table[at];
         if (page < 0 || page >= s.n_pages) continue;
         const uint8_t* v = s.v + (int64_t)page * s.page_bytes + (int64_t)(j - at * s.page_size) * s.token_bytes;
         const bool sees = j >= lo && j < hi;
@@ -265,55 +296,69 @@ __device__ __forceinline__ void add_special(State<DP>& st, const Pool& s, const 
     }
 }
 
-// kbuf, vbuf: the tile's buffers; row: the block's first key in them; j0: that key's number; the row sees [lo, hi).
-// masked (uniform): some row of the wavefront does not see the whole block.
-template <int DP, int TYPE>
-__device__ __forceinline__ void attend_block(State<DP>& st, const v4i* qf, const uint8_t* kbuf, const uint8_t* vbuf, int row, int j0, int lo, int hi, float c,
-                                             bool masked) {
+// The pieces of a block's work; kbuf, vbuf: the tile's buffers, row: the block's first key in them.
+// Operand K: chunks 2 kk + half of key lane % 32, an xor with a constant below 256 bytes, an offset above.
+template <int DP>
+__device__ __forceinline__ v4i read_k(const uint8_t* kbuf, int row, int kk) {
     using S = Shape<DP>;
-    const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
-    v16f s;
+    const int lane = threadIdx.x & 63;
+    const uint32_t r = (uint32_t)(lane & 31), a0 = r * S::ROW + (((uint32_t)(lane >> 5) ^ k_swizzle<DP>(r)) << 4);
+    return *reinterpret_cast<const v4i*>(kbuf + row * S::ROW + (a0 ^ ((uint32_t)(kk & 7) << 5)) + (kk >> 3) * 256);
+}
+// Operand V^T, value dims 32 b .. and keys 16 e ..: lane (16 g + t) asks for key 4 half + t / 4 of a run of eight and dims 16 (g & 1)
+// + 4 (t & 3) .. and gets four keys of one dim.
+template <int DP>
+__device__ __forceinline__ v4i read_v(const uint8_t* vbuf, int row, int b, int e) {
+    using S = Shape<DP>;
+    const int lane = threadIdx.x & 63;
+    const uint32_t key0 = (uint32_t)(4 * (lane >> 5) + ((lane & 15) >> 2)), chunk0 = (uint32_t)((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+    const uint32_t v0 = key0 * S::ROW + ((chunk0 ^ v_swizzle<DP>(key0)) << 4) + (lane & 1) * 8;
+    const uint8_t* vr = vbuf + row * S::ROW;
+    union { v4s h[2]; v4i v; } f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = 0.f;
-    {
-        // chunk 2 kk + half of the lane's key: an xor with a constant below 256 bytes, an offset above
-        const uint32_t r = (uint32_t)l32, a0 = r * S::ROW + (((uint32_t)half ^ k_swizzle<DP>(r)) << 4);
-        const uint8_t* kr = kbuf + row * S::ROW;
-#pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk) {
-            const v4i a = *reinterpret_cast<const v4i*>(kr + (a0 ^ ((uint32_t)(kk & 7) << 5)) + (kk >> 3) * 256);
-            s = mfma<TYPE>(a, qf[kk], s);
-        }
+    for (int x = 0; x < 2; ++x) {
+        // eight keys further the swizzle has bit 1 of the chunk flipped (two chunks of four bits at DP = 64: none)
+        const uint32_t flip = ((uint32_t)(b & 3) << 6) ^ (DP != 64 && x ? 32u : 0u);
+        f.h[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(vr + (v0 ^ flip) + (16 * e + 8 * x) * S::ROW + (b >> 2) * 256));
     }
-    if (masked) {
+    return f.v;
+}
+__device__ __forceinline__ void mask_scores(v16f& s, int j0, int lo, int hi) {
+    const int half = (threadIdx.x & 63) >> 5;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int j = j0 + 8 * (i >> 2) + 4 * half + (i & 3);
-            s[i] = j >= lo && j < hi ? s[i] : kNone;
-        }
+    for (int i = 0; i < 16; ++i) {
+        const int j = j0 + 8 * (i >> 2) + 4 * half + (i & 3);
+        s[i] = j >= lo && j < hi ? s[i] : kNone;
     }
-    float mx = s[0];
+}
+template <int NB>
+__device__ __forceinline__ float max_score(const v16f (&s)[NB]) {
+    float mx = s[0][0];
 #pragma unroll
-    for (int i = 1; i < 16; ++i) mx = __builtin_fmaxf(mx, s[i]);
-    mx = other_half_max(mx) * c;
-    if (__any(mx > st.m + kRescaleAt)) {
-        const float m = __builtin_fmaxf(st.m, mx);
-        const float a = m == kNone ? 1.0f : __builtin_amdgcn_exp2f(st.m - m);
-        if (__any(st.m != kNone)) {   // (else O and l are zero)
-            st.l *= a;
+    for (int i = 1; i < 16 * NB; ++i) mx = __builtin_fmaxf(mx, s[i / 16][i % 16]);
+    return other_half_max(mx);
+}
+// The row's maximum may have become `mx` (scaled): does any row of the wavefront need its O rescaled, and that.
+__device__ __forceinline__ bool maximum_rises(float m, float mx) { return __any(mx > m + kRescaleAt); }
+template <int DP>
+__device__ __forceinline__ void raise_maximum(State<DP>& st, float mx) {
+    const float m = __builtin_fmaxf(st.m, mx);
+    const float a = m == kNone ? 1.0f : __builtin_amdgcn_exp2f(st.m - m);   // (0 the first time, when O and l are zero)
+    st.l *= a;
 #pragma unroll
-            for (int b = 0; b < DP / 32; ++b)
+    for (int b = 0; b < DP / 32; ++b)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) st.o[b][i] *= a;
-        }
-        st.m = m;
-    }
-    const float base = st.m == kNone ? 0.f : st.m;
+        for (int i = 0; i < 16; ++i) st.o[b][i] *= a;
+    st.m = m;
+}
+// Scores to probabilities, as the second product's operand.  The sum is of the rounded ones, those that the product uses:
+// their common error cancels.
+template <int TYPE>
+__device__ __forceinline__ float probabilities(v16f& s, v4i (&pf)[2], float m, float c) {
+    const float base = m == kNone ? 0.f : m;
+    float sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -base));
-    // the sum is of the rounded probabilities, those that the second product uses: their common error cancels
-    v4i pf[2];
-    float sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -322,32 +367,83 @@ __device__ __forceinline__ void attend_block(State<DP>& st, const v4i* qf, const
             pf[e][i] = (int)w;
             sum[e] = add_pair<TYPE>(w, sum[e]);
         }
-    st.l += sum[0] + sum[1];
-    // V^T: lane (16 g + t) asks for key 4 half + t / 4 of a run of eight and dims 16 (g & 1) + 4 (t & 3) .. of a block of 32
-    const uint32_t key0 = (uint32_t)(4 * half + ((lane & 15) >> 2)), chunk0 = (uint32_t)((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
-    const uint32_t v0 = key0 * S::ROW + ((chunk0 ^ v_swizzle<DP>(key0)) << 4) + (lane & 1) * 8;
-    const uint8_t* vr = vbuf + row * S::ROW;
-    auto read_v = [&](int b, int e) -> v4i {
-        union { v4s h[2]; v4i v; } f;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            // eight keys further the swizzle has bit 1 of the chunk flipped (two chunks of four bits at DP = 64: none)
-            const uint32_t flip = ((uint32_t)(b & 3) << 6) ^ (DP != 64 && x ? 32u : 0u);
-            f.h[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(vr + (v0 ^ flip) + (16 * e + 8 * x) * S::ROW + (b >> 2) * 256));
-        }
-        return f.v;
-    };
-#pragma unroll
-    for (int b = 0; b < DP / 32; ++b)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) st.o[b] = mfma<TYPE>(read_v(b, e), pf[e], st.o[b]);
+    return sum[0] + sum[1];
 }
 
-// A row of the tile: which token and head it is and which keys it sees.
-struct Row {
-    int token, head, lo, hi;
-    bool valid;
-};
+// The keys from 32 NB blk on, NB blocks of 32 a step.  top(step) makes a step's keys available and says where they are (null:
+// no row of the wavefront sees any of it); all rows see whole_lo .. whole_hi.  The loop inside touches O by matrix products
+// alone; a step that raises a maximum leaves it, is finished outside, and the loop goes on behind it.  (With the rescaling
+// inside, 256 dims' O moved from the accumulation registers and back for every block: 256 instructions beside 32 products.)
+template <int DP, int TYPE, int NB, typename Top>
+__device__ __forceinline__ void attend_steps(State<DP>& st, const v4i* qf, int step, int end, const Row& row, int whole_lo, int whole_hi, float c, Top top) {
+    using S = Shape<DP>;
+    // V is read while the scores are turned into probabilities; as much of it as there are registers for
+    constexpr int EARLY = DP == 64 ? 2 : NB == 1 || DP == 256 ? 4 : 2;
+    while (step < end) {
+        v16f s[NB];
+        float mx = kNone;
+        const uint8_t *k = nullptr, *v = nullptr;
+        bool rises = false;
+#pragma unroll 1
+        for (; step < end; ++step) {
+            k = top(step);
+            if (k == nullptr) continue;
+            v = k + NB * 32 * S::ROW;
+            v4i kf[DP / 16], vf[EARLY][2], pf[NB][2];
+            // a block's reads all together, during the products of the one before: left to itself the compiler reads two,
+            // waits, multiplies, and waits again
+#pragma unroll
+            for (int kk = 0; kk < DP / 16; ++kk) kf[kk] = read_k<DP>(k, 0, kk);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[n][i] = 0.f;
+#pragma unroll
+                for (int kk = 0; kk < DP / 16; ++kk) {
+                    s[n] = mfma<TYPE>(kf[kk], qf[kk], s[n]);
+                    if (n + 1 < NB) kf[kk] = read_k<DP>(k, 32 * (n + 1), kk);
+                }
+                if (n + 1 == NB) {
+#pragma unroll
+                    for (int b = 0; b < EARLY; ++b)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) vf[b][e] = read_v<DP>(v, 0, b, e);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            const int j0 = step * (32 * NB);
+            if (j0 < whole_lo || j0 + 32 * NB > whole_hi) {
+#pragma unroll
+                for (int n = 0; n < NB; ++n) mask_scores(s[n], j0 + 32 * n, row.lo, row.hi);
+            }
+            mx = max_score<NB>(s) * c;
+            rises = maximum_rises(st.m, mx);
+            if (rises) break;
+#pragma unroll
+            for (int n = 0; n < NB; ++n) st.l += probabilities<TYPE>(s[n], pf[n], st.m, c);
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) st.o[b] = mfma<TYPE>(n == 0 && b < EARLY ? vf[b % EARLY][e] : read_v<DP>(v, 32 * n, b, e), pf[n][e], st.o[b]);
+        }
+        if (!rises) break;
+        raise_maximum<DP>(st, mx);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            v4i pf[2];
+            st.l += probabilities<TYPE>(s[n], pf, st.m, c);
+#pragma unroll
+            for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) st.o[b] = mfma<TYPE>(read_v<DP>(v, 32 * n, b, e), pf[e], st.o[b]);
+        }
+        ++step;
+    }
+}
+
 __device__ __forceinline__ Row row_of(const PagedAttention& p, const Tile& t, const Plan& g, int kv_head, int row) {
     Row r;
     r.valid = row < t.rows;
@@ -396,6 +492,8 @@ __device__ __forceinline__ Pool make_pool(const PagedAttention& p, const Tile& t
     s.page_size = p.page_size;
     s.kv_len = t.kv_len;
     s.by_page = g.page;
+    s.table = p.table + (int64_t)t.b * p.table_ld;
+    s.table_width = p.table_width;
     s.d_chunks = p.D / 8;
     s.neat = p.D == DP && p.page_size % Shape<DP>::PER_COPY == 0;
     return s;
@@ -421,7 +519,7 @@ __global__ __launch_bounds__(SplitShape<DP>::WAVES * 64, 1) void attend_split_ke
     using S = Shape<DP>;
     using X = SplitShape<DP>;
     __shared__ __align__(16) uint8_t lds[X::WAVES * X::WAVE_BYTES];
-    __shared__ uint32_t ids[X::WAVES][64];
+    __shared__ uint32_t ids[X::WAVES][2][64];
     __shared__ float ml[X::WAVES][32][2], weight[X::WAVES][32];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tile = blockIdx.x, kv_head = blockIdx.y, z = blockIdx.z;
@@ -435,7 +533,6 @@ __global__ __launch_bounds__(SplitShape<DP>::WAVES * 64, 1) void attend_split_ke
     const int me = z * X::WAVES + wave, each = divide(n, g.workers), rest = n - each * g.splits * X::WAVES;
     const int begin = b0 + me * each + (me < rest ? me : rest), end = begin + each + (me < rest ? 1 : 0);
     const Pool pool = make_pool<DP, TYPE>(p, t, kv_head, g);
-    const int32_t* table = p.table + (int64_t)t.b * p.table_ld;
     const float c = p.scale * 1.4426950408889634f;
 
     State<DP> st;
@@ -448,31 +545,27 @@ __global__ __launch_bounds__(SplitShape<DP>::WAVES * 64, 1) void attend_split_ke
     uint8_t* mine = lds + wave * X::WAVE_BYTES;
     bool special = false;
     if (begin < end) {
-        const uint32_t base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)mine), idp = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)ids[wave]);
-        volatile uint32_t* my_id = &ids[wave][lane];
-        copy_page_id(pool, table, p.table_width, begin * 32 + (lane & 31), idp);
+        const uint32_t base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)mine);
+        Feeder<DP, 32, 32> feed(pool, begin, 0, ids[wave][0]);
+        constexpr int TURN = Feeder<DP, 32, 32>::BLOCKS;
+        feed.ask(0);
         v4i qf[DP / 16];
         load_q<DP>(p, row, qf);
-#pragma unroll 1
-        for (int blk = begin; blk < end; ++blk) {
+        attend_steps<DP, TYPE, 1>(st, qf, begin, end, row, all_lo, all_hi, c, [&](int blk) -> const uint8_t* {
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // the page numbers are there, the block before has been read
-            const int page = (int)*my_id;
-            copy_keys<DP, 32>(pool, page, blk * 32, 0, base, base + 32 * S::ROW);
-            if (blk + 1 < end) {
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                copy_page_id(pool, table, p.table_width, (blk + 1) * 32 + (lane & 31), idp);
-            }
+            const int turn = (blk - begin) / TURN;
+            if ((blk - begin) % TURN == 0) feed.look(turn);
+            feed.copy(blk, base, base + 32 * S::ROW);
+            if ((blk - begin) % TURN == 0 && blk + TURN < end) feed.ask(turn + 1);
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            const int j0 = blk * 32;
-            if (j0 < all_lo || j0 + 32 > all_hi) special |= clean_values<DP, TYPE, 32>(mine + 32 * S::ROW);
-            const bool whole = !row.valid || (j0 >= row.lo && j0 + 32 <= row.hi);
-            attend_block<DP, TYPE>(st, qf, mine, mine + 32 * S::ROW, 0, j0, row.lo, row.hi, c, !__all(whole));
-        }
+            if (blk * 32 < all_lo || blk * 32 + 32 > all_hi) special |= clean_values<DP, TYPE, 32>(mine + 32 * S::ROW);
+            return mine;
+        });
     }
     if (special) {
 #pragma unroll 1
         for (int blk = begin; blk < end; ++blk)
-            if (blk * 32 < all_lo || blk * 32 + 32 > all_hi) add_special<DP, TYPE>(st, pool, table, blk * 32, blk * 32 + 32, p.D, row.lo, row.hi);
+            if (blk * 32 < all_lo || blk * 32 + 32 > all_hi) add_special<DP, TYPE>(st, pool, blk * 32, blk * 32 + 32, p.D, row.lo, row.hi);
     }
     // the wavefronts' states meet
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -585,30 +678,34 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const PagedAttention p
 }
 
 // ---- many rows: four wavefronts of 32 rows each go through the same keys ----------------------------------------------
+// A step of 64 keys at a time, the next one on its way to LDS meanwhile; a wait for the wavefront's own copies and a barrier a
+// step.  Bound by the issue of instructions: two wavefronts a SIMD, of which each has 130 vector and 86 scalar ones beside 16
+// products for 32 keys when it takes those at a time (four such steps in LDS: 316 us for 2048 tokens of 32 heads of 128
+// dims over 8192 keys, 84 us for 16 x 816 of 8 heads of 256 over 816), and far fewer for 64 (270 and 77).
 template <int DP>
 struct ManyShape {
-    static constexpr int WAVES = 4, KEYS = DP == 256 ? 32 : 64;
-    static constexpr int STAGE = 2 * KEYS * Shape<DP>::ROW;
+    static constexpr int WAVES = 4, STEP = 64, MINE = STEP / WAVES, STAGE = 2 * STEP * Shape<DP>::ROW;
 };
 
 template <int DP, int TYPE>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(const PagedAttention p, const Plan g) {
     using S = Shape<DP>;
     using X = ManyShape<DP>;
-    constexpr int MINE = X::KEYS / X::WAVES;
     __shared__ __align__(16) uint8_t lds[2 * X::STAGE];
-    __shared__ uint32_t ids[X::WAVES][64];
+    __shared__ uint32_t ids[X::WAVES][2][64];
     __shared__ int specials[X::WAVES];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kv_head = blockIdx.y;
     Tile t;
     if (!locate(p, g.group_size, ROWS * X::WAVES, blockIdx.x, t)) return;
-    const Row row = row_of(p, t, g, kv_head, t.row0 + wave * ROWS + (lane & 31));
-    int lo, hi, all_lo, all_hi;
-    span_of(p, t, g, t.row0, t.row0 + ROWS * X::WAVES < t.rows ? t.row0 + ROWS * X::WAVES - 1 : t.rows - 1, lo, hi, all_lo, all_hi);
-    const int begin = lo / X::KEYS, end = (hi + X::KEYS - 1) / X::KEYS;
+    const int row0 = t.row0 + wave * ROWS, row_last = t.rows - 1;
+    const Row row = row_of(p, t, g, kv_head, row0 + (lane & 31));
+    int lo, hi, all_lo, all_hi;          // of the workgroup
+    span_of(p, t, g, t.row0, t.row0 + ROWS * X::WAVES - 1 < row_last ? t.row0 + ROWS * X::WAVES - 1 : row_last, lo, hi, all_lo, all_hi);
+    int my_lo = 0, my_hi = 0, whole_lo = 0, whole_hi = 0;   // of the wavefront
+    if (row0 <= row_last) span_of(p, t, g, row0, row0 + ROWS - 1 < row_last ? row0 + ROWS - 1 : row_last, my_lo, my_hi, whole_lo, whole_hi);
+    const int begin = lo / X::STEP, end = (hi + X::STEP - 1) / X::STEP;
     const Pool pool = make_pool<DP, TYPE>(p, t, kv_head, g);
-    const int32_t* table = p.table + (int64_t)t.b * p.table_ld;
     const float c = p.scale * 1.4426950408889634f;
     State<DP> st;
     st.m = kNone;
@@ -617,46 +714,43 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
     for (int b = 0; b < DP / 32; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i) st.o[b][i] = 0.f;
+    const uint32_t base = (uint32_t)(uintptr_t)lds;
+    using Feed = Feeder<DP, X::STEP, X::MINE>;
+    Feed feed(pool, begin, wave * X::MINE, ids[wave][0]);
+    auto copy = [&](int step) {
+        const int at = step - begin;
+        if (at % Feed::BLOCKS == 0) {
+            feed.look(at / Feed::BLOCKS);
+            if (step + Feed::BLOCKS < end) feed.ask(at / Feed::BLOCKS + 1);
+        }
+        const uint32_t to = base + (uint32_t)(at & 1) * X::STAGE;
+        feed.copy(step, to, to + X::STEP * S::ROW);
+    };
     v4i qf[DP / 16];
     load_q<DP>(p, row, qf);
-    const uint32_t base = (uint32_t)(uintptr_t)lds, idp = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)ids[wave]);
-    volatile uint32_t* my_id = &ids[wave][lane];
-    const int ahead = wave * MINE + (lane & (MINE - 1));   // the key of a tile whose page this lane looks up
-    if (begin < end) copy_page_id(pool, table, p.table_width, begin * X::KEYS + ahead, idp);
     bool special = false;
-    for (int blk = begin - 1; blk < end; ++blk) {
-        const int cur = (blk - begin) & 1;
-        // this tile and the next one's page numbers have landed; behind the barrier the other stage has been read
+    if (begin < end) {
+        feed.ask(0);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        if (blk >= begin && (blk * X::KEYS < all_lo || (blk + 1) * X::KEYS > all_hi))
-            special |= clean_values<DP, TYPE, MINE>(lds + cur * X::STAGE + (X::KEYS + wave * MINE) * S::ROW);
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (blk + 1 < end) {
-            const int page = (int)*my_id;
-            const uint32_t to = base + (cur ^ 1) * X::STAGE;
-            copy_keys<DP, MINE>(pool, page, (blk + 1) * X::KEYS + wave * MINE, wave * MINE, to, to + X::KEYS * S::ROW);
-            if (blk + 2 < end) {
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                copy_page_id(pool, table, p.table_width, (blk + 2) * X::KEYS + ahead, idp);
-            }
-        }
-        if (blk < begin) continue;
-        const uint8_t* k = lds + cur * X::STAGE;
-#pragma unroll
-        for (int x = 0; x < X::KEYS / 32; ++x) {
-            const int j0 = blk * X::KEYS + x * 32;
-            const bool whole = !row.valid || (j0 >= row.lo && j0 + 32 <= row.hi), none = j0 >= row.hi || j0 + 32 <= row.lo;
-            if (__all(none)) continue;
-            attend_block<DP, TYPE>(st, qf, k, k + X::KEYS * S::ROW, x * 32, j0, row.lo, row.hi, c, !__all(whole));
-        }
+        copy(begin);
     }
+    attend_steps<DP, TYPE, X::STEP / 32>(st, qf, begin, end, row, whole_lo, whole_hi, c, [&](int step) -> const uint8_t* {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this step has landed; behind the barrier everybody has read the one before it
+        uint8_t* k = lds + (uint32_t)((step - begin) & 1) * X::STAGE;
+        const int j0 = step * X::STEP;
+        if (j0 < all_lo || j0 + X::STEP > all_hi) special |= clean_values<DP, TYPE, X::MINE>(k + (X::STEP + wave * X::MINE) * S::ROW);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (step + 1 < end) copy(step + 1);
+        return j0 >= my_hi || j0 + X::STEP <= my_lo ? nullptr : k;
+    });
     if (lane == 0) specials[wave] = special ? 1 : 0;
     __syncthreads();
     if ((specials[0] | specials[1] | specials[2] | specials[3]) != 0) {
 #pragma unroll 1
-        for (int blk = begin; blk < end; ++blk)
-            if (blk * X::KEYS < all_lo || (blk + 1) * X::KEYS > all_hi)
-                add_special<DP, TYPE>(st, pool, table, blk * X::KEYS, (blk + 1) * X::KEYS, p.D, row.lo, row.hi);
+        for (int step = begin; step < end; ++step) {
+            const int j0 = step * X::STEP;
+            if (j0 < all_lo || j0 + X::STEP > all_hi) add_special<DP, TYPE>(st, pool, j0, j0 + X::STEP, p.D, row.lo, row.hi);
+        }
     }
     const float l = other_half_sum(st.l);
     const float inv = l == 0.f ? 0.f : 1.0f / l;
@@ -691,15 +785,20 @@ Plan make_plan(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int64_t m
     r.group_size = (int)group;
     r.page = division((uint32_t)page_size);
     r.group = division((uint32_t)group);
+    // Many rows a workgroup once there are workgroups for most of the chip and rows enough to fill them.  Measured, many
+    // against few: 128 workgroups of 256 dims 83 and 71 us, 816 of them 77 and 149; 128 of 128 dims 217 and 135, 256 of them
+    // 37 and 51; 512 of 64 dims (two to four fit a CU) 30.2 and 31.
+    const int DP = padded_dim(D), waves = DP == 256 ? 4 : 8;
     const int64_t many = tiles_bound(T, B, group, 128) * KV;
     const char* forced = tuning_env("PHYAI_LAYER_ATTEND");   // 0: many rows; n: few rows, n splits
-    r.many = forced != nullptr ? atoi(forced) == 0 : many >= 256 && T * group >= 64 * B;
+    r.many = forced != nullptr ? atoi(forced) == 0 : many >= (DP == 64 ? 512 : 192) && T * group >= 64 * B;
     r.tiles = (int)tiles_bound(T, B, group, r.many ? 128 : ROWS);
     r.splits = 1;
-    const int waves = padded_dim(D) == 256 ? 4 : 8;
     if (!r.many) {
-        const int64_t most = (max_kv + 32 * waves - 1) / (32 * waves);
-        int64_t s = (512 + r.tiles * KV - 1) / (r.tiles * KV);
+        // As many splits as workgroups run at once, and no more than give every wavefront a block: 32 tiles of 4096 keys 34 us
+        // in one split, 18.5 in seven; 200 tiles of 816 keys 27.6 in one, 46 in two.
+        const int64_t most = (max_kv + 32 * waves - 1) / (32 * waves), tiles = r.tiles * KV, at_once = DP == 64 ? 512 : 256;
+        int64_t s = at_once / tiles;
         s = s < most ? s : most;
         if (forced != nullptr) s = atoi(forced);
         r.splits = (int)(s < 1 ? 1 : s < MAX_SPLITS ? s : MAX_SPLITS);
