@@ -14,7 +14,7 @@ from __future__ import annotations
 
 from phyai_amd.linear.backend import Granularity, KernelProbe, LinearKernel
 from phyai_amd.linear.dispatch import KernelDispatcher, _set_linear_dispatcher, get_linear_dispatcher
-from phyai_amd.linear.kernels import HipFp8Kernel, TorchBf16Kernel
+from phyai_amd.linear.kernels import HipFp8BlockKernel, HipFp8Kernel, TorchBf16Kernel
 from phyai_amd.linear.layers import (
     ColumnParallelLinear,
     LinearBase,
@@ -38,7 +38,8 @@ from phyai_amd.utils import sm_arch
 def supported_specs_for_sm(sm: int) -> list[str]:
     """Specs ``validate()`` must find a kernel for on this device: bf16 everywhere,
     per-tensor / per-channel fp8 where the device reports capability >= 89
-    (reference ``__init__.py:54-79``; gfx950 reports 95)."""
+    (reference ``__init__.py:54-79``; gfx950 reports 95).  ``fp8_block_128_128`` has a kernel there too; as in the reference
+    it is not among the specs that a start-up insists on."""
     specs = ["bf16"]
     if sm >= 89:
         specs += ["fp8_per_tensor", "fp8_per_channel"]
@@ -70,5 +71,5 @@ __all__ = [
     "Bf16Spec", "Fp8Spec", "ActivationView", "AllocationRequest", "WeightSpec", "Granularity",
     "KernelDispatcher", "get_linear_dispatcher", "LinearKernelRegistry", "DefaultPolicy", "ForcedPolicy",
     "Policy", "LinearKernel", "KernelProbe", "register_linear_kernel", "list_registered_linear_kernels",
-    "HipFp8Kernel", "TorchBf16Kernel",
+    "HipFp8Kernel", "HipFp8BlockKernel", "TorchBf16Kernel",
 ]

@@ -6,6 +6,9 @@ graph capture, and runs it as one C-ABI call (row-wise quantizer + fp8 MFMA GEMM
 with the scale/bias epilogue).  It replaces ``TorchKernel._fp8_per_channel`` and
 ``_fp8_per_tensor`` of the reference (``layers/linear/backends/torch.py:123-176``).
 
+``HipFp8BlockKernel`` ("hip_fp8_block") takes ``fp8_block_128_128`` linears: weights with one scale per
+128 x 128 block, activations quantized per token and 128 elements of it.
+
 ``TorchBf16Kernel`` ("torch") only covers unquantized bf16 weights through
 ``F.linear``, as the reference's always-present fallback does for that spec
 (``backends/torch.py:82-83,110-111``).  It never handles an fp8 spec: there is no
@@ -93,3 +96,34 @@ class TorchBf16Kernel:
         if layer.spec.spec_id != "bf16":
             raise RuntimeError(f"TorchBf16Kernel got unhandled spec_id={layer.spec.spec_id!r}")
         return F.linear(x, layer.weight, bias)
+
+
+_BLOCK_SPEC = "fp8_block_128_128"
+
+
+@register_linear_kernel(prefer_for={(_BLOCK_SPEC, r) for r in ("prefill", "decode")})
+class HipFp8BlockKernel:
+    name = "hip_fp8_block"
+
+    def supports_capture(self) -> bool:
+        # As HipFp8Kernel: its workspace is the graph's own, nothing is synchronised or compiled lazily.
+        return True
+
+    def can_handle(self, probe: KernelProbe) -> bool:
+        if probe.spec_id != _BLOCK_SPEC or probe.sm < _MIN_SM:
+            return False
+        if probe.in_dtype != torch.bfloat16 or probe.out_dtype != torch.bfloat16:
+            return False
+        return probe.K % 16 == 0 and probe.N % 16 == 0
+
+    def apply(self, layer: torch.nn.Module, x: torch.Tensor, bias: torch.Tensor | None) -> torch.Tensor:
+        """bf16 ``x`` is quantized per token and block of 128 on the way; an ``ActivationView`` brings its codes, with a
+        scale per token (from a norm with the quantizer in it, or ``spec.quantize_activation``) or per token and block."""
+        if layer.spec.spec_id != _BLOCK_SPEC:
+            raise RuntimeError(f"HipFp8BlockKernel got unhandled spec_id={layer.spec.spec_id!r}")
+        if isinstance(x, ActivationView):
+            if x.granularity is Granularity.PER_TENSOR or x.x_scale is None:
+                raise RuntimeError(f"HipFp8BlockKernel: pre-quantized activations need scales per token or per token and "
+                                   f"block, got granularity={x.granularity}")
+            return ops.fp8_block_gemm(x.x, x.x_scale, layer.weight, layer.weight_scale, bias)
+        return ops.fp8_block_linear(x, layer.weight, layer.weight_scale, bias)

@@ -119,7 +119,11 @@ class LinearBase(nn.Module):
             if isinstance(p, nn.Parameter):
                 p.hf_keys = [(f"{base}.{name}", sid) for base, sid in legs]
                 p.optional = True
-                if not fused:
+                if p.dim() == 2:
+                    # one scale per block of the weight; checkpoints call it weight_scale or weight_scale_inv, of the same meaning
+                    p.hf_keys += [(f"{base}.{name}_inv", sid) for base, sid in legs]
+                    p.weight_loader = W.fused_blocks(offsets, self.output_size_per_partition // p.shape[0]) if fused else W.replicated()
+                elif not fused:
                     p.weight_loader = W.replicated()
                 elif p.shape[0] == self.output_size_per_partition:
                     p.weight_loader = rows                                    # one scale per output row

@@ -48,7 +48,8 @@ class Fp8Spec:
       after loading) and one static activation scale.
     * ``PER_CHANNEL``: fp32 scale per output row; activations are quantized per
       token at run time.  This is the format the HIP kernels are built for.
-    * ``BLOCK``: ``[N/bn, K/bk]`` weight scales (storage only here).
+    * ``BLOCK``: ``[N/bn, K/bk]`` weight scales.  A layer with blocks of 128 x 128 runs: activations are quantized
+      per token and 128 elements of it (``ops.fp8_block_linear``).  Other shapes are storage only.
     """
 
     granularity: Granularity = Granularity.PER_CHANNEL

@@ -10,9 +10,10 @@ final adaptive norm, action projection, ``x_t <- x_t + dt * v_t`` (``:689-738``)
 
 What is NOT mirrored is the reference's attention back end (paged KV pool, flashinfer planning):
 attention is a callback ``attend(fused_qkv, layer_index) -> [M, heads * head_dim]``.
-:class:`PrefixAttentionStandIn` is a plain-torch one (RoPE + SDPA over a fixed prefix KV plus the
-chunk's own keys and values) so that data really chains through the layers; it is a stand-in,
-not a kernel of this package.
+:class:`phyai_amd.runtime.PagedPrefixAttention` is the one on this library's kernels (rotation and
+cache write, then attention over pages).  :class:`PrefixAttentionStandIn` is a plain-torch one (RoPE +
+SDPA over a fixed prefix KV plus the chunk's own keys and values); it is a stand-in, not a kernel of
+this package.
 
 Three forms of the layer run on the same weights:
 
@@ -42,6 +43,7 @@ from phyai_amd.linear import QKVParallelLinear, ReplicatedLinear, RowParallelLin
 from phyai_amd.mlp import DenseMLP
 from phyai_amd.norm import AdaRMSNorm
 from phyai_amd.quant import Fp8Spec
+from phyai_amd.quant.types import Granularity
 from phyai_amd.runtime.graph import HipGraph
 
 VARIANTS = ("fused", "unfused", "torch")
@@ -105,6 +107,10 @@ class ExpertLayer(nn.Module):
             out = self._three_calls(h, attend, index, modulation)
             if out is not None:
                 return out
+            if any(getattr(getattr(lin, "spec", None), "granularity", None) is Granularity.BLOCK
+                   for lin in (self.qkv_proj, self.o_proj, self.mlp.gate_up_proj, self.mlp.down_proj)):
+                # weights with scales per block: their linears take bf16 (quantized per token and block) and have no fused epilogue
+                return self.forward(h, attend, index, modulation, "unfused")
             view, gate_attn = self.input_layernorm.forward_fp8(h, modulation=modulation.input_ln)
             fused, _ = self.qkv_proj(view)
             h = self.o_proj.forward_addcmul(attend(fused, index), residual, gate_attn)

@@ -69,6 +69,24 @@ def fused_rows(legs: dict) -> WeightLoader:
     return load
 
 
+def fused_blocks(legs: dict, block: int) -> WeightLoader:
+    """As :func:`fused_rows` for scales per block of ``block`` rows, ``[N / block, K / ...]``: every leg has to be whole
+    blocks, since a block's scale serves rows of one checkpoint tensor only."""
+
+    def load(param: nn.Parameter, loaded: torch.Tensor, shard_id) -> None:
+        if shard_id not in legs:
+            raise KeyError(f"fused parameter has no leg {shard_id!r} (legs: {sorted(map(str, legs))})")
+        off, size = legs[shard_id]
+        if off % block or size % block:
+            raise ValueError(f"leg {shard_id!r}: rows {off} to {off + size} of the fused weight are not whole blocks of {block}")
+        want = (size // block, param.shape[1])
+        if tuple(loaded.shape) != want:
+            raise ValueError(f"leg {shard_id!r}: scales {tuple(loaded.shape)} in the checkpoint, {want} in the layer")
+        param.data.narrow(0, off // block, want[0]).copy_(_as_param_dtype(loaded, param))
+
+    return load
+
+
 def leg_slots(order: list) -> WeightLoader:
     """One scalar per leg into a ``[legs]`` parameter (per-tensor fp8 scales of a fused layer, fanned
     out to rows by the spec's ``process_after_loading``, reference ``quant/fp8.py:36-43,128-135``)."""
@@ -190,4 +208,4 @@ def load_pretrained(model: nn.Module, source: "str | Path | Iterable[str | Path]
     return report
 
 
-__all__ = ["WeightLoader", "replicated", "fused_rows", "leg_slots", "LoadReport", "load_pretrained"]
+__all__ = ["WeightLoader", "replicated", "fused_rows", "fused_blocks", "leg_slots", "LoadReport", "load_pretrained"]
