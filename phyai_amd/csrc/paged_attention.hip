@@ -162,35 +162,37 @@ struct Feeder {
     const Pool& s;
     const int begin, row;
     lds_u32* const ids;                // two times 64 words of LDS, this wavefront's
-    int lo, hi, kind;                  // of the lane's key: offset, and 0, 1 (beyond the last) or 2 (its page does not exist)
-    uint64_t odd;                      // lanes whose kind is not 0
+    int lo, hi, gone;                  // of the lane's key: its offset; its page does not exist
+    uint64_t odd;                      // lanes whose key is gone
     uint32_t k_at, v_at;               // the lane's part of an address: of K and V, copy 0
 
     __device__ __forceinline__ Feeder(const Pool& pool, int first, int first_row, uint32_t* words)
-        : s(pool), begin(first), row(first_row), ids((lds_u32*)words), lo(0), hi(0), kind(0), odd(0) {
+        : s(pool), begin(first), row(first_row), ids((lds_u32*)words), lo(0), hi(0), gone(0), odd(0) {
         const uint32_t lane = threadIdx.x & 63, lr = lane / Shape<DP>::CHUNKS, lc = lane % Shape<DP>::CHUNKS;
         k_at = (lc ^ k_swizzle<DP>((uint32_t)row + lr)) << 4;
         v_at = (lc ^ v_swizzle<DP>((uint32_t)row + lr)) << 4;
     }
+    // The lane's key.  In the place of one beyond the last, the first of the last key's copy: no row sees what is copied
+    // there, it only has to be in the cache, like all keys of that copy (filled with zeros instead, by lanes that each have an
+    // address of their own, a block took 3 us longer at 256 dims).
     __device__ __forceinline__ int key(int turn) const {
-        const int lane = threadIdx.x & 63;
-        return (begin + turn * BLOCKS + lane / N) * STEP + row + lane % N;
+        const int lane = threadIdx.x & 63, j = (begin + turn * BLOCKS + lane / N) * STEP + row + lane % N;
+        return j < s.kv_len ? j : (s.kv_len - 1) & ~(PER_COPY - 1);
     }
     // The page numbers of a turn of BLOCKS blocks; to be waited for before look().
     __device__ __forceinline__ void ask(int turn) {
-        int page = divide(key(turn), s.by_page);
-        page = page < s.table_width ? page : s.table_width - 1;
+        const int page = divide(key(turn), s.by_page);
         copy4_to_lds<kBaseSettles>(reinterpret_cast<const uint8_t*>(s.table), (uint32_t)page * 4u,
                                    __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(ids + (turn & 1) * 64)));
     }
     __device__ __forceinline__ void look(int turn) {
         const int page = (int)((volatile lds_u32*)ids)[(turn & 1) * 64 + (threadIdx.x & 63)];
         const int j = key(turn);
-        kind = j >= s.kv_len ? 1 : page < 0 || page >= s.n_pages ? 2 : 0;
+        gone = page < 0 || page >= s.n_pages;
         const int64_t off = (int64_t)page * s.page_bytes + (int64_t)(j - divide(j, s.by_page) * s.page_size) * s.token_bytes;
         lo = (int)(uint32_t)off;
         hi = (int)(off >> 32);
-        odd = __ballot(kind != 0);
+        odd = __ballot(gone);
     }
     // Block `blk`, whose turn has been looked up, to the buffers at k_lds and v_lds: 2 COPIES copies.
     __device__ __forceinline__ void copy(int blk, uint32_t k_lds, uint32_t v_lds) {
@@ -212,11 +214,10 @@ struct Feeder {
         for (int t = 0; t < COPIES; ++t) {
             const int lane = from + t * PER_COPY + (int)(threadIdx.x & 63) / Shape<DP>::CHUNKS;
             const int64_t at = (int64_t)(uint32_t)__shfl(lo, lane) | (int64_t)__shfl(hi, lane) << 32;
-            const int what = __shfl(kind, lane);
+            const int none = __shfl(gone, lane);
             const uint32_t kc = k_at ^ k_swizzle<DP>(t * PER_COPY) << 4, vc = v_at ^ v_swizzle<DP>(t * PER_COPY) << 4;
-            const uint8_t* fill = what == 2 ? s.nan : s.zero;
-            const uint8_t* ka = what != 0 ? fill : (int)(kc >> 4) < s.d_chunks ? s.k + at + kc : s.zero;
-            const uint8_t* va = what != 0 ? fill : (int)(vc >> 4) < s.d_chunks ? s.v + at + vc : s.zero;
+            const uint8_t* ka = (int)(kc >> 4) >= s.d_chunks ? s.zero : none ? s.nan : s.k + at + kc;
+            const uint8_t* va = (int)(vc >> 4) >= s.d_chunks ? s.zero : none ? s.nan : s.v + at + vc;
             const uint32_t to = (uint32_t)(row + t * PER_COPY) * ROW;
             copy16_from(ka, __builtin_amdgcn_readfirstlane(k_lds + to));
             copy16_from(va, __builtin_amdgcn_readfirstlane(v_lds + to));
@@ -250,10 +251,10 @@ __device__ __forceinline__ uint32_t without_special(uint32_t w) {
     return w;
 }
 // A probability of zero times an infinity or a NaN is a NaN.  In a tile that some rows see only part of, such values are
-// taken out of V as it lands (each wavefront looks through the keys it has copied itself; true if there were any), and
-// add_special gives them to the rows that see their key after the last tile.
+// taken out of V as it lands (each wavefront looks through the `keys` keys it has copied itself and whatever lies behind them;
+// true if there were any among the keys), and add_special gives them to the rows that see their key after the last tile.
 template <int DP, int TYPE, int N>
-__device__ __forceinline__ bool clean_values(uint8_t* v) {
+__device__ __forceinline__ bool clean_values(uint8_t* v, int keys) {
     bool special = false;
 #pragma unroll 1
     for (int x = (threadIdx.x & 63) * 16; x < N * Shape<DP>::ROW; x += 1024) {
@@ -265,7 +266,7 @@ __device__ __forceinline__ bool clean_values(uint8_t* v) {
             f[i] = (int)without_special<TYPE>((uint32_t)f[i]);
         }
         if (any) *reinterpret_cast<v4i*>(v + x) = f;
-        special |= any;
+        special |= any && x / Shape<DP>::ROW < keys;
     }
     return __any(special);
 }
@@ -558,7 +559,7 @@ __global__ __launch_bounds__(SplitShape<DP>::WAVES * 64, 1) void attend_split_ke
             feed.copy(blk, base, base + 32 * S::ROW);
             if ((blk - begin) % TURN == 0 && blk + TURN < end) feed.ask(turn + 1);
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            if (blk * 32 < all_lo || blk * 32 + 32 > all_hi) special |= clean_values<DP, TYPE, 32>(mine + 32 * S::ROW);
+            if (blk * 32 < all_lo || blk * 32 + 32 > all_hi) special |= clean_values<DP, TYPE, 32>(mine + 32 * S::ROW, t.kv_len - blk * 32);
             return mine;
         });
     }
@@ -585,7 +586,8 @@ __global__ __launch_bounds__(SplitShape<DP>::WAVES * 64, 1) void attend_split_ke
         ml[wave][lane][1] = l;
     }
     __syncthreads();
-    float* part_o = part + (((int64_t)z * gridDim.y + kv_head) * g.tiles + tile) * (ROWS * (DP + 2));
+    // split z's sums of row i of out: DP floats at part + (z * T * H + i) * DP; their maximum and weight: behind all sums
+    const int64_t all = (int64_t)p.T * p.H, first = (int64_t)z * all;
     if (threadIdx.x < 32) {
         // every wavefront's share of a row; divided by the row's sum where nothing else is to be added
         float m = kNone, sum = 0.f, a[X::WAVES];
@@ -599,10 +601,8 @@ __global__ __launch_bounds__(SplitShape<DP>::WAVES * 64, 1) void attend_split_ke
         const float by = g.splits > 1 ? 1.0f : sum == 0.f ? 0.f : 1.0f / sum;
 #pragma unroll
         for (int w = 0; w < X::WAVES; ++w) weight[w][lane] = a[w] * by;
-        if (g.splits > 1) {
-            part_o[ROWS * DP + 2 * lane] = m;
-            part_o[ROWS * DP + 2 * lane + 1] = sum;
-        }
+        if (g.splits > 1 && row.valid)
+            *reinterpret_cast<float2*>(part + g.splits * all * DP + (first + (int64_t)row.token * p.H + row.head) * 2) = make_float2(m, sum);
     }
     __syncthreads();
     const int rows = t.rows - t.row0 < ROWS ? t.rows - t.row0 : ROWS;
@@ -617,64 +617,72 @@ __global__ __launch_bounds__(SplitShape<DP>::WAVES * 64, 1) void attend_split_ke
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(ow[e], a, v[e]);
         }
-        if (g.splits > 1) {
-            *reinterpret_cast<v4f*>(part_o + r * DP + d) = v;
-        } else {
-            const Row w = row_of(p, t, g, kv_head, t.row0 + r);
-            *reinterpret_cast<uint2*>(p.out + ((int64_t)w.token * p.H + w.head) * p.D + d) = make_uint2(pack2<TYPE>(v[0], v[1]), pack2<TYPE>(v[2], v[3]));
-        }
+        const Row w = row_of(p, t, g, kv_head, t.row0 + r);
+        const int64_t i = (int64_t)w.token * p.H + w.head;
+        if (g.splits > 1) *reinterpret_cast<v4f*>(part + (first + i) * DP + d) = v;
+        else *reinterpret_cast<uint2*>(p.out + i * p.D + d) = make_uint2(pack2<TYPE>(v[0], v[1]), pack2<TYPE>(v[2], v[3]));
     }
 }
 
-// The workgroups' sums of a tile's rows joined, in the order of the splits.  One lane per four value dims of a row; what each
-// split's share is, the lanes of a wavefront work out one split each.
+// The workgroups' sums of a row joined, in the order of the splits; DP / 4 lanes a row, four value dims each.  Rows lie as in
+// out, so that nothing has to be looked up before the loads: the first splits' sums, all maxima and weights and the ends of
+// the sequences come in one turn of memory's latency (found by its tile, a row took three).
 constexpr int MAX_SPLITS = 64;
 template <int DP, int TYPE>
 __global__ __launch_bounds__(256) void attend_join_kernel(const PagedAttention p, const Plan g, const float* __restrict__ part) {
-    constexpr int QUADS = DP / 4, PER = 256 / QUADS;   // rows of a workgroup
+    constexpr int QUADS = DP / 4, PER = 256 / QUADS, EACH = MAX_SPLITS / QUADS;   // lanes and rows; splits whose share a lane works out
     __shared__ float weight[PER][MAX_SPLITS];
-    const int tile = blockIdx.x, kv_head = blockIdx.y;
-    Tile t;
-    if (!locate(p, g.group_size, ROWS, tile, t)) return;
-    const int r0 = blockIdx.z * PER, rows = t.rows - t.row0;
-    if (r0 >= rows) return;   // (the whole workgroup)
-    const float* all = part + ((int64_t)kv_head * g.tiles + tile) * (ROWS * (DP + 2));
-    const int64_t step = (int64_t)p.KV * g.tiles * (ROWS * (DP + 2));
-    const int lane = threadIdx.x & 63;
-    for (int i = threadIdx.x >> 6; i < PER; i += 4) {
-        float m = kNone, l = 0.f;
-        if (lane < g.splits && r0 + i < rows) {
-            const float* one = all + lane * step + ROWS * DP + 2 * (r0 + i);
-            m = one[0];
-            l = one[1];
-        }
-        float top = m;
+    const int64_t all = (int64_t)p.T * p.H;
+    const int mine = threadIdx.x / QUADS, at = threadIdx.x % QUADS, d = at * 4;
+    const int64_t i = (int64_t)blockIdx.x * PER + mine, r = i < all ? i : all - 1;
+    const float* one = part + r * DP + d;
+    const float* ml = part + g.splits * all * DP + r * 2;
+    constexpr int AHEAD = 8;
+    v4f o[AHEAD];
 #pragma unroll
-        for (int s = 1; s < 64; s <<= 1) top = __builtin_fmaxf(top, __shfl_xor(top, s));
-        const float a = share(m, l, top);
-        float sum = wave_sum_f32(l * a);
-        weight[i][lane] = a * (sum == 0.f ? 0.f : 1.0f / sum);
+    for (int k = 0; k < AHEAD; ++k) o[k] = *reinterpret_cast<const v4f*>(one + (k < g.splits ? k : 0) * all * DP);
+    float m = kNone, sm[EACH], sl[EACH];
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+        const int z = k * QUADS + at;
+        const float2 v = *reinterpret_cast<const float2*>(ml + (z < g.splits ? z : 0) * all * 2);
+        sm[k] = z < g.splits ? v.x : kNone;
+        sl[k] = z < g.splits ? v.y : 0.f;
     }
+    const int begin = p.q_offsets[0], end = p.q_offsets[p.B];
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) m = __builtin_fmaxf(m, sm[k]);
+#pragma unroll
+    for (int x = 1; x < QUADS; x <<= 1) m = __builtin_fmaxf(m, __shfl_xor(m, x));
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+        const float a = share(sm[k], sl[k], m);
+        weight[mine][k * QUADS + at] = a;
+        sum = __builtin_fmaf(sl[k], a, sum);
+    }
+#pragma unroll
+    for (int x = 1; x < QUADS; x <<= 1) sum += __shfl_xor(sum, x);
     __syncthreads();
-    const int i = threadIdx.x / QUADS, r = r0 + i, d = (threadIdx.x % QUADS) * 4;
-    if (r >= rows || d >= p.D) return;
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
     v4f v = {0, 0, 0, 0};
-    const float* one = all + r * DP + d;
-    for (int z = 0; z < g.splits; z += 8) {
-        v4f o[8];
+    for (int z = 0; z < g.splits; z += AHEAD) {
+        if (z > 0) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) o[k] = *reinterpret_cast<const v4f*>(one + (z + k < g.splits ? z + k : z) * step);
+            for (int k = 0; k < AHEAD; ++k) o[k] = *reinterpret_cast<const v4f*>(one + (z + k < g.splits ? z + k : z) * all * DP);
+        }
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const float a = z + k < g.splits ? weight[i][z + k] : 0.f;
-            if (a != 0.f) {   // (a split that has seen nothing may have left anything)
+        for (int k = 0; k < AHEAD; ++k) {
+            const float a = z + k < g.splits ? weight[mine][z + k] : 0.f;
+            if (a != 0.f) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(o[k][e], a, v[e]);
             }
         }
     }
-    const Row w = row_of(p, t, g, kv_head, t.row0 + r);
-    *reinterpret_cast<uint2*>(p.out + ((int64_t)w.token * p.H + w.head) * p.D + d) = make_uint2(pack2<TYPE>(v[0], v[1]), pack2<TYPE>(v[2], v[3]));
+    const int token = (int)(r / p.H);
+    if (i >= all || d >= p.D || token < begin || token >= end) return;
+    *reinterpret_cast<uint2*>(p.out + r * p.D + d) = make_uint2(pack2<TYPE>(v[0] * inv, v[1] * inv), pack2<TYPE>(v[2] * inv, v[3] * inv));
 }
 
 // ---- many rows: four wavefronts of 32 rows each go through the same keys ----------------------------------------------
@@ -738,7 +746,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this step has landed; behind the barrier everybody has read the one before it
         uint8_t* k = lds + (uint32_t)((step - begin) & 1) * X::STAGE;
         const int j0 = step * X::STEP;
-        if (j0 < all_lo || j0 + X::STEP > all_hi) special |= clean_values<DP, TYPE, X::MINE>(k + (X::STEP + wave * X::MINE) * S::ROW);
+        if (j0 < all_lo || j0 + X::STEP > all_hi) special |= clean_values<DP, TYPE, X::MINE>(k + (X::STEP + wave * X::MINE) * S::ROW, t.kv_len - j0 - wave * X::MINE);
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (step + 1 < end) copy(step + 1);
         return j0 >= my_hi || j0 + X::STEP <= my_lo ? nullptr : k;
@@ -813,7 +821,7 @@ hipError_t launch(const PagedAttention& p, const Plan& plan, hipStream_t stream)
     float* part = static_cast<float*>(p.workspace);
     const hipError_t e = enqueue(attend_split_kernel<DP, TYPE>, dim3(plan.tiles, p.KV, plan.splits), dim3(SplitShape<DP>::WAVES * 64), stream, p, plan, part);
     if (e != hipSuccess || plan.splits == 1) return e;
-    return enqueue(attend_join_kernel<DP, TYPE>, dim3(plan.tiles, p.KV, ROWS / (256 / (DP / 4))), dim3(256), stream, p, plan, (const float*)part);
+    return enqueue(attend_join_kernel<DP, TYPE>, dim3((unsigned)(((int64_t)p.T * p.H + 1024 / DP - 1) / (1024 / DP))), dim3(256), stream, p, plan, (const float*)part);
 }
 template <int TYPE>
 hipError_t launch_d(const PagedAttention& p, const Plan& plan, hipStream_t stream) {
@@ -830,7 +838,7 @@ size_t paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t H, int64_t 
     if (T <= 0 || B <= 0) return 0;
     const Plan plan = make_plan(T, B, H, KV, D, max_kv, 1);
     if (plan.many || plan.splits == 1) return 0;
-    return (size_t)plan.splits * KV * plan.tiles * (ROWS * (padded_dim(D) + 2)) * sizeof(float);
+    return (size_t)plan.splits * T * H * (padded_dim(D) + 2) * sizeof(float);
 }
 
 hipError_t launch_paged_attention(const PagedAttention& p, hipStream_t stream) {

@@ -282,3 +282,41 @@ def test_long_sequences_of_any_page_size(dev, monkeypatch, plan, page):
         q, k, v, table, offsets, lens, kw = attend_case(([3, 40], [1501, 1090], page, 2, 1, 64, causal, window), torch.bfloat16, dev, seed=page)
         want, bound = oracle.paged_attention(q, k, v, table, offsets, lens, **kw)
         within(ops.paged_attention(*(t.to(dev) for t in (q, k, v, table, offsets, lens)), **kw), want, bound, f"{causal} {window}")
+
+
+@pytest.mark.parametrize("plan", ["0", "1", "2"])
+@pytest.mark.parametrize("d", [72, 128, 200])
+@pytest.mark.parametrize("page", [16, 3])
+def test_a_missing_page_reaches_only_the_rows_that_see_it(dev, monkeypatch, plan, d, page):
+    """Its NaNs stay out of the keys that take its place in shared memory, whatever part of a buffer a key fills."""
+    from test_gpu_layer_ops import attend_case
+
+    from phyai_amd import ops
+
+    monkeypatch.setenv("PHYAI_LAYER_ATTEND", plan)
+    q, k, v, table, offsets, lens, kw = attend_case(([200], [500], page, 2, 1, d, True, 100), torch.bfloat16, dev, seed=d)
+    want, bound = oracle.paged_attention(q, k, v, table, offsets, lens, **kw)
+    gone = table.clone()
+    at = 210 // page
+    gone[0, at] = k.shape[0]
+    out = ops.paged_attention(*(t.to(dev) for t in (q, k, v, gone, offsets, lens)), **kw).cpu()
+    position = torch.arange(300, 500)
+    sees = (position >= at * page) & (position - 99 < (at + 1) * page)
+    assert bool(sees.any()) and bool((~sees).any())
+    assert bool(torch.isnan(out[sees]).all())
+    within(out[~sees], want[~sees], bound[~sees], "rows that do not see it")
+
+
+@pytest.mark.parametrize("plan", ["0", "1"])
+def test_uninitialised_places_of_a_cache_cost_and_change_nothing(dev, monkeypatch, plan):
+    """Infinities behind the last key of a page, in the places whose copies are made all the same."""
+    from test_gpu_layer_ops import attend_case
+
+    from phyai_amd import ops
+
+    monkeypatch.setenv("PHYAI_LAYER_ATTEND", plan)
+    q, k, v, table, offsets, lens, kw = attend_case(([3, 50], [17, 129], 32, 4, 2, 128, False, None), torch.bfloat16, dev)
+    want, bound = oracle.paged_attention(q, k, v, table, offsets, lens, **kw)
+    for fill in (float("inf"), float("-inf"), float("nan"), 3e38):
+        kk, vv = (torch.where(torch.isnan(t), torch.full_like(t, fill), t).to(dev) for t in (k, v))
+        within(ops.paged_attention(q.to(dev), kk, vv, *(t.to(dev) for t in (table, offsets, lens)), **kw), want, bound, str(fill))
