@@ -62,7 +62,8 @@ enum { PHYAI_LAYER_BF16 = 0, PHYAI_LAYER_F16 = 1 };
  * throughout, one rounding.  A position outside the table turns its token's query and key into NaNs.
  * q_out: [T, heads, head_dim].  With k_out ([T, kv_heads, head_dim]) keys go there and values nowhere; with k_out NULL keys
  * and values go to k_pages / v_pages (strides in elements: page, token, head): token t to token slots[t] % page_size of
- * page slots[t] / page_size.  A slot outside [0, n_pages * page_size) is not written (padding); slots must differ.
+ * page slots[t] / page_size.  A slot outside [0, n_pages * page_size) is not written (padding); slots must differ, and
+ * so must the places that the strides give them.
  * Limits: rot and head_dim multiples of 8, rot <= head_dim <= 512; strides multiples of 8; pointers 16-byte aligned.
  */
 int phyai_layer_head_rope(const void *qkv, int64_t ld, const void *q_weight, const void *k_weight, const float *cos_sin,

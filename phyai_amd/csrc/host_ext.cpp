@@ -886,8 +886,13 @@ PyObject* py_qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor *kp = tensor(a[11]), *vp = tensor(a[12]), *slots = tensor(a[13]);
     const bool paged = a[11] != Py_None || a[12] != Py_None || a[13] != Py_None;
     int64_t ks[3], vs[3];
-    if (paged && (!pages_of(kp, dtype, D, at_.dev, ks) || !pages_of(vp, dtype, D, at_.dev, vs) || kp->sizes() != vp->sizes() || kp->size(2) != KV ||
-                  !vector_on(slots, at::kLong, T, at_.dev)))
+    auto expanded = [](const at::Tensor& t) {
+        for (int i = 0; i < 3; ++i)
+            if (t.size(i) > 1 && t.stride(i) == 0) return true;
+        return false;
+    };
+    if (paged && (!pages_of(kp, dtype, D, at_.dev, ks) || !pages_of(vp, dtype, D, at_.dev, vs) || expanded(*kp) || expanded(*vp) ||
+                  kp->sizes() != vp->sizes() || kp->size(2) != KV || !vector_on(slots, at::kLong, T, at_.dev)))
         return declined();
     at::Tensor q, k;
     if (a[14] != Py_None) {

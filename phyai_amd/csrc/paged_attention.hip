@@ -82,6 +82,19 @@ struct Plan {
     int group_size, tiles, splits, many;
 };
 
+// The sum over the lanes up to this one: four steps inside a row of sixteen lanes, two across rows.
+template <int CTRL, int ROWS_OF = 0xF>
+__device__ __forceinline__ int dpp_or_zero(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS_OF, 0xF, true); }
+__device__ __forceinline__ int sum_up_to_lane(int v) {
+    v += dpp_or_zero<0x111>(v);
+    v += dpp_or_zero<0x112>(v);
+    v += dpp_or_zero<0x114>(v);
+    v += dpp_or_zero<0x118>(v);
+    v += dpp_or_zero<0x142, 0xA>(v);   // lane 15's to the next row, 47's likewise
+    v += dpp_or_zero<0x143, 0xC>(v);   // lane 31's to the upper half
+    return v;
+}
+
 // Where a tile of `rows_per_tile` packed rows lies: the tiles of the sequences are numbered one sequence after another.
 // Every wavefront finds it by itself, 64 sequences at a time.
 struct Tile {
@@ -99,12 +112,7 @@ __device__ __forceinline__ bool locate(const PagedAttention& p, int group, int r
             q1 = clamp_i(p.q_offsets[b + 1], q0, p.T);
         }
         const int tiles = ((q1 - q0) * group + rows_per_tile - 1) / rows_per_tile;
-        int upto = tiles;
-#pragma unroll
-        for (int s = 1; s < 64; s <<= 1) {
-            const int v = __shfl_up(upto, s);
-            if (lane >= s) upto += v;
-        }
+        const int upto = sum_up_to_lane(tiles);
         const uint64_t hit = __ballot(before + upto > tile);
         if (hit != 0) {
             const int l = __builtin_ctzll(hit);

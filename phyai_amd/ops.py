@@ -674,7 +674,7 @@ def fp8_mlp(x: torch.Tensor, weight1: torch.Tensor, weight1_scale: torch.Tensor,
 BLOCK = 128   # elements per scale, along K and (of weights) along N
 
 
-def _device_of(op: str, device: torch.device):
+def _device_of(device: torch.device):
     """Context in which ``device`` is the current one: kernels are launched on its current stream."""
     return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
@@ -707,7 +707,7 @@ def fp8_block_quant(x: torch.Tensor, *, out: torch.Tensor | None = None,
         raise _err(op, f"scale_out must be a contiguous float32 tensor of shape {sshape}")
     if M == 0:
         return out, scale_out
-    with _device_of(op, x.device):
+    with _device_of(x.device):
         rc = _lib.load().phyai_layer_block_quant(x2.data_ptr(), x2.stride(0) if M > 1 else K, M, K, out.data_ptr(),
                                                  scale_out.data_ptr(), blocks, 1, _stream_ptr())
     _lib.check_layer(rc, op)
@@ -754,7 +754,7 @@ def fp8_block_gemm(xq: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor
     if M == 0:
         return out
     per_row = x_scale.shape[-1]
-    with _device_of(op, xq.device):
+    with _device_of(xq.device):
         rc = _lib.load().phyai_layer_block_gemm(x2.data_ptr(), x_scale.data_ptr(), per_row, 1 if per_row == blocks else 0, weight.data_ptr(),
                                                 weight_scale.data_ptr(), bias.data_ptr() if bias is not None else None, out.data_ptr(), N,
                                                 M, N, K, _stream_ptr())
@@ -782,7 +782,7 @@ def fp8_block_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.
     if M == 0:
         return out
     lib = _lib.load()
-    with _device_of(op, x.device):
+    with _device_of(x.device):
         need = lib.phyai_layer_block_linear_workspace_bytes(M, N, K)
         ws = reserve_workspace(need, x.device) if need else None
         rc = lib.phyai_layer_block_linear(x2.data_ptr(), x2.stride(0) if M > 1 else K, weight.data_ptr(), weight_scale.data_ptr(),
@@ -889,6 +889,8 @@ def qk_norm_rope(qkv: torch.Tensor, cos_sin: torch.Tensor, positions: torch.Tens
         _check_pages(op, k_pages, v_pages, dtype, D, dev)
         if k_pages.shape[2] != KV:
             raise _err(op, f"pages have {k_pages.shape[2]} heads, num_kv_heads is {KV}")
+        if any(s == 0 and n > 1 for t in (k_pages, v_pages) for s, n in zip(t.stride(), t.shape)):
+            raise _err(op, "pages must not be expanded: several tokens or heads would be written to one place")
         slot_ptr = _vector(op, "slots", slots, torch.int64, T, dev)
         n_pages, page_size = k_pages.shape[:2]
         ks, vs = ((ctypes.c_int64 * 3)(*_page_strides(t)) for t in (k_pages, v_pages))
@@ -896,7 +898,7 @@ def qk_norm_rope(qkv: torch.Tensor, cos_sin: torch.Tensor, positions: torch.Tens
         k = torch.empty(T, KV, D, dtype=dtype, device=dev)
     if T == 0:
         return out, k
-    with _device_of(op, dev):
+    with _device_of(dev):
         rc = _lib.load().phyai_layer_head_rope(
             qkv.data_ptr(), qkv.stride(0) if T > 1 else width, *weights, cos_sin.data_ptr(), cos_sin.shape[0], pos, out.data_ptr(),
             k.data_ptr() if k is not None else None, k_pages.data_ptr() if paged else None, v_pages.data_ptr() if paged else None, ks, vs,
@@ -958,7 +960,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     import ctypes
 
     lib = _lib.load()
-    with _device_of(op, dev):
+    with _device_of(dev):
         need = lib.phyai_layer_paged_attention_workspace_bytes(T, B, H, KV, D, W * page_size)
         ws = reserve_workspace(need, dev) if need else None
         rc = lib.phyai_layer_paged_attention(

@@ -246,6 +246,8 @@ def test_qk_norm_rope_refuses(dev):
                  dict(k_pages=pages[0]), dict(k_pages=pages[0], v_pages=pages[1]), dict(slots=slots),
                  dict(k_pages=pages[0], v_pages=pages[1], slots=slots.int()), dict(k_pages=pages[0], v_pages=pages[1][:2], slots=slots),
                  dict(k_pages=pages[0].half(), v_pages=pages[1].half(), slots=slots), dict(k_pages=pages[0].cpu(), v_pages=pages[1], slots=slots),
+                 dict(k_pages=pages[0][:, :, :1].expand(4, 8, 2, d), v_pages=pages[1], slots=slots),
+                 dict(k_pages=pages[0], v_pages=pages[1][:1].expand(4, 8, 2, d), slots=slots),
                  dict(k_pages=pages[0][:, :, :1], v_pages=pages[1][:, :, :1], slots=slots), dict(out=torch.empty(t, heads, d, device=dev)),
                  dict(out=torch.empty(t, heads + 1, d, dtype=torch.bfloat16, device=dev))):
         refuses(ops.qk_norm_rope, **(good | over))
@@ -320,3 +322,58 @@ def test_uninitialised_places_of_a_cache_cost_and_change_nothing(dev, monkeypatc
     for fill in (float("inf"), float("-inf"), float("nan"), 3e38):
         kk, vv = (torch.where(torch.isnan(t), torch.full_like(t, fill), t).to(dev) for t in (k, v))
         within(ops.paged_attention(q.to(dev), kk, vv, *(t.to(dev) for t in (table, offsets, lens)), **kw), want, bound, str(fill))
+
+
+def test_a_cache_without_pages(dev):
+    from phyai_amd import ops
+
+    q = seeded((3, 4, 64), 1).to(dev)
+    none = torch.zeros(0, 16, 2, 64, dtype=torch.bfloat16, device=dev)
+    table, offsets = torch.zeros(2, 1, dtype=torch.int32, device=dev), torch.tensor([0, 1, 3], dtype=torch.int32, device=dev)
+    lens = torch.tensor([0, 2], dtype=torch.int32, device=dev)
+    out = ops.paged_attention(q, none, none, table, offsets, lens)
+    assert not out[0].any() and bool(torch.isnan(out[1:]).all())
+    assert not ops.paged_attention(q, none, none, table[:, :0], offsets, lens).any()   # a table of no pages: no keys
+    assert ops.paged_attention(q[:0], none, none, table, offsets * 0, lens).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("heads", [1, 8])
+def test_many_sequences_of_unequal_lengths(dev, heads):
+    """More sequences than are looked at together, some without tokens or keys, in front of and behind rows of no sequence."""
+    from test_gpu_layer_ops import cache
+
+    from phyai_amd import ops
+
+    g = gen(3)
+    counts = torch.randint(0, 4, (300,), generator=g)
+    kvs = [int(n) + int(x) for n, x in zip(counts, torch.randint(0, 50, (300,), generator=g))]
+    k, v, table = cache(kvs, 8, 1, 64, torch.bfloat16, 4)
+    first = 5
+    offsets = (torch.cat([torch.zeros(1, dtype=torch.int64), counts.cumsum(0)]) + first).int()
+    total = int(offsets[-1]) + 7
+    q = seeded((total, heads, 64), 5)
+    lens = torch.tensor(kvs, dtype=torch.int32)
+    want, bound = oracle.paged_attention(q, k, v, table, offsets, lens)
+    out = torch.full((total, heads, 64), 7.0, dtype=torch.bfloat16, device=dev)
+    ops.paged_attention(*(t.to(dev) for t in (q, k, v, table, offsets, lens)), out=out)
+    inside = slice(first, int(offsets[-1]))
+    within(out[inside], want[inside], bound[inside], "rows")
+    assert bool((out[:first] == 7).all()) and bool((out[int(offsets[-1]):] == 7).all())
+
+
+def test_one_token_of_a_padded_batch_leaves_the_padding_alone(dev):
+    """Split over many workgroups, with rows behind the last sequence."""
+    from test_gpu_layer_ops import attend_case
+
+    from phyai_amd import ops
+
+    q, k, v, table, offsets, lens, kw = attend_case(([1, 1], [3000, 17], 16, 4, 1, 128, True, None), torch.bfloat16, dev)
+    want, bound = oracle.paged_attention(q, k, v, table, offsets, lens, **kw)
+    padded = torch.cat([q, seeded((6, 4, 128), 9)]).to(dev)
+    out = torch.full((8, 4, 128), 7.0, dtype=torch.bfloat16, device=dev)
+    ops.paged_attention(padded, *(t.to(dev) for t in (k, v, table, offsets, lens)), out=out, **kw)
+    within(out[:2], want, bound, "rows")
+    assert bool((out[2:] == 7).all())
+    replaced = padded.clone()
+    ops.paged_attention(replaced, *(t.to(dev) for t in (k, v, table, offsets, lens)), out=replaced, **kw)   # q's own place
+    assert bf16_equal(replaced[:2], out[:2]) and bf16_equal(replaced[2:], padded[2:])
