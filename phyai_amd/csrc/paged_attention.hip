@@ -354,10 +354,12 @@ __device__ __forceinline__ void raise_maximum(State<DP>& st, float mx) {
     const float m = __builtin_fmaxf(st.m, mx);
     const float a = m == kNone ? 1.0f : __builtin_amdgcn_exp2f(st.m - m);   // (0 the first time, when O and l are zero)
     st.l *= a;
+    if (!__all(st.m == kNone)) {   // (the first keys of all find only zeros there)
 #pragma unroll
-    for (int b = 0; b < DP / 32; ++b)
+        for (int b = 0; b < DP / 32; ++b)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) st.o[b][i] *= a;
+            for (int i = 0; i < 16; ++i) st.o[b][i] *= a;
+    }
     st.m = m;
 }
 // Scores to probabilities, as the second product's operand.  The sum is of the rounded ones, those that the product uses:
@@ -723,13 +725,6 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
     const int begin = lo / X::STEP, end = (hi + X::STEP - 1) / X::STEP;
     const Pool pool = make_pool<DP, TYPE>(p, t, kv_head, g);
     const float c = p.scale * 1.4426950408889634f;
-    State<DP> st;
-    st.m = kNone;
-    st.l = 0.f;
-#pragma unroll
-    for (int b = 0; b < DP / 32; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) st.o[b][i] = 0.f;
     const uint32_t base = (uint32_t)(uintptr_t)lds;
     using Feed = Feeder<DP, X::STEP, X::MINE>;
     Feed feed(pool, begin, wave * X::MINE, ids[wave][0]);
@@ -750,6 +745,13 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         copy(begin);
     }
+    State<DP> st;
+    st.m = kNone;
+    st.l = 0.f;
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st.o[b][i] = 0.f;
     attend_steps<DP, TYPE, X::STEP / 32>(st, qf, begin, end, row, whole_lo, whole_hi, c, [&](int step) -> const uint8_t* {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this step has landed; behind the barrier everybody has read the one before it
         uint8_t* k = lds + (uint32_t)((step - begin) & 1) * X::STAGE;
