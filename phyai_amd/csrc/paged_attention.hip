@@ -156,7 +156,7 @@ struct Pool {
     int n_pages, page_size, kv_len, table_width;
     Division by_page;
     int d_chunks;                      // 16-byte chunks of a key that exist
-    bool neat;                         // whole keys of a copy instruction are neighbours in a page
+    bool neat;                         // runs of eight keys are neighbours in a page, and a key fills a row of LDS
 };
 
 // A wavefront's part of bringing blocks `begin`, begin + 1, ... of STEP keys into LDS: N keys of each, from key `row` of the
@@ -167,6 +167,7 @@ struct Pool {
 template <int DP, int STEP, int N>
 struct Feeder {
     static constexpr int BLOCKS = 64 / N, PER_COPY = Shape<DP>::PER_COPY, COPIES = N / PER_COPY, ROW = Shape<DP>::ROW;
+    static constexpr int RUN = 8;      // keys, neighbours in a page, that copies share an address for
     const Pool& s;
     const int begin, row;
     lds_u32* const ids;                // two times 64 words of LDS, this wavefront's
@@ -180,12 +181,12 @@ struct Feeder {
         k_at = (lc ^ k_swizzle<DP>((uint32_t)row + lr)) << 4;
         v_at = (lc ^ v_swizzle<DP>((uint32_t)row + lr)) << 4;
     }
-    // The lane's key.  In the place of one beyond the last, the first of the last key's copy: no row sees what is copied
-    // there, it only has to be in the cache, like all keys of that copy (filled with zeros instead, by lanes that each have an
+    // The lane's key.  In the place of one beyond the last, the first of the last key's run: no row sees what is copied
+    // there, it only has to be in the cache, like all keys of that run (filled with zeros instead, by lanes that each have an
     // address of their own, a block took 3 us longer at 256 dims).
     __device__ __forceinline__ int key(int turn) const {
         const int lane = threadIdx.x & 63, j = (begin + turn * BLOCKS + lane / N) * STEP + row + lane % N;
-        return j < s.kv_len ? j : (s.kv_len - 1) & ~(PER_COPY - 1);
+        return j < s.kv_len ? j : (s.kv_len - 1) & ~(RUN - 1);
     }
     // The page numbers of a turn of BLOCKS blocks; to be waited for before look().
     __device__ __forceinline__ void ask(int turn) {
@@ -206,15 +207,18 @@ struct Feeder {
     __device__ __forceinline__ void copy(int blk, uint32_t k_lds, uint32_t v_lds) {
         const int from = ((blk - begin) % BLOCKS) * N;   // the block's first lane
         if (s.neat && ((odd >> from) & (N == 64 ? ~0ull : (1ull << (N & 63)) - 1)) == 0) {
-            const uint32_t run = ((threadIdx.x & 63) / Shape<DP>::CHUNKS) * (uint32_t)s.token_bytes;
+            const uint32_t token = (uint32_t)s.token_bytes, lr = (threadIdx.x & 63) / Shape<DP>::CHUNKS;
 #pragma unroll
-            for (int t = 0; t < COPIES; ++t) {
-                const uint32_t to = (uint32_t)(row + t * PER_COPY) * ROW;
-                const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(lo, from + t * PER_COPY) |
-                                    (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, from + t * PER_COPY) << 32;
-                // (the swizzles of copy t are those of copy 0 with the bits of t's first key flipped)
-                copy16_to_lds<kBaseSettles>(s.k + at, (k_at ^ k_swizzle<DP>(t * PER_COPY) << 4) + run, __builtin_amdgcn_readfirstlane(k_lds + to));
-                copy16_to_lds<kBaseSettles>(s.v + at, (v_at ^ v_swizzle<DP>(t * PER_COPY) << 4) + run, __builtin_amdgcn_readfirstlane(v_lds + to));
+            for (int r = 0; r < N; r += RUN) {
+                const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(lo, from + r) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, from + r) << 32;
+                const uint8_t *k = s.k + at, *v = s.v + at;
+#pragma unroll
+                for (int i = 0; i < RUN; i += PER_COPY) {
+                    const uint32_t to = (uint32_t)(row + r + i) * ROW, key = (lr + i) * token;
+                    // (the swizzles of these keys are those of the first with the bits of r + i flipped)
+                    copy16_to_lds<kBaseSettles>(k, (k_at ^ k_swizzle<DP>(r + i) << 4) + key, __builtin_amdgcn_readfirstlane(k_lds + to));
+                    copy16_to_lds<kBaseSettles>(v, (v_at ^ v_swizzle<DP>(r + i) << 4) + key, __builtin_amdgcn_readfirstlane(v_lds + to));
+                }
             }
             return;
         }
@@ -264,17 +268,24 @@ __device__ __forceinline__ uint32_t without_special(uint32_t w) {
 template <int DP, int TYPE, int N>
 __device__ __forceinline__ bool clean_values(uint8_t* v, int keys) {
     bool special = false;
+    constexpr int PER = N * Shape<DP>::ROW / 1024, AT_ONCE = PER < 4 ? PER : 4;   // 16 bytes of a lane: in all, read together
 #pragma unroll 1
-    for (int x = (threadIdx.x & 63) * 16; x < N * Shape<DP>::ROW; x += 1024) {
-        v4i f = *reinterpret_cast<const v4i*>(v + x);
-        bool any = false;
+    for (int x = (threadIdx.x & 63) * 16; x < N * Shape<DP>::ROW; x += AT_ONCE * 1024) {
+        v4i f[AT_ONCE];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            any |= any_special<TYPE>((uint32_t)f[i]);
-            f[i] = (int)without_special<TYPE>((uint32_t)f[i]);
+        for (int k = 0; k < AT_ONCE; ++k) f[k] = *reinterpret_cast<const v4i*>(v + x + k * 1024);
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) {
+            bool any = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) any |= any_special<TYPE>((uint32_t)f[k][i]);
+            if (any) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) f[k][i] = (int)without_special<TYPE>((uint32_t)f[k][i]);
+                *reinterpret_cast<v4i*>(v + x + k * 1024) = f[k];
+            }
+            special |= any && (x + k * 1024) / Shape<DP>::ROW < keys;
         }
-        if (any) *reinterpret_cast<v4i*>(v + x) = f;
-        special |= any && x / Shape<DP>::ROW < keys;
     }
     return __any(special);
 }
@@ -506,7 +517,7 @@ __device__ __forceinline__ Pool make_pool(const PagedAttention& p, const Tile& t
     s.table = p.table + (int64_t)t.b * p.table_ld;
     s.table_width = p.table_width;
     s.d_chunks = p.D / 8;
-    s.neat = p.D == DP && p.page_size % Shape<DP>::PER_COPY == 0;
+    s.neat = p.D == DP && p.page_size % 8 == 0;
     return s;
 }
 
