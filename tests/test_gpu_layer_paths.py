@@ -377,3 +377,24 @@ def test_one_token_of_a_padded_batch_leaves_the_padding_alone(dev):
     replaced = padded.clone()
     ops.paged_attention(replaced, *(t.to(dev) for t in (k, v, table, offsets, lens)), out=replaced, **kw)   # q's own place
     assert bf16_equal(replaced[:2], out[:2]) and bf16_equal(replaced[2:], padded[2:])
+
+
+@pytest.mark.parametrize("t,heads,kv_heads,d,rot", [(2200, 12, 3, 72, 48), (9000, 4, 1, 128, 128)])
+def test_head_norms_and_rotation_of_many_tokens(dev, t, heads, kv_heads, d, rot):
+    """More heads than fit the chip at once: an odd number of them, query, key and value heads in one group."""
+    from phyai_amd import ops
+
+    qkv = seeded((t, (heads + 2 * kv_heads) * d), 1)
+    table = ops.rope_table(t, rot, device="cpu")
+    positions = torch.randperm(t, generator=gen(2))
+    weights = [seeded((d,), s, 0.3) + 1 for s in (3, 4)]
+    k_pages, v_pages = (torch.zeros(-(-t // 16), 16, kv_heads, d, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    slots = torch.randperm(t, generator=gen(3))
+    q, _ = ops.qk_norm_rope(qkv.to(dev), table.to(dev), positions.to(dev), heads, kv_heads, d, q_weight=weights[0].to(dev), k_weight=weights[1].to(dev),
+                            k_pages=k_pages, v_pages=v_pages, slots=slots.to(dev))
+    rows = qkv.view(t, -1, d)
+    within(q, *oracle.head_rope(rows[:, :heads], weights[0], table, positions, 1e-6, False, False), "q")
+    within(k_pages.cpu().view(-1, kv_heads, d)[slots], *oracle.head_rope(rows[:, heads: heads + kv_heads], weights[1], table, positions, 1e-6, False, False), "k")
+    assert torch.equal(v_pages.cpu().view(-1, kv_heads, d)[slots], rows[:, heads + kv_heads:])
+    q2, k2 = ops.qk_norm_rope(qkv.to(dev), table.to(dev), positions.to(dev), heads, kv_heads, d, q_weight=weights[0].to(dev), k_weight=weights[1].to(dev))
+    assert bf16_equal(q2, q) and bf16_equal(k2.cpu(), k_pages.cpu().view(-1, kv_heads, d)[slots])
