@@ -1,7 +1,7 @@
 """Attention of action chunks over a paged cache that holds their prefix.
 
 The part of the reference's attention back end that the expert loop needs (a paged KV pool, its page
-table, and the plan that the reference makes with flashinfer): the prefix of every sequence goes into
+table, and the plan of a run over it): the prefix of every sequence goes into
 pages once per layer (:meth:`PagedPrefixAttention.prefill`), then each denoise step writes the chunk's
 keys and values behind it and attends over both.  Two kernels a call: ``ops.qk_norm_rope`` rotates the
 fused projection's query and key heads and writes keys and values where they belong,
