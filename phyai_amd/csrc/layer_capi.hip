@@ -229,7 +229,8 @@ int phyai_layer_paged_attention(const void* q, int64_t q_token_stride, int64_t q
         return fail(PHYAI_FP8_EUNSUPPORTED, "%s: T * heads and batch must be below 2^30, n_pages below 2^31, kv_heads below 2^16", fn);
     if (table_width >= kMost / 4 || page_size >= kMost || (table_width > 0 && page_size > (kMost / 2 - 1) / table_width))
         return fail(PHYAI_FP8_EUNSUPPORTED, "%s: table width * page size must be below 2^30", fn);
-    if (table_width > 0 && table_stride < table_width && batch > 1) return fail(PHYAI_FP8_EINVAL, "%s: row stride of the page table is smaller than its width", fn);
+    if (table_width > 0 && batch > 1 && table_stride != 0 && table_stride < table_width)
+        return fail(PHYAI_FP8_EINVAL, "%s: row stride of the page table is smaller than its width", fn);
     if (kv_strides[1] >= (int64_t)1 << 28) return fail(PHYAI_FP8_EUNSUPPORTED, "%s: stride between a page's tokens of 2^28 or more", fn);
     const size_t need = phyai_layer_paged_attention_workspace_bytes(T, batch, heads, kv_heads, head_dim, table_width * page_size);
     if (need > 0 && (!workspace || !aligned(workspace, 256) || workspace_bytes < need))

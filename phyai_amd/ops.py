@@ -942,7 +942,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if H % KV != 0:
         raise _err(op, f"{H} query heads are not a multiple of {KV} key heads")
     if not (isinstance(page_table, torch.Tensor) and page_table.device == dev and page_table.dtype == torch.int32 and page_table.dim() == 2
-            and (page_table.numel() == 0 or page_table.stride(1) == 1)):
+            and (page_table.numel() == 0 or page_table.shape[1] == 1 or page_table.stride(1) == 1)):
         raise _err(op, f"page_table must be a 2-D int32 tensor on {dev} with contiguous rows")
     B, W = page_table.shape
     offsets, lens = _vector(op, "q_offsets", q_offsets, torch.int32, B + 1, dev), _vector(op, "kv_lens", kv_lens, torch.int32, B, dev)

@@ -398,3 +398,21 @@ def test_head_norms_and_rotation_of_many_tokens(dev, t, heads, kv_heads, d, rot)
     assert torch.equal(v_pages.cpu().view(-1, kv_heads, d)[slots], rows[:, heads + kv_heads:])
     q2, k2 = ops.qk_norm_rope(qkv.to(dev), table.to(dev), positions.to(dev), heads, kv_heads, d, q_weight=weights[0].to(dev), k_weight=weights[1].to(dev))
     assert bf16_equal(q2, q) and bf16_equal(k2.cpu(), k_pages.cpu().view(-1, kv_heads, d)[slots])
+
+
+def test_sequences_that_share_a_row_of_the_table(dev):
+    """An expanded table, and one of a single column that lies across another."""
+    from test_gpu_layer_ops import attend_case
+
+    from phyai_amd import ops
+
+    q, k, v, table, offsets, lens, kw = attend_case(([2, 3, 1], [40, 40, 40], 16, 2, 1, 64, True, None), torch.bfloat16, dev)
+    one = table[:1].to(dev)
+    rest = [t.to(dev) for t in (offsets, lens)]
+    want = ops.paged_attention(q.to(dev), k.to(dev), v.to(dev), one.repeat(3, 1), *rest, **kw)
+    assert bf16_equal(ops.paged_attention(q.to(dev), k.to(dev), v.to(dev), one.expand(3, -1), *rest, **kw), want)
+    lens = torch.tensor([16, 9, 3], dtype=torch.int32, device=dev)
+    column = table[:, :1].to(dev)
+    want = ops.paged_attention(q.to(dev), k.to(dev), v.to(dev), column.contiguous(), rest[0], lens, **kw)
+    across = column.t().contiguous().t()
+    assert across.stride(0) == 1 and bf16_equal(ops.paged_attention(q.to(dev), k.to(dev), v.to(dev), across, rest[0], lens, **kw), want)
