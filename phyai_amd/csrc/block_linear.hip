@@ -83,18 +83,18 @@ __global__ __launch_bounds__(256) void block_quant_kernel(const uint16_t* __rest
 // the blocks of K in turn, each with its weights straight from memory in the MFMA's registers (lane q of a row: bytes
 // 16 q and 64 + 16 q), DEPTH blocks ahead.  The partial sums meet in LDS, added in wavefront order.  1 x 2560 x 1024: 3.5 us
 // in a graph, the launch and two trips to memory; 2 x 22656 x 5632: 34 us, 3.7 TB/s of weights.
-constexpr int SMALL_WAVES = 8;
+constexpr int FEW_WAVES = 8;
 
 template <int NT>
 struct FewShape {
     static constexpr int ROWS = 8, BLOCKS = 32;                     // of K in LDS at a time
     static constexpr int ROW = BLOCKS * QB + QB;               // bytes between rows: an odd number of lines, for the banks
-    static constexpr int SCALES_AT = ROWS * ROW, CODES = SCALES_AT + ROWS * BLOCKS * 4, SUMS = SMALL_WAVES * NT * 1024;
+    static constexpr int SCALES_AT = ROWS * ROW, CODES = SCALES_AT + ROWS * BLOCKS * 4, SUMS = FEW_WAVES * NT * 1024;
     static constexpr int LDS = CODES > SUMS ? CODES : SUMS;
 };
 
 template <int NT, int DEPTH, bool CODES>
-__global__ __launch_bounds__(SMALL_WAVES * 64) void block_few_kernel(const BlockLinear p) {
+__global__ __launch_bounds__(FEW_WAVES * 64) void block_few_kernel(const BlockLinear p) {
     using S = FewShape<NT>;
     __shared__ __align__(16) uint8_t lds[S::LDS];
     float* const scales = reinterpret_cast<float*>(lds + S::SCALES_AT);   // [block][token]
@@ -125,26 +125,26 @@ __global__ __launch_bounds__(SMALL_WAVES * 64) void block_few_kernel(const Block
     };
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d)
-        if (wave + d * SMALL_WAVES < blocks) load(wave + d * SMALL_WAVES, stage[d]);
+        if (wave + d * FEW_WAVES < blocks) load(wave + d * FEW_WAVES, stage[d]);
 
     v4f acc[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[t] = v4f{0, 0, 0, 0};
     const int xrow = l16 < S::ROWS ? l16 : 0;   // (columns of the products past the last token are nobody's)
-    static_assert(S::BLOCKS % (SMALL_WAVES) == 0, "a stretch is whole turns of the wavefronts");
+    static_assert(S::BLOCKS % (FEW_WAVES) == 0, "a stretch is whole turns of the wavefronts");
     for (int first = 0; first < blocks; first += S::BLOCKS) {
         const int here = blocks - first < S::BLOCKS ? blocks - first : S::BLOCKS;
         if (first > 0) __syncthreads();   // (the stretch before has been read)
         // codes of `rows` tokens and `here` blocks, four of them per sixteen lanes in flight
         const int c = threadIdx.x & 15;
-        for (int item = threadIdx.x >> 4; item < rows * here; item += 4 * SMALL_WAVES * 4) {
+        for (int item = threadIdx.x >> 4; item < rows * here; item += 4 * FEW_WAVES * 4) {
             int r[4], g[4];
             uint4 v[4];
             uint2 e[4];
             float s[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int it = item + i * 4 * SMALL_WAVES;
+                const int it = item + i * 4 * FEW_WAVES;
                 r[i] = it < rows * here ? (int)((uint32_t)it / (uint32_t)here) : 0;
                 g[i] = it < rows * here ? it - r[i] * here : 0;
                 const int k = (first + g[i]) * QB + c * 8;
@@ -169,17 +169,17 @@ __global__ __launch_bounds__(SMALL_WAVES * 64) void block_few_kernel(const Block
                     block_encode(one, s[i], code);
                     e[i] = code[0];
                 }
-                if (item + i * 4 * SMALL_WAVES >= rows * here) continue;
+                if (item + i * 4 * FEW_WAVES >= rows * here) continue;
                 *reinterpret_cast<uint2*>(lds + r[i] * S::ROW + g[i] * QB + (((uint32_t)(c >> 1) ^ ((uint32_t)(r[i] >> 1) & 7u)) << 4) + (c & 1) * 8) = e[i];
                 if (c == 0) scales[g[i] * S::ROWS + r[i]] = s[i];
             }
         }
         __syncthreads();
-        for (int g0 = wave; g0 < S::BLOCKS; g0 += SMALL_WAVES * DEPTH) {
+        for (int g0 = wave; g0 < S::BLOCKS; g0 += FEW_WAVES * DEPTH) {
 #pragma unroll
             for (int d = 0; d < DEPTH; ++d) {
-                const int g = g0 + d * SMALL_WAVES;
-                if (S::BLOCKS / SMALL_WAVES % DEPTH != 0 && g >= S::BLOCKS) continue;
+                const int g = g0 + d * FEW_WAVES;
+                if (S::BLOCKS / FEW_WAVES % DEPTH != 0 && g >= S::BLOCKS) continue;
                 Stage& o = stage[d];
                 if (g < here) {
                     const uint8_t* xr = lds + xrow * S::ROW + g * QB;
@@ -196,7 +196,7 @@ __global__ __launch_bounds__(SMALL_WAVES * 64) void block_few_kernel(const Block
                         for (int i = 0; i < 4; ++i) acc[t][i] = __builtin_fmaf(y[i], f, acc[t][i]);
                     }
                 }
-                const int next = first + g + DEPTH * SMALL_WAVES;
+                const int next = first + g + DEPTH * FEW_WAVES;
                 if (next < blocks) load(next, o);
             }
         }
@@ -209,7 +209,7 @@ __global__ __launch_bounds__(SMALL_WAVES * 64) void block_few_kernel(const Block
     if (wave >= NT) return;
     v4f y = sums[wave * 64 + lane];
 #pragma unroll
-    for (int w = 1; w < SMALL_WAVES; ++w) {
+    for (int w = 1; w < FEW_WAVES; ++w) {
         const v4f o = sums[(w * NT + wave) * 64 + lane];
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] += o[e];
@@ -238,10 +238,11 @@ __device__ __forceinline__ uint32_t quad_rows_max(uint32_t v) {
 // blocks ahead, and quantizes the values there - the whole block of a row is in four lanes - while the others' loads are on
 // their way.  The partial sums meet in LDS, added in wavefront order.  (More than 16 tokens a workgroup, so that weights are read
 // fewer times, is slower: every size from 17 to 64 tokens, most by a third; the second reading comes out of the L2.)
-// Bound by the quantizer's eight instructions a value, done once per 16 NT columns: 50 x 1024 x 4096 9.1 us, 3.6 of them that.
-template <int NT, int DEPTH, bool CODES>
-__global__ __launch_bounds__(SMALL_WAVES * 64) void block_small_kernel(const BlockLinear p) {
-    __shared__ float sums[SMALL_WAVES][NT][64][4];
+// Bound by the quantizer's eight instructions a value, done once per 16 NT columns (blocks further ahead change nothing): 50 x 1024 x
+// 4096 8.7 us, 3.6 of them that.
+template <int NT, int WAVES, int DEPTH, bool CODES>
+__global__ __launch_bounds__(WAVES * 64) void block_small_kernel(const BlockLinear p) {
+    __shared__ float sums[WAVES][NT][64][4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, q = lane >> 4;
     const int m0 = blockIdx.y * 16, n0 = blockIdx.x * (16 * NT);
     const int blocks = (p.K + QB - 1) / QB;
@@ -313,11 +314,11 @@ __global__ __launch_bounds__(SMALL_WAVES * 64) void block_small_kernel(const Blo
     };
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d)
-        if (wave + d * SMALL_WAVES < blocks) load(wave + d * SMALL_WAVES, stage[d]);
-    for (int g = wave; g < blocks; g += DEPTH * SMALL_WAVES) {
+        if (wave + d * WAVES < blocks) load(wave + d * WAVES, stage[d]);
+    for (int g = wave; g < blocks; g += DEPTH * WAVES) {
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d) {
-            const int now = g + d * SMALL_WAVES, next = now + DEPTH * SMALL_WAVES;
+            const int now = g + d * WAVES, next = now + DEPTH * WAVES;
             if (now < blocks) multiply(stage[d]);
             if (next < blocks) load(next, stage[d]);
         }
@@ -328,7 +329,7 @@ __global__ __launch_bounds__(SMALL_WAVES * 64) void block_small_kernel(const Blo
     if (wave >= NT) return;
     v4f y = *reinterpret_cast<const v4f*>(sums[0][wave][lane]);
 #pragma unroll
-    for (int w = 1; w < SMALL_WAVES; ++w) {
+    for (int w = 1; w < WAVES; ++w) {
         const v4f o = *reinterpret_cast<const v4f*>(sums[w][wave][lane]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] += o[e];
@@ -706,15 +707,15 @@ hipError_t launch_tile(const BlockLinear& p, hipStream_t stream) {
 template <int NT, int DEPTH>
 hipError_t launch_few(const BlockLinear& p, hipStream_t stream) {
     const dim3 grid((uint32_t)((p.N + 16 * NT - 1) / (16 * NT)));
-    return p.x == nullptr ? enqueue(block_few_kernel<NT, DEPTH, true>, grid, dim3(SMALL_WAVES * 64), stream, p)
-                          : enqueue(block_few_kernel<NT, DEPTH, false>, grid, dim3(SMALL_WAVES * 64), stream, p);
+    return p.x == nullptr ? enqueue(block_few_kernel<NT, DEPTH, true>, grid, dim3(FEW_WAVES * 64), stream, p)
+                          : enqueue(block_few_kernel<NT, DEPTH, false>, grid, dim3(FEW_WAVES * 64), stream, p);
 }
 
-template <int NT, int DEPTH>
+template <int NT, int WAVES, int DEPTH>
 hipError_t launch_small(const BlockLinear& p, hipStream_t stream) {
     const dim3 grid((uint32_t)((p.N + 16 * NT - 1) / (16 * NT)), (uint32_t)((p.M + 15) / 16));
-    return p.x == nullptr ? enqueue(block_small_kernel<NT, DEPTH, true>, grid, dim3(SMALL_WAVES * 64), stream, p)
-                          : enqueue(block_small_kernel<NT, DEPTH, false>, grid, dim3(SMALL_WAVES * 64), stream, p);
+    return p.x == nullptr ? enqueue(block_small_kernel<NT, WAVES, DEPTH, true>, grid, dim3(WAVES * 64), stream, p)
+                          : enqueue(block_small_kernel<NT, WAVES, DEPTH, false>, grid, dim3(WAVES * 64), stream, p);
 }
 
 }  // namespace
@@ -733,16 +734,21 @@ namespace {
 // fifth nearly everywhere, and the shapes' order where it matters).
 constexpr int FEW_ROWS = 4;   // up to here quantizing into LDS first wins: 1 x 12288 x 2048 7.4 us, 8.0 where they are multiplied; 16 x 2048 x 16384 41 and 26
 enum Shape { SHAPE_SMALL, SHAPE_64_SPLIT, SHAPE_64, SHAPE_128, SHAPE_224 };
-// Weight tiles of a workgroup of the kernels for few tokens: about one workgroup per CU, each with all the weights that go with
-// the rows it quantizes.  16 x 16384 x 1024 12.3 / 8.8 / 6.3 us with 1 / 2 / 4, 32 x 2048 x 2048 6.0 / 6.7 / 8.5.
+// Weight tiles of a workgroup of the kernels for few tokens.  For up to FEW_ROWS one, or four once there are workgroups for every
+// CU all the same (two are never ahead): 1 x 8192 x 8192 15.1 us with one and 20.1 with four, 1 x 12288 x 2048 7.8 and 7.1.  Beyond,
+// about one workgroup per CU, each with all the weights that go with the rows it quantizes: 16 x 16384 x 1024 12.3 / 8.8 / 6.3 us with
+// 1 / 2 / 4, 32 x 2048 x 2048 6.0 / 6.7 / 8.5.
 int small_tiles(int64_t M, int64_t N) {
     const int64_t units = (N + 15) / 16 * ((M + 15) / 16);
-    if (M <= FEW_ROWS) return units < 384 ? 1 : units < 768 ? 2 : 4;
+    if (M <= FEW_ROWS) return units < 640 ? 1 : 4;
     return units <= 288 ? 1 : units <= 576 ? 2 : 4;
 }
+// Wavefronts of block_small_kernel: 16 for long K and one weight tile, whose instructions then fill the SIMDs' gaps: 14 x 896 x 7024 11.6 us
+// with 8 and 10.3 with 16, 50 x 1024 x 4096 9.5 and 8.7; 16 x 2560 x 1024 4.2 and 4.4.
+bool small_wide(int nt, int64_t K) { return nt == 1 && K >= 2048; }
 double small_cost(int64_t M, int64_t N, int64_t K) {
     const int nt = small_tiles(M, N);
-    const int64_t groups = ((N + 16 * nt - 1) / (16 * nt)) * ((M + 15) / 16), turns = (K + QB * SMALL_WAVES - 1) / (QB * SMALL_WAVES);
+    const int64_t groups = ((N + 16 * nt - 1) / (16 * nt)) * ((M + 15) / 16), turns = (K + QB * 8 - 1) / (QB * 8);
     return 2.6 + turns * (nt == 1 ? 1.5 : nt == 2 ? 2.05 : 3.1) * (groups <= 256 ? 1.0 : groups / 256.0);
 }
 // The quantizer, and a tile kernel: rounds of workgroups (one per CU, or two), each K block the dearer the more CUs are busy.
@@ -768,13 +774,15 @@ bool block_linear_small(int64_t M, int64_t N, int64_t K) { return choose(M, N, K
 
 hipError_t launch_block_linear_small(const BlockLinear& p, hipStream_t stream) {
     int nt = small_tiles(p.M, p.N);
-    bool few = p.M <= FEW_ROWS;
-    if (const char* forced = tuning_env("PHYAI_LAYER_SMALL")) {   // weight tiles of a workgroup; + 10: not the kernel of a few tokens
+    bool few = p.M <= FEW_ROWS, wide = small_wide(nt, p.K);
+    if (const char* forced = tuning_env("PHYAI_LAYER_SMALL")) {   // weight tiles of a workgroup; + 10: not the kernel of a few tokens; + 30: nor 8 wavefronts
         nt = atoi(forced) % 10;
         few = p.M <= 8 && atoi(forced) < 10;
+        wide = nt == 1 && atoi(forced) >= 30;
     }
-    if (few) return nt == 1 ? launch_few<1, 4>(p, stream) : nt == 2 ? launch_few<2, 4>(p, stream) : launch_few<4, 2>(p, stream);
-    return nt == 1 ? launch_small<1, 4>(p, stream) : nt == 2 ? launch_small<2, 4>(p, stream) : launch_small<4, 2>(p, stream);
+    if (few) return nt == 1 ? launch_few<1, 4>(p, stream) : launch_few<4, 2>(p, stream);
+    if (wide) return launch_small<1, 16, 2>(p, stream);
+    return nt == 1 ? launch_small<1, 8, 4>(p, stream) : nt == 2 ? launch_small<2, 8, 4>(p, stream) : launch_small<4, 8, 2>(p, stream);
 }
 
 hipError_t launch_block_gemm(const BlockLinear& p, hipStream_t stream) {
