@@ -19,6 +19,9 @@ constexpr int QB = 128;   // elements per scale
 constexpr float kBlockAmaxFloor = 1e-12f;
 
 __device__ __forceinline__ float block_scale(uint32_t amax_bits) {
+    // The maximum before and the shift here stay two instructions: as one that writes half a register (SDWA) its result was read
+    // too early where a single vector instruction lay between - the maximum of before, a scale of 1e-12 / 448, codes of NaN.
+    asm volatile("" : "+v"(amax_bits));
     const float a = bf16_bits_to_f32(amax_bits);
     return (a < kBlockAmaxFloor ? kBlockAmaxFloor : a) / kFp8Max;   // (a NaN stays one)
 }
@@ -743,9 +746,9 @@ int small_tiles(int64_t M, int64_t N) {
     if (M <= FEW_ROWS) return units < 640 ? 1 : 4;
     return units <= 288 ? 1 : units <= 576 ? 2 : 4;
 }
-// Wavefronts of block_small_kernel: 16 for long K and one weight tile, whose instructions then fill the SIMDs' gaps: 14 x 896 x 7024 11.6 us
-// with 8 and 10.3 with 16, 50 x 1024 x 4096 9.5 and 8.7; 16 x 2560 x 1024 4.2 and 4.4.
-bool small_wide(int nt, int64_t K) { return nt == 1 && K >= 2048; }
+// Wavefronts of block_small_kernel: 16 for long K and up to two weight tiles, whose instructions then fill the SIMDs' gaps: 14 x 896 x
+// 7024 11.6 us with 8 and 10.3 with 16, 50 x 1024 x 4096 9.5 and 8.7, 40 x 2048 x 4096 11.4 and 10.1; 16 x 2560 x 1024 4.2 and 4.4.
+bool small_wide(int nt, int64_t K) { return nt <= 2 && K >= 2048; }
 double small_cost(int64_t M, int64_t N, int64_t K) {
     const int nt = small_tiles(M, N);
     const int64_t groups = ((N + 16 * nt - 1) / (16 * nt)) * ((M + 15) / 16), turns = (K + QB * 8 - 1) / (QB * 8);
@@ -778,10 +781,10 @@ hipError_t launch_block_linear_small(const BlockLinear& p, hipStream_t stream) {
     if (const char* forced = tuning_env("PHYAI_LAYER_SMALL")) {   // weight tiles of a workgroup; + 10: not the kernel of a few tokens; + 30: nor 8 wavefronts
         nt = atoi(forced) % 10;
         few = p.M <= 8 && atoi(forced) < 10;
-        wide = nt == 1 && atoi(forced) >= 30;
+        wide = nt <= 2 && atoi(forced) >= 30;
     }
     if (few) return nt == 1 ? launch_few<1, 4>(p, stream) : launch_few<4, 2>(p, stream);
-    if (wide) return launch_small<1, 16, 2>(p, stream);
+    if (wide) return nt == 1 ? launch_small<1, 16, 2>(p, stream) : launch_small<2, 16, 1>(p, stream);
     return nt == 1 ? launch_small<1, 8, 4>(p, stream) : nt == 2 ? launch_small<2, 8, 4>(p, stream) : launch_small<4, 8, 2>(p, stream);
 }
 

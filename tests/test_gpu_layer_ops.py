@@ -79,7 +79,7 @@ SHAPES = [(1, 16, 16), (2, 144, 4224), (8, 272, 8304), (4, 64, 1072), (1, 256, 1
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
-@pytest.mark.parametrize("shape", [None, "few 1", "few 2", "few 4", "few 11", "few 12", "few 14", "few 31", "1", "2", "3", "4"])
+@pytest.mark.parametrize("shape", [None, "few 1", "few 2", "few 4", "few 11", "few 12", "few 14", "few 31", "few 32", "1", "2", "3", "4"])
 def test_block_linear(dev, monkeypatch, m, n, k, shape):
     if shape is not None:
         few, _, small = shape.partition(" ")
