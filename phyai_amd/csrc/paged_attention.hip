@@ -40,7 +40,11 @@ __device__ __forceinline__ v16f mfma(v4i a, v4i b, v16f c) {
 template <int TYPE>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
     if constexpr (TYPE == HEAD_BF16) return pack_bf16x2(a, b);
-    else return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)a) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)b) << 16;
+    else {   // (both at once: no instruction that writes half a register)
+        typedef float two __attribute__((ext_vector_type(2)));
+        typedef _Float16 pair __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(two{a, b}, pair));
+    }
 }
 template <int TYPE>
 __device__ __forceinline__ float to_f32(uint32_t h) {
