@@ -79,7 +79,7 @@ int phyai_layer_head_rope(const void *qkv, int64_t ld, const void *q_weight, con
  * window (window > 0).  out[t, h] = sum_j softmax_j(scale * q.k_j) v_j with key head h / (heads / kv_heads), zero if it
  * sees nothing; out: [T, heads, head_dim] dense.  Key j lies in token j % page_size of page page_table[b, j / page_size]
  * (table_stride between its rows; 0: one row for all).  Rows outside every sequence are left as they are; keys beyond the
- * table's width do not exist; a page number outside [0, n_pages) makes the rows that see its keys NaN.  K and V have the
+ * table's width do not exist (where the tokens stand goes by kv_lens all the same); a page number outside [0, n_pages) makes the rows that see its keys NaN.  K and V have the
  * same strides (elements: page, token, head).
  * Sums, maxima and products' sums are fp32; probabilities are rounded to the element type for the second product.
  * Limits: head_dim a multiple of 8 up to 256; strides multiples of 8; pointers 16-byte aligned; scale > 0; T * heads and

@@ -102,7 +102,8 @@ __device__ __forceinline__ int sum_up_to_lane(int v) {
 // Where a tile of `rows_per_tile` packed rows lies: the tiles of the sequences are numbered one sequence after another.
 // Every wavefront finds it by itself, 64 sequences at a time.
 struct Tile {
-    int b, row0, rows, q_begin, q_len, kv_len;
+    int b, row0, rows, q_begin, q_len;
+    int length, kv_len;   // keys as stated, which is where the tokens stand, and those of them that the table has room for
 };
 __device__ __forceinline__ bool locate(const PagedAttention& p, int group, int rows_per_tile, int tile, Tile& o) {   // (rows_per_tile: a power of two)
     const int lane = threadIdx.x & 63;
@@ -127,7 +128,8 @@ __device__ __forceinline__ bool locate(const PagedAttention& p, int group, int r
             o.row0 = (tile - before - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(tiles, l))) * rows_per_tile;
             const int64_t most = (int64_t)p.table_width * p.page_size;
             kv = __builtin_amdgcn_readlane(kv, l);
-            o.kv_len = kv < 0 ? 0 : kv > most ? (int)most : kv;
+            o.length = kv < 0 ? 0 : kv;
+            o.kv_len = o.length > most ? (int)most : o.length;
             return true;
         }
         before += __builtin_amdgcn_readlane(upto, 63);
@@ -476,7 +478,7 @@ __device__ __forceinline__ Row row_of(const PagedAttention& p, const Tile& t, co
     const int i = r.valid ? divide(row, g.group) : 0;
     r.token = t.q_begin + i;
     r.head = kv_head * g.group_size + (r.valid ? row - i * g.group_size : 0);
-    const int position = t.kv_len - t.q_len + i;
+    const int position = t.length - t.q_len + i;
     r.hi = !r.valid ? 0 : p.causal ? clamp_i(position + 1, 0, t.kv_len) : t.kv_len;
     r.lo = p.window > 0 && position >= p.window ? position - p.window + 1 : 0;
     return r;
@@ -484,7 +486,7 @@ __device__ __forceinline__ Row row_of(const PagedAttention& p, const Tile& t, co
 // First and last + 1 key that any of the rows row0 .. row1 sees, and that all of them see.
 __device__ __forceinline__ void span_of(const PagedAttention& p, const Tile& t, const Plan& g, int row0, int row1, int& lo, int& hi, int& all_lo, int& all_hi) {
     const int i0 = divide(row0, g.group), i1 = divide(row1, g.group);
-    const int position0 = t.kv_len - t.q_len + i0, position1 = t.kv_len - t.q_len + i1;
+    const int position0 = t.length - t.q_len + i0, position1 = t.length - t.q_len + i1;
     lo = p.window > 0 && position0 >= p.window ? position0 - p.window + 1 : 0;
     hi = p.causal ? clamp_i(position1 + 1, 0, t.kv_len) : t.kv_len;
     lo = lo < hi ? lo : hi;

@@ -918,7 +918,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     (``[B + 1]`` int32).  ``k_pages`` / ``v_pages``: ``[pages, page_size, kv_heads, head_dim]`` with equal strides; key j of
     sequence b is token ``j % page_size`` of page ``page_table[b, j // page_size]`` (``[B, width]`` int32), ``kv_lens[b]``
     (``[B]`` int32) of them.  The new tokens are the last of these: token i stands at ``kv_lens[b] - tokens + i`` and sees
-    keys up to its own (``causal``), or all, and with ``window`` none that lie ``window`` or more before it.  Query head h
+    keys up to its own (``causal``), or all, and with ``window`` none that lie ``window`` or more before it; keys beyond the
+    table's width do not exist, which moves no token.  Query head h
     reads key head ``h // (heads // kv_heads)``.  ``scale`` defaults to ``head_dim ** -0.5``.
 
     Returns ``[T, heads, head_dim]``; a row that sees nothing is zero, rows outside every sequence are left as they were
