@@ -77,7 +77,7 @@ int phyai_layer_head_rope(const void *qkv, int64_t ld, const void *q_weight, con
  * heads, head_dim], strides in elements) and kv_lens[b] keys, its new tokens' among them: new token i stands at position
  * p = kv_lens[b] - (q_offsets[b + 1] - q_offsets[b]) + i and sees the keys j < kv_lens[b] with j <= p (causal) and j > p -
  * window (window > 0).  out[t, h] = sum_j softmax_j(scale * q.k_j) v_j with key head h / (heads / kv_heads), zero if it
- * sees nothing; out: [T, heads, head_dim] dense.  Key j lies in token j % page_size of page page_table[b, j / page_size]
+ * sees nothing and NaN if it sees only scores of -inf; out: [T, heads, head_dim] dense.  Key j lies in token j % page_size of page page_table[b, j / page_size]
  * (table_stride between its rows; 0: one row for all).  Rows outside every sequence are left as they are; keys beyond the
  * table's width do not exist (where the tokens stand goes by kv_lens all the same); a page number outside [0, n_pages) makes the rows that see its keys NaN.  K and V have the
  * same strides (elements: page, token, head).

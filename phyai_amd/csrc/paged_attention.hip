@@ -7,7 +7,8 @@
 // the lane 32 further) and the softmax needs a single exchange; P^T then lies in the registers exactly as the B operand of
 // O^T = V^T P^T wants it, if V's keys are taken in the same order - which the transposing LDS read is free to do - and m,
 // l and the rescaling of O are one value per lane.  O is only rescaled when a row's maximum grows by more than 2^8:
-// probabilities stay below 2^8, which neither bf16, fp16 nor the fp32 sums mind.
+// probabilities stay below 2^8, which neither bf16, fp16 nor the fp32 sums mind.  A row that sees keys, but none with a score
+// above -inf, is NaN, as its softmax is.
 //
 // Keys and values are copied from their pages straight into LDS.  16-byte chunk c of key r lies in slot c ^ f(r), with an
 // f of its own for K (sixteen neighbouring keys, one chunk: sixteen bank groups) and for V (four keys, four chunks).
@@ -26,6 +27,7 @@ typedef _Float16 v8hf __attribute__((ext_vector_type(8)));
 
 constexpr int ROWS = 32;               // rows of a wavefront's tile
 constexpr float kNone = -__builtin_huge_valf();
+constexpr float kLowest = -3.40282347e38f;   // maximum of a row part whose keys all have a score of -inf, where kNone is one that sees no key
 constexpr float kRescaleAt = 8.0f;     // log2 of how far a row's maximum may grow before O is rescaled
 
 // Sixteen bytes of zeros and of NaNs: where copies of keys that do not exist and of pages that do not exist come from.
@@ -540,6 +542,8 @@ struct SplitShape {
     static constexpr int OLD = DP + 4;                            // floats of a row of O in LDS
     static constexpr int WAVE_BYTES = STAGE > 32 * OLD * 4 ? STAGE : 32 * OLD * 4;
 };
+// What a row's O is divided by, inverted: a sum of zero is a row's that sees nothing, or only scores of -inf.
+__device__ __forceinline__ float one_over(float sum, bool sees) { return sum != 0.f ? 1.0f / sum : sees ? __builtin_nanf("") : 0.f; }
 // How much of a state with maximum m belongs into one with the larger maximum `all` (m = -inf: it has seen nothing, or NaN).
 __device__ __forceinline__ float share(float m, float l, float all) { return m == kNone ? (l != l ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(m - all); }
 
@@ -610,7 +614,8 @@ __global__ __launch_bounds__(SplitShape<DP>::WAVES * 64, 1) void attend_split_ke
             *reinterpret_cast<v4f*>(o + (lane & 31) * X::OLD + 32 * b + 8 * i + 4 * (lane >> 5)) = v;
         }
     if (lane < 32) {
-        ml[wave][lane][0] = st.m;
+        const int from = row.lo > begin * 32 ? row.lo : begin * 32, to = row.hi < end * 32 ? row.hi : end * 32;
+        ml[wave][lane][0] = st.m == kNone && l == 0.f && from < to ? kLowest : st.m;
         ml[wave][lane][1] = l;
     }
     __syncthreads();
@@ -626,7 +631,7 @@ __global__ __launch_bounds__(SplitShape<DP>::WAVES * 64, 1) void attend_split_ke
             a[w] = share(ml[w][lane][0], ml[w][lane][1], m);
             sum = __builtin_fmaf(ml[w][lane][1], a[w], sum);
         }
-        const float by = g.splits > 1 ? 1.0f : sum == 0.f ? 0.f : 1.0f / sum;
+        const float by = g.splits > 1 ? 1.0f : one_over(sum, m != kNone);
 #pragma unroll
         for (int w = 0; w < X::WAVES; ++w) weight[w][lane] = a[w] * by;
         if (g.splits > 1 && row.valid)
@@ -692,7 +697,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const PagedAttention p
 #pragma unroll
     for (int x = 1; x < QUADS; x <<= 1) sum += __shfl_xor(sum, x);
     __syncthreads();
-    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    const float inv = one_over(sum, m != kNone);
     v4f v = {0, 0, 0, 0};
     for (int z = 0; z < g.splits; z += AHEAD) {
         if (z > 0) {
@@ -789,7 +794,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
         }
     }
     const float l = other_half_sum(st.l);
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    const float inv = one_over(l, row.lo < row.hi);
     if (!row.valid) return;
     uint16_t* out = p.out + ((int64_t)row.token * p.H + row.head) * p.D;
 #pragma unroll

@@ -922,7 +922,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     table's width do not exist, which moves no token.  Query head h
     reads key head ``h // (heads // kv_heads)``.  ``scale`` defaults to ``head_dim ** -0.5``.
 
-    Returns ``[T, heads, head_dim]``; a row that sees nothing is zero, rows outside every sequence are left as they were
+    Returns ``[T, heads, head_dim]``; a row that sees nothing is zero, one whose scores are all -inf is NaN, rows outside every sequence are left as they were
     (of a fresh result: undefined), and rows that see keys of a page that does not exist are NaN."""
     op = "paged_attention"
     got = _native().paged_attention(q, k_pages, v_pages, page_table, q_offsets, kv_lens, scale, causal, window, out)

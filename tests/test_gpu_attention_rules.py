@@ -76,3 +76,21 @@ def test_a_token_stands_where_the_stated_length_puts_it(dev, monkeypatch, plan, 
     q = seeded((60, 4, 64), 4)
     want, bound = by_the_text(q, k, v, table, offsets, lens, causal=causal, window=window)
     within(attend(dev, q, k, v, table, offsets, lens, causal=causal, window=window), want, bound, f"{causal} {window}")
+
+
+@pytest.mark.parametrize("plan", ["0", "1", "3", "64"])
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 64), (torch.float16, 128), (torch.bfloat16, 256)])
+def test_a_row_that_sees_only_infinitely_low_scores_has_no_softmax(dev, monkeypatch, plan, dtype, d):
+    """The softmax of scores that are all -inf is NaN, in 64 bits as here; one finite score makes theirs weightless.  Only a row
+    that sees no key is zero."""
+    monkeypatch.setenv("PHYAI_LAYER_ATTEND", plan)
+    k, v, table = cache([200, 3, 0], 16, 1, d, dtype, 5)
+    for b, low in ((0, 140), (1, 3)):
+        for j in range(low):
+            k[table[b, j // 16].long(), j % 16] = -math.inf
+    lens = torch.tensor([200, 3, 0], dtype=torch.int32)
+    offsets = torch.tensor([0, 200, 205, 207], dtype=torch.int32)   # the second sequence's first two tokens stand in front of its keys
+    q = (seeded((207, 2, d), 6).abs() + 0.1).to(dtype)
+    want, bound = by_the_text(q, k, v, table, offsets, lens)
+    assert want[:140].isnan().all() and want[202:205].isnan().all() and not want[200:202].any() and not want[140:200].isnan().any()
+    within(attend(dev, q, k, v, table, offsets, lens), want, bound, "rows")
