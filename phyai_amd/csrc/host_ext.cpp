@@ -146,7 +146,7 @@ bool workspace(size_t need, const Where& w, Scratch* s) {
     const bool shared = owner == nullptr || owner == Py_None;
     Py_XDECREF(owner);
     if (shared) {
-        PyObject* key = Py_BuildValue("iK", (int)w.dev.index(), (unsigned long long)reinterpret_cast<uintptr_t>(w.stream));
+        PyObject* key = Py_BuildValue("iKk", (int)w.dev.index(), (unsigned long long)reinterpret_cast<uintptr_t>(w.stream), PyThread_get_thread_ident());
         if (!key) return false;
         const at::Tensor* t = tensor(PyDict_GetItemWithError(py.workspaces, key));
         Py_DECREF(key);

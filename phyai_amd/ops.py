@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import contextlib
 import contextvars
+import sys
 import threading
 
 import torch
@@ -77,14 +78,18 @@ def _as_rows(op: str, x: torch.Tensor, name: str, dtype: torch.dtype) -> torch.T
 # ---- workspace --------------------------------------------------------------
 # Scratch of the GEMM (split-K counters and partial sums) and of the whole-linear entry points
 # (activation codes and per-token scales): zero-initialised byte tensors whose header the kernels
-# keep zero between calls.  Eager calls share one tensor per (device, stream).  A HIP graph bakes
+# keep zero between calls.  Eager calls share one tensor per (device, stream, thread): what a thread
+# enqueues between taking a workspace and its last launch is then in order on the stream, also where
+# another thread uses the same one (with one tensor for both, its launches could come between a
+# quantizer and the GEMM that reads its codes; the GIL is released there).  A thread that has ended
+# leaves its tensors to the next one on that stream.  A HIP graph bakes
 # the addresses it was recorded with into its kernel nodes, so a graph owns its workspace
 # (`WorkspaceOwner`, entered by `HipGraph.capture` around warm-up and recording): it lives as long
 # as the graph and is shared with nobody - not with eager work that later runs on the pooled
 # stream the graph was recorded on, not with other graphs.  A workspace that has to grow is
 # replaced, never freed while anything may still hold its address: the old tensor stays with its
 # owner (or, for the eager ones, in `_retired` until the process ends).
-_workspaces: dict[tuple[int, int], torch.Tensor] = {}
+_workspaces: dict[tuple[int, int, int], torch.Tensor] = {}
 _retired: list[torch.Tensor] = []
 
 
@@ -101,7 +106,7 @@ _owner: contextvars.ContextVar[WorkspaceOwner | None] = contextvars.ContextVar("
 
 @contextlib.contextmanager
 def workspace_owner(owner: WorkspaceOwner):
-    """Calls inside the scope take their workspace from ``owner`` instead of the per-stream table."""
+    """Calls inside the scope take their workspace from ``owner`` instead of the table of eager ones."""
     token = _owner.set(owner)
     try:
         yield owner
@@ -184,14 +189,29 @@ def describe_linear_plan(M: int, N: int, K: int, epilogue=EPI_NONE, weight_layou
     return buf.value.decode()
 
 
+def _left_behind(key: tuple[int, int, int]) -> torch.Tensor | None:
+    """The workspace of a thread that no longer runs, on the same stream: what it launched there comes before anything
+    this thread launches."""
+    running = sys._current_frames()   # (a thread that is inside a call has a frame)
+    for other in list(_workspaces):
+        if other[:2] == key[:2] and other[2] not in running:
+            ws = _workspaces.pop(other, None)
+            if ws is not None:
+                return ws
+    return None
+
+
 def reserve_workspace(nbytes: int, device: torch.device | None = None) -> torch.Tensor:
-    """Make sure the workspace in scope on ``device`` (the enclosing graph's, else the current
-    stream's) holds ``nbytes``."""
+    """Make sure the workspace in scope on ``device`` (the enclosing graph's, else this thread's
+    on the current stream) holds ``nbytes``."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     idx = dev.index if dev.index is not None else torch.cuda.current_device()
     owner = _owner.get()
-    store, key, retired = (owner.tensors, idx, owner.retired) if owner is not None else (_workspaces, (idx, _stream_ptr()), _retired)
+    store, key, retired = (owner.tensors, idx, owner.retired) if owner is not None else (
+        _workspaces, (idx, _stream_ptr(), threading.get_ident()), _retired)
     ws = store.get(key)
+    if ws is None and owner is None and (ws := _left_behind(key)) is not None:
+        store[key] = ws
     if ws is None or ws.numel() < nbytes:
         # Outside capture this is a one-off allocation.  Inside a capture (an op met for the first
         # time while recording) the tensor comes from the graph's memory pool and the zero fill is
@@ -922,8 +942,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     table's width do not exist, which moves no token.  Query head h
     reads key head ``h // (heads // kv_heads)``.  ``scale`` defaults to ``head_dim ** -0.5``.
 
-    Returns ``[T, heads, head_dim]``; a row that sees nothing is zero, one whose scores are all -inf is NaN, rows outside every sequence are left as they were
-    (of a fresh result: undefined), and rows that see keys of a page that does not exist are NaN."""
+    Returns ``[T, heads, head_dim]``; a row that sees nothing is zero, one whose scores are all -inf is NaN, rows outside every
+    sequence are left as they were (of a fresh result: undefined), and rows that see keys of a page that does not exist are NaN."""
     op = "paged_attention"
     got = _native().paged_attention(q, k_pages, v_pages, page_table, q_offsets, kv_lens, scale, causal, window, out)
     if got is not None:
