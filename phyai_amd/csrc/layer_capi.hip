@@ -214,7 +214,8 @@ int phyai_layer_paged_attention(const void* q, int64_t q_token_stride, int64_t q
     if (heads % kv_heads != 0) return fail(PHYAI_FP8_EINVAL, "%s: heads=%lld must be a multiple of kv_heads=%lld", fn, (long long)heads, (long long)kv_heads);
     if (head_dim % 8 != 0 || head_dim > 256) return fail(PHYAI_FP8_EUNSUPPORTED, "%s: head_dim=%lld must be a multiple of 8 up to 256", fn, (long long)head_dim);
     if (type != PHYAI_LAYER_BF16 && type != PHYAI_LAYER_F16) return fail(PHYAI_FP8_EINVAL, "%s: unknown type %d", fn, type);
-    if (!(scale > 0.f) || isinf(scale)) return fail(PHYAI_FP8_EINVAL, "%s: scale must be a positive number", fn);
+    if (!(scale > 0.f) || isinf(scale * 1.4426950408889634f))   // (scores are taken to base 2)
+        return fail(PHYAI_FP8_EINVAL, "%s: scale must be a positive number, and times log2(e) a finite one", fn);
     if (window < 0) return fail(PHYAI_FP8_EINVAL, "%s: window=%lld must not be negative", fn, (long long)window);
     if (T == 0 || batch == 0) return PHYAI_FP8_OK;
     if (!q || !out || !q_offsets || !kv_lens) return fail(PHYAI_FP8_EINVAL, "%s: null pointer", fn);
