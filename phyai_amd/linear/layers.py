@@ -24,7 +24,7 @@ import torch.nn as nn
 from phyai_amd import ops
 from phyai_amd.linear.dispatch import get_linear_dispatcher
 from phyai_amd.quant import AllocationRequest, Bf16Spec
-from phyai_amd.quant.types import ActivationView
+from phyai_amd.quant.types import ActivationView, Granularity
 from phyai_amd.state import current_mode
 
 
@@ -119,7 +119,7 @@ class LinearBase(nn.Module):
             if isinstance(p, nn.Parameter):
                 p.hf_keys = [(f"{base}.{name}", sid) for base, sid in legs]
                 p.optional = True
-                if p.dim() == 2:
+                if name == "weight_scale" and p.dim() == 2 and getattr(self.spec, "granularity", None) is Granularity.BLOCK:
                     # one scale per block of the weight; checkpoints call it weight_scale or weight_scale_inv, of the same meaning
                     p.hf_keys += [(f"{base}.{name}_inv", sid) for base, sid in legs]
                     p.weight_loader = W.fused_blocks(offsets, self.output_size_per_partition // p.shape[0]) if fused else W.replicated()
