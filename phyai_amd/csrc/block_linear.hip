@@ -19,10 +19,7 @@ constexpr int QB = 128;   // elements per scale
 constexpr float kBlockAmaxFloor = 1e-12f;
 
 __device__ __forceinline__ float block_scale(uint32_t amax_bits) {
-    // The maximum before and the shift here stay two instructions: as one that writes half a register (SDWA) its result was read
-    // too early where a single vector instruction lay between - the maximum of before, a scale of 1e-12 / 448, codes of NaN.
-    asm volatile("" : "+v"(amax_bits));
-    const float a = bf16_bits_to_f32(amax_bits);
+    const float a = bf16_max_to_f32(amax_bits);
     return (a < kBlockAmaxFloor ? kBlockAmaxFloor : a) / kFp8Max;   // (a NaN stays one)
 }
 

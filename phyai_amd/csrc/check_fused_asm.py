@@ -28,6 +28,13 @@ instruction may read an SGPR only five wait states after a VALU instruction wrot
 for its own instructions but does not look inside the inline assembly of the global -> LDS copies, in front of which
 it may put a ``v_readlane`` (a spilled SGPR read back) or ``v_readfirstlane`` of their base pointer.  It disassembles
 the code objects of the built library and follows every path through every kernel.
+
+It also reports instructions that write half a register where that has been seen to go wrong or is as close to it: a
+``v_max_u32_sdwa ... dst_sel:WORD_1`` whose result was read one wait state later - what the compiler keeps between the two -
+gave the register's old value.  So no kernel may have an SDWA write of a part of a register at all (bf16_max_to_f32 keeps the
+compiler from it), and a vector or matrix instruction reads a register whose half a conversion has written (``op_sel``, what
+the fp8 encoders use) two wait states later or more.  Stores and LDS writes of such a register follow at once in kernels
+that are checked byte for byte; they may.
 """
 
 from __future__ import annotations
@@ -273,11 +280,54 @@ def sgpr_problems(function: str) -> tuple[list[str], int]:
             for i, n in sorted(bad.items())], memory
 
 
+HALF_SETTLES = 2   # wait states from a conversion into half of a register to a vector instruction that reads it
+_PART = re.compile(r"dst_sel:(?!DWORD\b)\w+")
+_UPPER = re.compile(r"op_sel:\[(?:[01],)+1\]")
+
+
+def half_problems(function: str) -> list[str]:
+    """SDWA writes of a part of a register in one disassembled function, and vector instructions that read a register too soon
+    behind a conversion into its upper half, over all ways there."""
+    if "dst_sel" not in function and "op_sel" not in function:
+        return []
+    lines = [line.split("//")[0].strip() for line in function.split("\n")]
+    name, code = lines[0].rstrip(":"), [t for t in lines[1:] if t]
+    label = {t[1:-2]: i for i, t in enumerate(code) if t.startswith("<") and t.endswith(">:")}
+    bad = {}
+
+    def reads(t: str) -> set[int]:
+        first, _, rest = t.partition(" ")[2].partition(",")
+        return _vgprs(rest)
+
+    def follow(i: int, left: int, written: set[int]) -> None:
+        while i < len(code) and left > 0:
+            t = code[i]
+            op, _, operands = t.partition(" ")
+            if not t.startswith("<"):
+                if op.startswith("v_") and reads(t) & written:
+                    bad[i] = f"{name}: `{t}` reads half a register less than {HALF_SETTLES} wait states behind its write"
+                if op.startswith("s_cbranch") or op == "s_branch":
+                    follow(label[operands.strip()], left - 1, written)
+                if op in ("s_branch", "s_endpgm"):
+                    return
+                left -= int(operands, 0) + 1 if op == "s_nop" else 1
+            i += 1
+
+    for i, t in enumerate(code):
+        if not t.startswith("v_"):
+            continue
+        if _PART.search(t):
+            bad[i] = f"{name}: `{t}` writes a part of a register"
+        elif t.startswith("v_cvt_") and _UPPER.search(t):
+            follow(i + 1, HALF_SETTLES, _vgprs(t.partition(" ")[2].split(",")[0]))
+    return [bad[i] for i in sorted(bad)]
+
+
 def check_disassembly(text: str) -> tuple[list[str], int, int]:
     """Problems, functions, vector-memory instructions."""
     functions = functions_of(text)
     results = [sgpr_problems(f) for f in functions]
-    return [p for bad, _ in results for p in bad], len(functions), sum(n for _, n in results)
+    return [p for bad, _ in results for p in bad] + [p for f in functions for p in half_problems(f)], len(functions), sum(n for _, n in results)
 
 
 def disassemble(library: str) -> list[str]:

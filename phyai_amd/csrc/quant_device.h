@@ -27,6 +27,13 @@ __device__ __forceinline__ uint32_t absmax_finish(uint32_t m2) {
     const uint32_t lo = m2 & 0xFFFFu, hi = m2 >> 16;
     return lo > hi ? lo : hi;
 }
+// The value of a maximum kept as bf16 bits.  The maximum before and the shift here stay two instructions: as one that writes
+// half a register (SDWA) its result was read too early where a single vector instruction lay between - the maximum of before,
+// in a quantizer a scale of 1e-12 / 448 and codes of NaN.
+__device__ __forceinline__ float bf16_max_to_f32(uint32_t bits) {
+    asm volatile("" : "+v"(bits));
+    return bf16_bits_to_f32(bits);
+}
 __device__ __forceinline__ uint32_t absmax8(uint4 q, uint32_t m) {
     const uint32_t r = absmax_finish(absmax8_pk(q, 0u));
     return r > m ? r : m;
@@ -191,7 +198,7 @@ __device__ __forceinline__ float scale_from_amax_bits(uint32_t amax_bits) {
         // (an Inf or NaN amax gives the same Inf or NaN either way)
         return bf16_bits_to_f32(f32_to_bf16_bits(bf16_bits_to_f32(amax_bits) * (1.0f / kFp8Max)));
     } else {
-        float s = bf16_bits_to_f32(amax_bits) / kFp8Max;
+        float s = bf16_max_to_f32(amax_bits) / kFp8Max;
         return s >= 1.17549435e-38f ? s : 1.17549435e-38f;
     }
 }
