@@ -82,7 +82,8 @@ int phyai_layer_head_rope(const void *qkv, int64_t ld, const void *q_weight, con
  * table's width do not exist (where the tokens stand goes by kv_lens all the same); a page number outside [0, n_pages) makes the rows that see its keys NaN.  K and V have the
  * same strides (elements: page, token, head).
  * Sums, maxima and products' sums are fp32; probabilities are rounded to the element type for the second product.
- * Limits: head_dim a multiple of 8 up to 256; strides multiples of 8; pointers 16-byte aligned; scale and scale * log2(e) positive and finite; T * heads and
+ * Limits: head_dim a multiple of 8 up to 256; strides multiples of 8; pointers 16-byte aligned; scale and scale * log2(e)
+ * positive and finite; T * heads and
  * page_table's width * page_size below 2^30.
  * Workspace as for phyai_layer_block_linear; max_kv: table width * page_size.
  */

@@ -860,7 +860,7 @@ def qk_norm_rope(qkv: torch.Tensor, cos_sin: torch.Tensor, positions: torch.Tens
     ``k_weight`` (``[head_dim]``, both or neither): RMSNorm of every head with that weight (``1 + weight`` with ``gemma``).
     ``cos_sin``: ``[table, rot]`` fp32 (:func:`rope_table`), the angles of the first ``rot`` elements of a head at each
     position; pairs are ``(i, i + rot / 2)`` or, ``interleaved``, ``(2 i, 2 i + 1)``.  ``positions``: ``[T]`` int64; one
-    outside the table turns its token into NaNs.
+    outside the table turns the rotated elements of its token's query and key into NaNs (the others know no position).
 
     With ``k_pages`` / ``v_pages`` (``[pages, page_size, num_kv_heads, head_dim]``) and ``slots`` (``[T]`` int64, page *
     page_size + place) keys and values go into the cache and ``(q, None)`` is returned; a slot outside the cache (-1: padding)
@@ -941,6 +941,10 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     keys up to its own (``causal``), or all, and with ``window`` none that lie ``window`` or more before it; keys beyond the
     table's width do not exist, which moves no token.  Query head h
     reads key head ``h // (heads // kv_heads)``.  ``scale`` defaults to ``head_dim ** -0.5``.
+
+    Sums and maxima are fp32; probabilities are rounded to the element type for the second product and summed as rounded, which
+    puts the result about half a step of the type further from exact (of the weighted values' magnitudes; relative 0.0022 against
+    0.0017 over thousands of keys in bf16).
 
     Returns ``[T, heads, head_dim]``; a row that sees nothing is zero, one whose scores are all -inf is NaN, rows outside every
     sequence are left as they were (of a fresh result: undefined), and rows that see keys of a page that does not exist are NaN."""
