@@ -43,6 +43,7 @@ int phyai_layer_block_gemm(const void *xq, const float *x_scale, int64_t xs_row,
 
 /*
  * Both as one call.  Few token rows: one kernel, no workspace (phyai_layer_block_linear_workspace_bytes() says 0).
+ * out must not overlap x (of few rows some are read while others are written).
  * Otherwise codes and scales go through the workspace, behind its first PHYAI_FP8_WORKSPACE_HEADER_BYTES (which this
  * call leaves alone); 256-byte aligned, not shared by calls that may overlap.
  */
@@ -59,7 +60,7 @@ enum { PHYAI_LAYER_BF16 = 0, PHYAI_LAYER_F16 = 1 };
  *     n = x * rsqrt(mean(x^2) + eps) * w   (w + 1 with gemma != 0; weights NULL: n = x),
  * then its first rot elements are turned by the angles of row positions[t] of cos_sin ([table_rows, rot] fp32: rot / 2
  * cosines, then rot / 2 sines), pair i being elements (i, i + rot / 2), or (2 i, 2 i + 1) with interleaved != 0; fp32
- * throughout, one rounding.  A position outside the table turns its token's query and key into NaNs.
+ * throughout, one rounding.  A position outside the table turns those elements of its token's query and key into NaNs.
  * q_out: [T, heads, head_dim].  With k_out ([T, kv_heads, head_dim]) keys go there and values nowhere; with k_out NULL keys
  * and values go to k_pages / v_pages (strides in elements: page, token, head): token t to token slots[t] % page_size of
  * page slots[t] / page_size.  A slot outside [0, n_pages * page_size) is not written (padding); slots must differ, and
@@ -77,14 +78,13 @@ int phyai_layer_head_rope(const void *qkv, int64_t ld, const void *q_weight, con
  * heads, head_dim], strides in elements) and kv_lens[b] keys, its new tokens' among them: new token i stands at position
  * p = kv_lens[b] - (q_offsets[b + 1] - q_offsets[b]) + i and sees the keys j < kv_lens[b] with j <= p (causal) and j > p -
  * window (window > 0).  out[t, h] = sum_j softmax_j(scale * q.k_j) v_j with key head h / (heads / kv_heads), zero if it
- * sees nothing and NaN if it sees only scores of -inf; out: [T, heads, head_dim] dense.  Key j lies in token j % page_size of page page_table[b, j / page_size]
- * (table_stride between its rows; 0: one row for all).  Rows outside every sequence are left as they are; keys beyond the
- * table's width do not exist (where the tokens stand goes by kv_lens all the same); a page number outside [0, n_pages) makes the rows that see its keys NaN.  K and V have the
- * same strides (elements: page, token, head).
+ * sees nothing and NaN if it sees only scores of -inf; out: [T, heads, head_dim] dense.  Key j lies in token j % page_size of
+ * page page_table[b, j / page_size] (table_stride between its rows; 0: one row for all).  Rows outside every sequence are left
+ * as they are; keys beyond the table's width do not exist (where the tokens stand goes by kv_lens all the same); a page number
+ * outside [0, n_pages) makes the rows that see its keys NaN.  K and V have the same strides (elements: page, token, head).
  * Sums, maxima and products' sums are fp32; probabilities are rounded to the element type for the second product.
  * Limits: head_dim a multiple of 8 up to 256; strides multiples of 8; pointers 16-byte aligned; scale and scale * log2(e)
- * positive and finite; T * heads and
- * page_table's width * page_size below 2^30.
+ * positive and finite; T * heads and page_table's width * page_size below 2^30.
  * Workspace as for phyai_layer_block_linear; max_kv: table width * page_size.
  */
 size_t phyai_layer_paged_attention_workspace_bytes(int64_t T, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,

@@ -161,7 +161,7 @@ struct Pool {
     const uint8_t *zero, *nan;
     const int32_t* table;              // the sequence's pages
     int64_t page_bytes, token_bytes;
-    int n_pages, page_size, kv_len, table_width;
+    int n_pages, page_size, kv_len;
     Division by_page;
     int d_chunks;                      // 16-byte chunks of a key that exist
     bool neat;                         // runs of eight keys are neighbours in a page, and a key fills a row of LDS
@@ -523,7 +523,6 @@ __device__ __forceinline__ Pool make_pool(const PagedAttention& p, const Tile& t
     s.kv_len = t.kv_len;
     s.by_page = g.page;
     s.table = p.table + (int64_t)t.b * p.table_ld;
-    s.table_width = p.table_width;
     s.d_chunks = p.D / 8;
     s.neat = p.D == DP && p.page_size % 8 == 0;
     return s;
