@@ -35,7 +35,8 @@ int phyai_layer_block_quant(const void *x, int64_t ldx, int64_t M, int64_t K, vo
  * w: [N, K] e4m3fn bytes, dense, 16-byte aligned; w_scale: [ceil(N / 128), ceil(K / 128)] fp32, dense; x_scale as above
  * (xs_block = 0: one scale per row); bias: [N] bf16 or NULL; out: [M, N] bf16, row stride ldo (a multiple of 4), 8-byte
  * aligned.  N % 16 == 0 and K % 16 == 0.  Products of one block are summed by the matrix units (of eight neighbouring
- * k, what lies more than 13 bits below the largest product is cut off by the hardware), blocks in fp32.
+ * k, what lies more than 13 bits below the largest product is cut off by the hardware), blocks in fp32.  out must not
+ * overlap xq.
  */
 int phyai_layer_block_gemm(const void *xq, const float *x_scale, int64_t xs_row, int64_t xs_block, const void *w,
                            const float *w_scale, const void *bias, void *out, int64_t ldo, int64_t M, int64_t N, int64_t K,
@@ -43,7 +44,7 @@ int phyai_layer_block_gemm(const void *xq, const float *x_scale, int64_t xs_row,
 
 /*
  * Both as one call.  Few token rows: one kernel, no workspace (phyai_layer_block_linear_workspace_bytes() says 0).
- * out must not overlap x (of few rows some are read while others are written).
+ * out must not overlap x there, since some rows are read while others are written.
  * Otherwise codes and scales go through the workspace, behind its first PHYAI_FP8_WORKSPACE_HEADER_BYTES (which this
  * call leaves alone); 256-byte aligned, not shared by calls that may overlap.
  */
@@ -82,6 +83,7 @@ int phyai_layer_head_rope(const void *qkv, int64_t ld, const void *q_weight, con
  * page page_table[b, j / page_size] (table_stride between its rows; 0: one row for all).  Rows outside every sequence are left
  * as they are; keys beyond the table's width do not exist (where the tokens stand goes by kv_lens all the same); a page number
  * outside [0, n_pages) makes the rows that see its keys NaN.  K and V have the same strides (elements: page, token, head).
+ * out may be q, token for token and head for head; it must not overlap it otherwise.
  * Sums, maxima and products' sums are fp32; probabilities are rounded to the element type for the second product.
  * Limits: head_dim a multiple of 8 up to 256; strides multiples of 8; pointers 16-byte aligned; scale and scale * log2(e)
  * positive and finite; T * heads and page_table's width * page_size below 2^30.

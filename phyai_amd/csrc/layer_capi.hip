@@ -57,6 +57,16 @@ int check_linear(const char* fn, const void* w, const float* w_scale, const void
     return 0;
 }
 
+// Do M rows of `a` bytes from p, `lda` bytes apart, and M of `b` bytes from q share memory?  Rows of equal strides may lie beside each
+// other in one buffer.
+bool overlap(const void* p, int64_t lda, int64_t a, const void* q, int64_t ldb, int64_t b, int64_t M) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(p), y = reinterpret_cast<uintptr_t>(q);
+    if (x + (uintptr_t)((M - 1) * lda + a) <= y || y + (uintptr_t)((M - 1) * ldb + b) <= x) return false;
+    if (M == 1 || lda != ldb) return true;
+    const int64_t off = y >= x ? (int64_t)((y - x) % (uintptr_t)lda) : lda - 1 - (int64_t)((x - y - 1) % (uintptr_t)lda);
+    return off < a || off + b > lda;
+}
+
 }  // namespace
 
 extern "C" {
@@ -85,6 +95,7 @@ int phyai_layer_block_gemm(const void* xq, const float* x_scale, int64_t xs_row,
     if (xs_row < 0 || xs_block < 0 || xs_row >= kMost || xs_block >= kMost ||
         ((M - 1) * xs_row + (blocks_of(K) - 1) * xs_block + 1) * 4 >= kMost)
         return fail(PHYAI_FP8_EUNSUPPORTED, "%s: strides of x_scale must not be negative and reach less than 2^29 elements", fn);
+    if (overlap(xq, K, K, out, ldo * 2, N * 2, M)) return fail(PHYAI_FP8_EINVAL, "%s: out overlaps xq", fn);
     phyai::BlockLinear p = {};
     p.xq = static_cast<const uint8_t*>(xq);
     p.ldq = K;
@@ -122,6 +133,8 @@ int phyai_layer_block_linear(const void* x, int64_t ldx, const void* w, const fl
     hipStream_t st = static_cast<hipStream_t>(stream);
     const uint16_t* rows = static_cast<const uint16_t*>(x);
     if (phyai::block_linear_small(M, N, K)) {
+        if (overlap(x, ldx * 2, K * 2, out, ldo * 2, N * 2, M))
+            return fail(PHYAI_FP8_EINVAL, "%s: out overlaps x, of whose few rows some are read while others are written", fn);
         p.x = rows;
         p.ldx = ldx;
         return launched(fn, phyai::launch_block_linear_small(p, st));

@@ -786,7 +786,7 @@ def fp8_block_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.
                      out: torch.Tensor | None = None) -> torch.Tensor:
     """The W8A8 linear of a checkpoint whose weights have one scale per block of 128 x 128 (``weight_block_size:
     [128, 128]``): :func:`fp8_block_quant` of bf16 ``x[..., K]`` and :func:`fp8_block_gemm` as one call, bf16 out.  Few
-    token rows are one kernel, which quantizes the rows it multiplies (same codes).
+    token rows are one kernel, which quantizes the rows it multiplies (same codes), so that ``out`` must not overlap ``x``.
 
     ``weight``: ``[N, K]`` e4m3fn; ``weight_scale``: ``[ceil(N / 128), ceil(K / 128)]`` fp32, what a code is multiplied
     with (called ``weight_scale_inv`` in some checkpoints); N and K are multiples of 16."""
