@@ -52,7 +52,7 @@ __device__ __forceinline__ void block_encode(uint4 (&v)[N], float s, uint2 (&cod
 
 // ---- the quantizer on its own -----------------------------------------------------------------------------------
 // Sixteen lanes a block, eight values (16 bytes) a lane; the block's maximum by four DPP steps inside the row of lanes.
-// One pass over the data, bound by memory: 13056 x 16384 in 112 us, 5.8 TB/s of reads and writes.
+// One pass over the data, bound by memory: 13056 x 16384 in 111 to 121 us, 5.3 to 5.8 TB/s of reads and writes.
 __global__ __launch_bounds__(256) void block_quant_kernel(const uint16_t* __restrict__ x, int64_t ldx, int K, int blocks, int64_t items,
                                                           uint8_t* __restrict__ xq, int64_t ldq, float* __restrict__ xs, int64_t xs_row,
                                                           int64_t xs_block) {
@@ -82,7 +82,7 @@ __global__ __launch_bounds__(256) void block_quant_kernel(const uint16_t* __rest
 // at a time (sixteen lanes a block of a row, as above), while the first weights are on their way; then its wavefronts take
 // the blocks of K in turn, each with its weights straight from memory in the MFMA's registers (lane q of a row: bytes
 // 16 q and 64 + 16 q), DEPTH blocks ahead.  The partial sums meet in LDS, added in wavefront order.  1 x 2560 x 1024: 3.5 us
-// in a graph, the launch and two trips to memory; 2 x 22656 x 5632: 34 us, 3.7 TB/s of weights.
+// in a graph, the launch and two trips to memory; 2 x 22656 x 5632: 36.5 us, 3.5 TB/s of weights.
 constexpr int FEW_WAVES = 8;
 
 template <int NT>
@@ -349,7 +349,7 @@ __global__ __launch_bounds__(WAVES * 64) void block_small_kernel(const BlockLine
 // copied straight into LDS; chunk c of row r lies in slot c ^ ((r >> 1) & 7), so the sixteen rows that a quarter of a
 // wavefront reads together are in sixteen different bank groups.  Copies go through buffer resources: rows past the
 // matrix repeat its last one, bytes past K arrive as zeros.  777 x 1168 x 4304: 12.9 us in 247 tiles of 64 x 64, one round of workgroups
-// that each wait for 17 steps; 2225 x 6912 x 2176 with its quantizer 56 us, 1.2 PFLOP/s.
+// that each wait for 17 steps; 2225 x 6912 x 2176 with its quantizer 51 us, 1.3 PFLOP/s.
 template <int TM, int TN, int WM, int WN, int WK, int DEPTH>
 struct BlockTile {
     static constexpr int BM = 16 * TM * WM, BN = 16 * TN * WN, WAVES = WM * WN;
@@ -524,8 +524,8 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void block_gemm_kernel(const Blo
 // products is the beginning: eight wavefronts behind a barrier that all want their first operands from LDS.  So the weight
 // fragments of a step are read at the end of the one before it - the stages of weights run one step further ahead than
 // those of tokens, in three buffers instead of two - and the last row block of a step is scaled and added behind the
-// barrier, while the first token fragment comes; the copies are issued between the products.  13056 x 2048 x 16384: 400 us, 2.2 PFLOP/s
-// with the MFMA busy 56 % of the time at the clock that the chip's power leaves.
+// barrier, while the first token fragment comes; the copies are issued between the products.  13056 x 2048 x 16384: 417 us, 2.1 PFLOP/s
+// with the MFMA busy 58 % of the time at the clock that the chip's power leaves.
 template <int TM>
 struct WideTile {
     static constexpr int TN = 4, WM = 2, WN = 4, WAVES = 8, BM = 32 * TM, BN = 256;
@@ -730,12 +730,14 @@ hipError_t launch_block_quant(const uint16_t* x, int64_t ldx, int64_t M, int64_t
 
 // ---- which kernel ---------------------------------------------------------------------------------------------------
 namespace {
-// Microseconds of M x N x K, as fitted to event-timed graphs of 60 shapes from 1 x 256 x 256 to 13056 x 32768 x 2048 (within a
-// fifth nearly everywhere, and the shapes' order where it matters).
+// Microseconds of M x N x K, as fitted to event-timed graphs of 60 shapes from 1 x 256 x 256 to 13056 x 32768 x 2048.  What they choose is
+// 0.7 % behind the best kernel in the geometric mean over 68 shapes of that range, three of them more than 8 % (100 x 2560 x 1024: 9.2 us
+// chosen, 7.6 in tiles of 64 x 64; 8 x 32768 x 2048 16.5 and 14.9); the microseconds themselves are within a fifth at 47 of 59 for
+// few tokens and at 249 of 272 for the tiles.
 constexpr int FEW_ROWS = 4;   // up to here quantizing into LDS first wins: 1 x 12288 x 2048 7.4 us, 8.0 where they are multiplied; 16 x 2048 x 16384 41 and 26
 enum Shape { SHAPE_SMALL, SHAPE_64_SPLIT, SHAPE_64, SHAPE_128, SHAPE_224 };
 // Weight tiles of a workgroup of the kernels for few tokens.  For up to FEW_ROWS one, or four once there are workgroups for every
-// CU all the same (two are never ahead): 1 x 8192 x 8192 15.1 us with one and 20.1 with four, 1 x 12288 x 2048 7.8 and 7.1.  Beyond,
+// CU all the same: 1 x 8192 x 8192 15.1 us with one and 20.1 with four, 1 x 12288 x 2048 7.8 and 7.1.  Beyond,
 // about one workgroup per CU, each with all the weights that go with the rows it quantizes: 16 x 16384 x 1024 12.3 / 8.8 / 6.3 us with
 // 1 / 2 / 4, 32 x 2048 x 2048 6.0 / 6.7 / 8.5.
 int small_tiles(int64_t M, int64_t N) {
@@ -775,7 +777,7 @@ bool block_linear_small(int64_t M, int64_t N, int64_t K) { return choose(M, N, K
 hipError_t launch_block_linear_small(const BlockLinear& p, hipStream_t stream) {
     int nt = small_tiles(p.M, p.N);
     bool few = p.M <= FEW_ROWS, wide = small_wide(nt, p.K);
-    if (const char* forced = tuning_env("PHYAI_LAYER_SMALL")) {   // weight tiles of a workgroup; + 10: not the kernel of a few tokens; + 30: nor 8 wavefronts
+    if (const char* forced = tuning_env("PHYAI_LAYER_SMALL")) {   // weight tiles of a workgroup (of a few tokens: 1, else 4); + 10: not the kernel of a few tokens; + 30: nor 8 wavefronts
         nt = atoi(forced) % 10;
         few = p.M <= 8 && atoi(forced) < 10;
         wide = nt <= 2 && atoi(forced) >= 30;

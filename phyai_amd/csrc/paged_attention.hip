@@ -533,7 +533,7 @@ __device__ __forceinline__ Pool make_pool(const PagedAttention& p, const Tile& t
 // copies the next; the others' copies are under way meanwhile (twice as many wavefronts beat two stages for each).  Then the
 // workgroup's states meet in LDS; with more than one workgroup per tile they leave unnormalised sums for
 // attend_join_kernel.  Many sequences: bound by memory, 64 x 8192 keys of 8 heads of 128 in 254 us, 5.1 TB/s.  Few: by the chain of
-// sequence, page numbers, keys (64 bytes a cycle into a CU), products, sums: 50 tokens over 866 keys of 256 dims 15.4 us, 3 of them the join.
+// sequence, page numbers, keys (64 bytes a cycle into a CU), products, sums: 50 tokens over 866 keys of 256 dims 15.3 us, 3 to 4 of them the join.
 template <int DP>
 struct SplitShape {
     static constexpr int WAVES = DP == 256 ? 4 : 8;
@@ -721,7 +721,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const PagedAttention p
 // A step of 64 keys at a time, the next one on its way to LDS meanwhile; a wait for the wavefront's own copies and a barrier a
 // step.  Bound by the issue of instructions: two wavefronts a SIMD, of which each has 130 vector and 86 scalar ones beside 16
 // products for 32 keys when it takes those at a time (four such steps in LDS: 316 us for 2048 tokens of 32 heads of 128
-// dims over 8192 keys, 84 us for 16 x 816 of 8 heads of 256 over 816), and far fewer for 64 (270 and 77).
+// dims over 8192 keys, 84 us for 16 x 816 of 8 heads of 256 over 816), and far fewer for 64 (then 270 and 77, now 260 and 68).
 template <int DP>
 struct ManyShape {
     static constexpr int WAVES = 4, STEP = 64, MINE = STEP / WAVES, STAGE = 2 * STEP * Shape<DP>::ROW;
@@ -826,8 +826,8 @@ Plan make_plan(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int64_t m
     r.page = division((uint32_t)page_size);
     r.group = division((uint32_t)group);
     // Many rows a workgroup once there are workgroups for most of the chip and rows enough to fill them.  Measured, many
-    // against few: 128 workgroups of 256 dims 83 and 71 us, 816 of them 77 and 149; 128 of 128 dims 217 and 135, 256 of them
-    // 37 and 51; 512 of 64 dims (two to four fit a CU) 30.2 and 31.
+    // against few: 104 workgroups of 256 dims 40 and 36 us, 208 of them 44 and 61 (156: 43 and 49); 136 of 128 dims 112 and 73, 264
+    // of them 111 and 126; 288 of 64 dims (two to four fit a CU) 28 and 25, 576 of them 37 and 42.
     const int DP = padded_dim(D), waves = DP == 256 ? 4 : 8;
     const int64_t many = tiles_bound(T, B, group, 128) * KV;
     const char* forced = tuning_env("PHYAI_LAYER_ATTEND");   // 0: many rows; n: few rows, n splits
