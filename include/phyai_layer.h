@@ -16,7 +16,7 @@
 extern "C" {
 #endif
 
-#define PHYAI_LAYER_ABI_VERSION 1
+#define PHYAI_LAYER_ABI_VERSION 2
 
 int phyai_layer_abi_version(void);
 const char *phyai_layer_last_error(void);
@@ -96,6 +96,71 @@ int phyai_layer_paged_attention(const void *q, int64_t q_token_stride, int64_t q
                                 int64_t table_stride, int64_t table_width, const int32_t *q_offsets, const int32_t *kv_lens, void *out,
                                 int64_t T, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, float scale, int causal,
                                 int64_t window, int type, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Since version 2: the same half of a layer over a cache in 8 bits, and batches that share a prefix.
+ *
+ * A cache in 8 bits holds e4m3fn codes (strides multiples of 16 bytes) and, for each token and head, a byte b in a tensor of
+ * its own (any strides): a code stands for code * 2^(b - 127), exactly, in bfloat16; in half precision as far as that
+ * reaches.  255: all of the head's elements are NaNs.  head_dim is a multiple of 16.
+ */
+
+/*
+ * phyai_layer_head_rope into such a cache.  b is the smallest with which the head's largest magnitude, in fp32 after norm and
+ * rotation, stays within 448 (1 at least), so no code is ever beyond the type; codes are rounded to nearest even from fp32.
+ * Finite values end at 1.875 times the type's largest power of two (half precision: 61440).  A head with an infinity or a NaN is written as NaNs.
+ */
+int phyai_layer_head_rope_fp8(const void *qkv, int64_t ld, const void *q_weight, const void *k_weight, const float *cos_sin,
+                              int64_t table_rows, const int64_t *positions, void *q_out, void *k_pages, void *v_pages,
+                              const int64_t *k_strides, const int64_t *v_strides, uint8_t *k_scales, uint8_t *v_scales,
+                              const int64_t *k_scale_strides, const int64_t *v_scale_strides, const int64_t *slots, int64_t n_pages,
+                              int64_t page_size, int64_t T, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t rot, float eps,
+                              int gemma, int interleaved, int type, void *stream);
+
+/* Keys and values of the tokens in slots[0 .. T) as they stand there: [T, kv_heads, head_dim] each; a slot outside the cache
+ * reads as zeros.  Outputs must not overlap the cache. */
+int phyai_layer_cache_read(const void *k_pages, const void *v_pages, const int64_t *k_strides, const int64_t *v_strides,
+                           const uint8_t *k_scales, const uint8_t *v_scales, const int64_t *k_scale_strides,
+                           const int64_t *v_scale_strides, const int64_t *slots, int64_t n_pages, int64_t page_size, void *k_out,
+                           void *v_out, int64_t T, int64_t kv_heads, int64_t head_dim, int type, void *stream);
+
+/*
+ * total = bf16(x + residual), and the RMS norm of the total quantized:
+ *     n = total * rsqrt(mean(total^2) + eps) * w  (w + 1 with gemma != 0), fp32,
+ *     scale = max(amax |n|, 1e-12) / 448 over 128 elements of a row, or (xs_block = 0) over the row,   codes = e4m3fn(n / scale).
+ * x, residual, total: [M, D] bf16, row strides multiples of 8, 16-byte aligned; total may be x or residual and overlaps neither
+ * otherwise.  xq: [M, D] dense; scales as in phyai_layer_block_quant.  D % 8 == 0.
+ */
+int phyai_layer_add_rmsnorm_quant(const void *x, int64_t ldx, const void *residual, int64_t ldr, const void *weight, int gemma,
+                                  float eps, int64_t M, int64_t D, void *total, int64_t ldt, void *xq, float *x_scale, int64_t xs_row,
+                                  int64_t xs_block, void *stream);
+
+/*
+ * phyai_layer_paged_attention with more: each field may be left at zero.
+ *   k_scales, v_scales (and scale_strides: page, token, head): the pages are a cache in 8 bits; keys and values are taken as q's type.
+ *   softcap: a score s (scaled) becomes softcap * tanh(s / softcap), before the mask.
+ *   prefix_lens: [batch]; a causal row sees the first prefix_lens[b] keys too, wherever it stands (those that exist; a window
+ *     hides them as it does others).  Without causal it changes nothing.
+ *   shared_prefix: the first shared_prefix keys of all sequences lie in the same pages: every row of the page table has the same
+ *     first shared_prefix / page_size entries (which is not checked; those of the first row are used).  They may then be read
+ *     once for the whole batch.  The split of the work changes the order of sums and nothing else.
+ */
+typedef struct {
+    const uint8_t *k_scales, *v_scales;
+    int64_t scale_strides[3];
+    const int32_t *prefix_lens;
+    int64_t shared_prefix;
+    float softcap;
+} phyai_layer_attention_options;
+
+size_t phyai_layer_paged_attention_more_workspace_bytes(int64_t T, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                                        int64_t page_size, int64_t table_width, int64_t shared_prefix);
+int phyai_layer_paged_attention_more(const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *k_pages,
+                                     const void *v_pages, const int64_t *kv_strides, int64_t n_pages, int64_t page_size,
+                                     const int32_t *page_table, int64_t table_stride, int64_t table_width, const int32_t *q_offsets,
+                                     const int32_t *kv_lens, void *out, int64_t T, int64_t batch, int64_t heads, int64_t kv_heads,
+                                     int64_t head_dim, float scale, int causal, int64_t window, int type,
+                                     const phyai_layer_attention_options *options, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -57,7 +57,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
 }
 
 # the same library's second interface; mirrors include/phyai_layer.h one to one
-LAYER_ABI_VERSION = 1
+LAYER_ABI_VERSION = 2
 _f32 = ctypes.c_float
 LAYER_SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "phyai_layer_abi_version": (_int, []),
@@ -71,7 +71,21 @@ LAYER_SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "phyai_layer_paged_attention_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64]),
     "phyai_layer_paged_attention": (_int, [_vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
                                            _i64, _f32, _int, _i64, _int, _vp, _sz, _vp]),
+    "phyai_layer_head_rope_fp8": (_int, [_vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
+                                         _i64, _i64, _i64, _i64, _f32, _int, _int, _int, _vp]),
+    "phyai_layer_cache_read": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _int, _vp]),
+    "phyai_layer_add_rmsnorm_quant": (_int, [_vp, _i64, _vp, _i64, _vp, _int, _f32, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _vp]),
+    "phyai_layer_paged_attention_more_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "phyai_layer_paged_attention_more": (_int, [_vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64,
+                                                _i64, _i64, _f32, _int, _i64, _int, _vp, _vp, _sz, _vp]),
 }
+
+
+class AttentionOptions(ctypes.Structure):
+    """``phyai_layer_attention_options``."""
+
+    _fields_ = [("k_scales", _vp), ("v_scales", _vp), ("scale_strides", _i64 * 3), ("prefix_lens", _vp), ("shared_prefix", _i64),
+                ("softcap", _f32)]
 
 
 class Fp8LibraryError(RuntimeError):

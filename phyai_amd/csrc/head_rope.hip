@@ -13,6 +13,8 @@
 // 32.1 us, 4.6 TB/s, where a large copy runs at 5.2; one token 4.5 us, the launch.
 #include "fp8_device.h"
 #include "layer_kernels.h"
+#include "quant_device.h"
+#include "widen.h"
 
 namespace phyai {
 namespace {
@@ -54,8 +56,53 @@ __device__ __forceinline__ void store_run(uint16_t* p, const Run<V>& r) {
     else *reinterpret_cast<uint2*>(p) = make_uint2(r.w[0], r.w[1]);
 }
 
-// LP lanes a head (a power of two, at least D / (2 V)); `heads_per_group` heads of one token, neighbours, per group.
+// The power of two that the codes of a head have, as the byte b of 2^(b - 127): the smallest with which its largest magnitude
+// (bits of an fp32 value) stays within 448 = 1.75 * 2^8, so the exponent of the magnitude less 8, one more above 1.75.
+__device__ __forceinline__ uint32_t power_of(uint32_t amax) {
+    const int b = (int)((amax + 0x1FFFFFu) >> 23) - 8;
+    return b < 1 ? 1u : (uint32_t)b;
+}
+template <int V>
+__device__ __forceinline__ void store_codes(uint8_t* p, const float* x, float by, bool known) {
+    uint32_t w[V / 4];
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) {
+        const uint32_t c = encode4(x[4 * i] * by, x[4 * i + 1] * by, x[4 * i + 2] * by, x[4 * i + 3] * by);
+        w[i] = known ? c : kNanCodes;
+    }
+    if constexpr (V == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(p) = w[0];
+}
+// A head's lanes write its codes and its power: x and y are the lane's runs, zeros in lanes that have none.  Finite
+// values end at 1.875 times the type's largest power of two (half precision: 61440), the largest that it and e4m3 times a power have in
+// common: what lies above would be read as infinite.  A head with an infinity or a NaN is all NaN.
 template <int TYPE, int V>
+__device__ __forceinline__ void write_codes(uint8_t* o, uint8_t* scale, int a, int b, float* x, float* y, bool active, bool write, int lp_log) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const uint32_t u = __float_as_uint(x[i]) & 0x7FFFFFFFu, v = __float_as_uint(y[i]) & 0x7FFFFFFFu;
+        m = max(m, max(u, v));
+    }
+    for (int k = 1; k < (1 << lp_log); k <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, k));
+    const bool known = m < 0x7F800000u;
+    constexpr float most = TYPE == HEAD_BF16 ? 0x1.Ep127f : 61440.0f;
+    m = min(m, __float_as_uint(most));
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        x[i] = __builtin_amdgcn_fmed3f(x[i], -most, most);
+        y[i] = __builtin_amdgcn_fmed3f(y[i], -most, most);
+    }
+    if (!active || !write) return;
+    const uint32_t power = known ? power_of(m) : 127u;
+    const float by = __uint_as_float((254u - power) << 23);
+    store_codes<V>(o + a, x, by, known);
+    store_codes<V>(o + b, y, by, known);
+    if ((threadIdx.x & ((1 << lp_log) - 1)) == 0) *scale = (uint8_t)power;
+}
+
+// LP lanes a head (a power of two, at least D / (2 V)); `heads_per_group` heads of one token, neighbours, per group.
+template <int TYPE, int V, bool FP8>
 __global__ __launch_bounds__(256) void head_rope_kernel(const HeadRope p, int lp_log, int heads_per_group, int groups_per_token, int64_t groups) {
     const int64_t group = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> lp_log;
     const int c = threadIdx.x & ((1 << lp_log) - 1);
@@ -106,8 +153,18 @@ __global__ __launch_bounds__(256) void head_rope_kernel(const HeadRope p, int lp
             rb = load_run<V>(row + (int64_t)h * p.D + b);
         }
         if (h >= p.H + p.KV) {
-            if (active && write) {
-                uint16_t* o = p.v_pages + page * p.v_stride[0] + at * p.v_stride[1] + (h - p.H - p.KV) * p.v_stride[2];
+            if constexpr (FP8) {
+                float x[V], y[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    x[i] = head_to_f32<TYPE>((ra.w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu);
+                    y[i] = head_to_f32<TYPE>((rb.w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu);
+                }
+                const int j = h - p.H - p.KV;
+                write_codes<TYPE, V>(static_cast<uint8_t*>(p.v_pages) + page * p.v_stride[0] + at * p.v_stride[1] + j * p.v_stride[2],
+                                     p.v_scales + page * p.v_scale_stride[0] + at * p.v_scale_stride[1] + j * p.v_scale_stride[2], a, b, x, y, active, write, lp_log);
+            } else if (active && write) {
+                uint16_t* o = static_cast<uint16_t*>(p.v_pages) + page * p.v_stride[0] + at * p.v_stride[1] + (h - p.H - p.KV) * p.v_stride[2];
                 store_run<V>(o + a, ra);
                 store_run<V>(o + b, rb);
             }
@@ -157,11 +214,19 @@ __global__ __launch_bounds__(256) void head_rope_kernel(const HeadRope p, int lp
                 }
             }
         }
+        if constexpr (FP8) {
+            if (h >= p.H) {   // (uniform in a head's lanes)
+                const int j = h - p.H;
+                write_codes<TYPE, V>(static_cast<uint8_t*>(p.k_pages) + page * p.k_stride[0] + at * p.k_stride[1] + j * p.k_stride[2],
+                                     p.k_scales + page * p.k_scale_stride[0] + at * p.k_scale_stride[1] + j * p.k_scale_stride[2], a, b, x, y, active, write, lp_log);
+                continue;
+            }
+        }
         if (!active) continue;
         uint16_t* o;
         if (h < p.H) o = p.q_out + ((int64_t)t * p.H + h) * p.D;
         else if (p.k_out != nullptr) o = p.k_out + ((int64_t)t * p.KV + (h - p.H)) * p.D;
-        else if (write) o = p.k_pages + page * p.k_stride[0] + at * p.k_stride[1] + (h - p.H) * p.k_stride[2];
+        else if (write) o = static_cast<uint16_t*>(p.k_pages) + page * p.k_stride[0] + at * p.k_stride[1] + (h - p.H) * p.k_stride[2];
         else continue;
 #pragma unroll
         for (int i = 0; i < V; i += 2) {
@@ -173,7 +238,7 @@ __global__ __launch_bounds__(256) void head_rope_kernel(const HeadRope p, int lp
     }
 }
 
-template <int TYPE, int V>
+template <int TYPE, int V, bool FP8>
 hipError_t launch_v(const HeadRope& p, hipStream_t stream) {
     int lp_log = 0;
     while ((1 << lp_log) * 2 * V < p.D) ++lp_log;
@@ -185,7 +250,7 @@ hipError_t launch_v(const HeadRope& p, hipStream_t stream) {
     const int per_token = (heads + per_group - 1) / per_group;
     const int64_t groups = (int64_t)p.T * per_token;
     const int64_t threads = groups << lp_log;
-    return enqueue(head_rope_kernel<TYPE, V>, dim3((uint32_t)((threads + 255) / 256)), dim3(256), stream, p, lp_log, per_group, per_token, groups);
+    return enqueue(head_rope_kernel<TYPE, V, FP8>, dim3((uint32_t)((threads + 255) / 256)), dim3(256), stream, p, lp_log, per_group, per_token, groups);
 }
 
 }  // namespace
@@ -193,8 +258,12 @@ hipError_t launch_v(const HeadRope& p, hipStream_t stream) {
 hipError_t launch_head_rope(const HeadRope& p, hipStream_t stream) {
     // runs of eight elements where half the rotated part and what lies behind it are whole runs (pairs of them), else of four
     const bool wide = (p.interleaved ? p.rot % 16 == 0 : (p.rot / 2) % 8 == 0) && (p.D - p.rot) % 16 == 0;
-    if (p.type == HEAD_BF16) return wide ? launch_v<HEAD_BF16, 8>(p, stream) : launch_v<HEAD_BF16, 4>(p, stream);
-    return wide ? launch_v<HEAD_F16, 8>(p, stream) : launch_v<HEAD_F16, 4>(p, stream);
+    if (p.k_scales != nullptr) {
+        if (p.type == HEAD_BF16) return wide ? launch_v<HEAD_BF16, 8, true>(p, stream) : launch_v<HEAD_BF16, 4, true>(p, stream);
+        return wide ? launch_v<HEAD_F16, 8, true>(p, stream) : launch_v<HEAD_F16, 4, true>(p, stream);
+    }
+    if (p.type == HEAD_BF16) return wide ? launch_v<HEAD_BF16, 8, false>(p, stream) : launch_v<HEAD_BF16, 4, false>(p, stream);
+    return wide ? launch_v<HEAD_F16, 8, false>(p, stream) : launch_v<HEAD_F16, 4, false>(p, stream);
 }
 
 }  // namespace phyai

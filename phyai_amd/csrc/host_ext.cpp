@@ -54,6 +54,11 @@ struct Lib {
     decltype(&phyai_layer_head_rope) head_rope;
     decltype(&phyai_layer_paged_attention) attention;
     decltype(&phyai_layer_paged_attention_workspace_bytes) attention_ws;
+    decltype(&phyai_layer_head_rope_fp8) head_rope_fp8;
+    decltype(&phyai_layer_cache_read) cache_read;
+    decltype(&phyai_layer_add_rmsnorm_quant) add_rmsnorm;
+    decltype(&phyai_layer_paged_attention_more) attention_more;
+    decltype(&phyai_layer_paged_attention_more_workspace_bytes) attention_more_ws;
 } lib = {};
 
 struct Py {
@@ -816,9 +821,24 @@ bool pages_of(const at::Tensor* t, at::ScalarType dtype, int64_t D, const at::De
         return false;
     for (int i = 0; i < 3; ++i) {
         strides[i] = t->size(i) > 1 ? t->stride(i) : 0;
-        if (strides[i] < 0 || strides[i] % 8 != 0) return false;
+        if (strides[i] < 0 || strides[i] * t->element_size() % 16 != 0) return false;
     }
     return true;
+}
+// The scales beside pages in 8 bits, of the pages' shape without its last axis.
+bool scales_of(const at::Tensor* t, const at::Tensor& pages, const at::Device& dev, int64_t* strides) {
+    if (!on(t, dev) || t->dim() != 3 || (t->scalar_type() != at::kFloat8_e8m0fnu && t->scalar_type() != at::kByte)) return false;
+    for (int i = 0; i < 3; ++i) {
+        if (t->size(i) != pages.size(i)) return false;
+        strides[i] = t->size(i) > 1 ? t->stride(i) : 0;
+    }
+    return true;
+}
+const uint8_t* bytes(const at::Tensor* t) { return static_cast<const uint8_t*>(t->const_data_ptr()); }
+bool expanded(const at::Tensor& t) {
+    for (int i = 0; i < 3; ++i)
+        if (t.size(i) > 1 && t.stride(i) == 0) return true;
+    return false;
 }
 bool integer(PyObject* o, int64_t* v) {
     if (!PyLong_CheckExact(o)) return false;
@@ -858,10 +878,10 @@ PyObject* py_block_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // qk_norm_rope(qkv, cos_sin, positions, heads, kv_heads, head_dim, q_weight, k_weight, eps, gemma, interleaved, k_pages, v_pages,
-// slots, out) -> (q, k or None)
+// slots, out, k_scales, v_scales) -> (q, k or None)
 PyObject* py_qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    const at::Tensor *x = n == 15 ? tensor(a[0]) : nullptr, *cs = n == 15 ? tensor(a[1]) : nullptr;
+    const at::Tensor *x = n == 17 ? tensor(a[0]) : nullptr, *cs = n == 17 ? tensor(a[1]) : nullptr;
     Where at_;
     int64_t H, KV, D;
     if (!x || !cs || x->dim() != 2 || x->numel() == 0 || !where(*x, &at_) || head_type(*x) < 0 || !integer(a[3], &H) || !integer(a[4], &KV) ||
@@ -884,16 +904,14 @@ PyObject* py_qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int gemma = PyObject_IsTrue(a[9]), inter = PyObject_IsTrue(a[10]);
     if (gemma < 0 || inter < 0) return declined();
     const at::Tensor *kp = tensor(a[11]), *vp = tensor(a[12]), *slots = tensor(a[13]);
-    const bool paged = a[11] != Py_None || a[12] != Py_None || a[13] != Py_None;
-    int64_t ks[3], vs[3];
-    auto expanded = [](const at::Tensor& t) {
-        for (int i = 0; i < 3; ++i)
-            if (t.size(i) > 1 && t.stride(i) == 0) return true;
-        return false;
-    };
-    if (paged && (!pages_of(kp, dtype, D, at_.dev, ks) || !pages_of(vp, dtype, D, at_.dev, vs) || expanded(*kp) || expanded(*vp) ||
+    const at::Tensor *ksc = tensor(a[15]), *vsc = tensor(a[16]);
+    const bool fp8 = a[15] != Py_None || a[16] != Py_None, paged = fp8 || a[11] != Py_None || a[12] != Py_None || a[13] != Py_None;
+    int64_t ks[3], vs[3], kss[3], vss[3];
+    const auto kept = fp8 ? at::kFloat8_e4m3fn : dtype;
+    if (paged && (!pages_of(kp, kept, D, at_.dev, ks) || !pages_of(vp, kept, D, at_.dev, vs) || expanded(*kp) || expanded(*vp) ||
                   kp->sizes() != vp->sizes() || kp->size(2) != KV || !vector_on(slots, at::kLong, T, at_.dev)))
         return declined();
+    if (fp8 && (D % 16 != 0 || !scales_of(ksc, *kp, at_.dev, kss) || !scales_of(vsc, *kp, at_.dev, vss) || expanded(*ksc) || expanded(*vsc))) return declined();
     at::Tensor q, k;
     if (a[14] != Py_None) {
         const at::Tensor* o = tensor(a[14]);
@@ -903,6 +921,15 @@ PyObject* py_qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
         q = *o;
     } else q = fresh3(T, H, D, dtype, at_.dev);
     if (!paged) k = fresh3(T, KV, D, dtype, at_.dev);
+    if (fp8) {
+        if (lib.head_rope_fp8(x->const_data_ptr(), ld, qw ? qw->const_data_ptr() : nullptr, kw ? kw->const_data_ptr() : nullptr, cs->const_data_ptr<float>(),
+                              cs->size(0), tensor(a[2])->const_data_ptr<int64_t>(), q.mutable_data_ptr(), kp->mutable_data_ptr(), vp->mutable_data_ptr(), ks, vs,
+                              static_cast<uint8_t*>(ksc->mutable_data_ptr()), static_cast<uint8_t*>(vsc->mutable_data_ptr()), kss, vss,
+                              slots->const_data_ptr<int64_t>(), kp->size(0), kp->size(1), T, H, KV, D, cs->size(1), (float)eps, gemma, inter, head_type(*x),
+                              at_.stream) != 0)
+            return declined();
+        return Py_BuildValue("NN", THPVariable_Wrap(std::move(q)), wrap_or_none(k));
+    }
     if (lib.head_rope(x->const_data_ptr(), ld, qw ? qw->const_data_ptr() : nullptr, kw ? kw->const_data_ptr() : nullptr, cs->const_data_ptr<float>(), cs->size(0),
                       tensor(a[2])->const_data_ptr<int64_t>(), q.mutable_data_ptr(), paged ? nullptr : k.mutable_data_ptr(),
                       paged ? kp->mutable_data_ptr() : nullptr, paged ? vp->mutable_data_ptr() : nullptr, ks, vs,
@@ -913,24 +940,46 @@ PyObject* py_qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// paged_attention(q, k_pages, v_pages, page_table, q_offsets, kv_lens, scale, causal, window, out)
+// paged_attention(q, k_pages, v_pages, page_table, q_offsets, kv_lens, scale, causal, window, out, k_scales, v_scales, softcap, prefix_lens,
+// shared_prefix)
 PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    const at::Tensor *q = n == 10 ? tensor(a[0]) : nullptr, *kp = n == 10 ? tensor(a[1]) : nullptr, *vp = n == 10 ? tensor(a[2]) : nullptr,
-                     *table = n == 10 ? tensor(a[3]) : nullptr;
+    const at::Tensor *q = n == 15 ? tensor(a[0]) : nullptr, *kp = n == 15 ? tensor(a[1]) : nullptr, *vp = n == 15 ? tensor(a[2]) : nullptr,
+                     *table = n == 15 ? tensor(a[3]) : nullptr;
     Where at_;
     if (!q || !kp || !vp || !table || q->dim() != 3 || q->numel() == 0 || !where(*q, &at_) || head_type(*q) < 0) return declined();
     const int64_t T = q->size(0), H = q->size(1), D = q->size(2);
     if (D % 8 != 0 || D > 256 || q->stride(2) != 1 || q->stride(0) % 8 != 0 || q->stride(1) % 8 != 0 || !aligned16(q->const_data_ptr())) return declined();
     const auto dtype = q->scalar_type();
     int64_t ks[3], vs[3];
-    if (!pages_of(kp, dtype, D, at_.dev, ks) || !pages_of(vp, dtype, D, at_.dev, vs) || kp->sizes() != vp->sizes() || ks[0] != vs[0] || ks[1] != vs[1] ||
+    const at::Tensor *ksc = tensor(a[10]), *vsc = tensor(a[11]), *prompts = tensor(a[13]);
+    const bool fp8 = a[10] != Py_None || a[11] != Py_None;
+    const auto kept = fp8 ? at::kFloat8_e4m3fn : dtype;
+    phyai_layer_attention_options more = {};
+    if (!integer(a[14], &more.shared_prefix) || more.shared_prefix < 0) return declined();
+    if (!pages_of(kp, kept, D, at_.dev, ks) || !pages_of(vp, kept, D, at_.dev, vs) || kp->sizes() != vp->sizes() || ks[0] != vs[0] || ks[1] != vs[1] ||
         ks[2] != vs[2] || H % kp->size(2) != 0)
         return declined();
     if (!on(table, at_.dev) || table->dim() != 2 || table->scalar_type() != at::kInt || table->numel() == 0 || table->stride(1) != 1) return declined();
     const int64_t B = table->size(0), W = table->size(1);
     const at::Tensor *offsets = tensor(a[4]), *lens = tensor(a[5]);
     if (!vector_on(offsets, at::kInt, B + 1, at_.dev) || !vector_on(lens, at::kInt, B, at_.dev)) return declined();
+    if (fp8) {
+        int64_t other[3];
+        if (D % 16 != 0 || !scales_of(ksc, *kp, at_.dev, more.scale_strides) || !scales_of(vsc, *kp, at_.dev, other)) return declined();
+        for (int i = 0; i < 3; ++i)
+            if (other[i] != more.scale_strides[i]) return declined();
+        more.k_scales = bytes(ksc);
+        more.v_scales = bytes(vsc);
+    }
+    if (a[12] != Py_None) {
+        more.softcap = (float)PyFloat_AsDouble(a[12]);
+        if (PyErr_Occurred() || !(more.softcap > 0.f)) return declined();
+    }
+    if (a[13] != Py_None) {
+        if (!vector_on(prompts, at::kInt, B, at_.dev)) return declined();
+        more.prefix_lens = prompts->const_data_ptr<int32_t>();
+    }
     const double scale = a[6] == Py_None ? 1.0 / std::sqrt((double)D) : PyFloat_AsDouble(a[6]);
     if (scale == -1.0 && PyErr_Occurred()) return declined();
     const int causal = PyObject_IsTrue(a[7]);
@@ -943,6 +992,15 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         o = *t;
     } else o = fresh3(T, H, D, dtype, at_.dev);
     Scratch ws = {nullptr, 0};
+    if (fp8 || more.softcap > 0.f || more.prefix_lens || more.shared_prefix > 0) {
+        const size_t need = lib.attention_more_ws(T, B, H, kp->size(2), D, kp->size(1), W, more.shared_prefix);
+        if (need > 0 && !workspace(need, at_, &ws)) return declined();
+        if (lib.attention_more(q->const_data_ptr(), q->stride(0), q->stride(1), kp->const_data_ptr(), vp->const_data_ptr(), ks, kp->size(0), kp->size(1),
+                               table->const_data_ptr<int32_t>(), table->stride(0), W, offsets->const_data_ptr<int32_t>(), lens->const_data_ptr<int32_t>(),
+                               o.mutable_data_ptr(), T, B, H, kp->size(2), D, (float)scale, causal, window, head_type(*q), &more, ws.p, ws.n, at_.stream) != 0)
+            return declined();
+        return THPVariable_Wrap(std::move(o));
+    }
     const size_t need = lib.attention_ws(T, B, H, kp->size(2), D, W * kp->size(1));
     if (need > 0 && !workspace(need, at_, &ws)) return declined();
     if (lib.attention(q->const_data_ptr(), q->stride(0), q->stride(1), kp->const_data_ptr(), vp->const_data_ptr(), ks, kp->size(0), kp->size(1),
@@ -950,6 +1008,55 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
                       o.mutable_data_ptr(), T, B, H, kp->size(2), D, (float)scale, causal, window, head_type(*q), ws.p, ws.n, at_.stream) != 0)
         return declined();
     return THPVariable_Wrap(std::move(o));
+    END_HANDLE_TH_ERRORS
+}
+
+// read_fp8_cache(k_pages, v_pages, k_scales, v_scales, slots, dtype) -> (k, v)
+PyObject* py_read_fp8_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const at::Tensor *kp = n == 6 ? tensor(a[0]) : nullptr, *vp = n == 6 ? tensor(a[1]) : nullptr, *slots = n == 6 ? tensor(a[4]) : nullptr;
+    Where at_;
+    if (!kp || !vp || !slots || kp->dim() != 4 || kp->numel() == 0 || !where(*kp, &at_) || slots->numel() == 0 || !THPDtype_Check(a[5])) return declined();
+    const auto dtype = reinterpret_cast<THPDtype*>(a[5])->scalar_type;
+    const int64_t T = slots->numel(), KV = kp->size(2), D = kp->size(3);
+    int64_t ks[3], vs[3], kss[3], vss[3];
+    if ((dtype != at::kBFloat16 && dtype != at::kHalf) || D % 16 != 0 || D > 512 || !pages_of(kp, at::kFloat8_e4m3fn, D, at_.dev, ks) ||
+        !pages_of(vp, at::kFloat8_e4m3fn, D, at_.dev, vs) || kp->sizes() != vp->sizes() || !scales_of(tensor(a[2]), *kp, at_.dev, kss) ||
+        !scales_of(tensor(a[3]), *kp, at_.dev, vss) || !vector_on(slots, at::kLong, T, at_.dev))
+        return declined();
+    at::Tensor k = fresh3(T, KV, D, dtype, at_.dev), v = fresh3(T, KV, D, dtype, at_.dev);
+    if (lib.cache_read(kp->const_data_ptr(), vp->const_data_ptr(), ks, vs, bytes(tensor(a[2])), bytes(tensor(a[3])), kss, vss, slots->const_data_ptr<int64_t>(),
+                       kp->size(0), kp->size(1), k.mutable_data_ptr(), v.mutable_data_ptr(), T, KV, D, head_type(k), at_.stream) != 0)
+        return declined();
+    return Py_BuildValue("NN", THPVariable_Wrap(std::move(k)), THPVariable_Wrap(std::move(v)));
+    END_HANDLE_TH_ERRORS
+}
+
+// add_rmsnorm_fp8(x, residual, weight, eps, gemma, per_block, out) -> (codes, scale, total)
+PyObject* py_add_rmsnorm_fp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const at::Tensor *x = n == 7 ? tensor(a[0]) : nullptr, *res = n == 7 ? tensor(a[1]) : nullptr, *w = n == 7 ? tensor(a[2]) : nullptr;
+    Rows r, q;
+    Where at_;
+    if (!x || !res || !w || !rows_of(*x, at::kBFloat16, &r) || !rows_of(*res, at::kBFloat16, &q) || x->sizes() != res->sizes() || !where(*x, &at_) ||
+        !on(res, at_.dev) || !vector_on(w, at::kBFloat16, r.K, at_.dev) || !aligned16(w->const_data_ptr()) || r.K % 8 != 0)
+        return declined();
+    const double eps = PyFloat_AsDouble(a[3]);
+    if (eps == -1.0 && PyErr_Occurred()) return declined();
+    const int gemma = PyObject_IsTrue(a[4]), per_block = PyObject_IsTrue(a[5]);
+    if (gemma < 0 || per_block < 0) return declined();
+    at::Tensor total;
+    if (a[6] != Py_None) {
+        const at::Tensor* o = tensor(a[6]);
+        if (!shaped(o, *x, r.K, at::kBFloat16) || !on(o, at_.dev) || !aligned16(o->const_data_ptr())) return declined();
+        total = *o;
+    } else total = fresh(*x, r.K, at::kBFloat16, at_.dev);
+    const int64_t groups = per_block ? (r.K + 127) / 128 : 1;
+    at::Tensor codes = fresh(*x, r.K, at::kFloat8_e4m3fn, at_.dev), scale = fresh(*x, groups, at::kFloat, at_.dev);
+    if (lib.add_rmsnorm(r.p, r.ld, q.p, q.ld, w->const_data_ptr(), gemma, (float)eps, r.M, r.K, total.mutable_data_ptr(), r.K, codes.mutable_data_ptr(),
+                        scale.mutable_data_ptr<float>(), groups, per_block ? 1 : 0, at_.stream) != 0)
+        return declined();
+    return Py_BuildValue("NNN", THPVariable_Wrap(std::move(codes)), THPVariable_Wrap(std::move(scale)), THPVariable_Wrap(std::move(total)));
     END_HANDLE_TH_ERRORS
 }
 
@@ -991,6 +1098,11 @@ PyObject* py_bind(PyObject*, PyObject* args) {
     get(l.head_rope, "phyai_layer_head_rope");
     get(l.attention, "phyai_layer_paged_attention");
     get(l.attention_ws, "phyai_layer_paged_attention_workspace_bytes");
+    get(l.head_rope_fp8, "phyai_layer_head_rope_fp8");
+    get(l.cache_read, "phyai_layer_cache_read");
+    get(l.add_rmsnorm, "phyai_layer_add_rmsnorm_quant");
+    get(l.attention_more, "phyai_layer_paged_attention_more");
+    get(l.attention_more_ws, "phyai_layer_paged_attention_more_workspace_bytes");
     if (!ok) return PyErr_Format(PyExc_RuntimeError, "%s lacks an entry point this extension binds", path);
     for (PyObject* o : {p.workspaces, p.owner, p.reserve, p.epilogues, p.layouts, p.view_type, p.per_channel, p.per_tensor}) Py_INCREF(o);
     lib = l;
@@ -1058,6 +1170,8 @@ PyMethodDef methods[] = {
     PHYAI_FAST("block_linear", py_block_linear),
     PHYAI_FAST("qk_norm_rope", py_qk_norm_rope),
     PHYAI_FAST("paged_attention", py_paged_attention),
+    PHYAI_FAST("add_rmsnorm_fp8", py_add_rmsnorm_fp8),
+    PHYAI_FAST("read_fp8_cache", py_read_fp8_cache),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_phyai_host", "Eager call path of phyai_amd.ops and of the fp8 layers.", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

@@ -6,6 +6,15 @@
 
 namespace phyai {
 
+// Four values within the type's range as four codes.  A conversion into the upper half of a register needs two wait states before
+// a vector instruction reads it, which are put here.
+__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+    asm volatile("s_nop 1" : "+v"(w));
+    return (uint32_t)w;
+}
+
 enum QuantMode : int {
     QUANT_ACT_DYNAMIC = 0,  // bf16 amax floored at bf16(1e-12); scale = fp32(bf16(amax/448)); no clamp
     QUANT_WEIGHT = 1,       // fp32 amax/448 floored at FLT_MIN; clamp to +-448

@@ -825,6 +825,48 @@ def rope_table(positions: int, rot: int, base: float = 10000.0, *, device=None) 
     return torch.cat([angle.cos(), angle.sin()], dim=1).float().to(device=device if device is not None else "cuda").contiguous()
 
 
+def add_rmsnorm_fp8(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *, gemma: bool = False,
+                    per_block: bool = True, out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The residual's addition, the RMSNorm of the sum and its quantization in one pass: ``total = (x + residual)`` in bf16, ``n =
+    total * rsqrt(mean(total^2) + eps) * weight`` (``1 + weight`` with ``gemma``) in fp32, ``scale = max(amax |n|, 1e-12) / 448`` and
+    ``codes = e4m3fn(n / scale)``.
+
+    Returns ``(codes [..., D] float8_e4m3fn, scale, total)``: what :func:`fp8_block_gemm` takes, with a scale per 128 elements
+    (``[..., ceil(D / 128)]``, the last block may be shorter) or, without ``per_block``, one per row (``[..., 1]``, which
+    :func:`fp8_gemm` takes as well), and the sum that the residual stream goes on with.  Nothing is rounded between norm and codes,
+    where :func:`rmsnorm_fp8` rounds to bf16.  ``out``: where the total goes; it may be ``x`` or ``residual`` itself and must
+    not overlap them otherwise."""
+    op = "add_rmsnorm_fp8"
+    got = _native().add_rmsnorm_fp8(x, residual, weight, eps, gemma, per_block, out)
+    if got is not None:
+        return got
+    x2 = _as_rows(op, x, "x", torch.bfloat16)
+    r2 = _as_rows(op, residual, "residual", torch.bfloat16)
+    if residual.shape != x.shape:
+        raise _err(op, f"residual must have x's shape {tuple(x.shape)}, got {tuple(residual.shape)}")
+    M, D = x2.shape
+    _same_device(op, x.device, residual=residual, weight=weight, out=out)
+    if weight is None or weight.dtype != torch.bfloat16 or weight.shape != (D,) or not weight.is_contiguous() or weight.data_ptr() % 16:
+        raise _err(op, f"weight must be a contiguous 16-byte aligned bfloat16 GPU tensor of shape ({D},)")
+    if D == 0 or D % 8 != 0:
+        raise _err(op, f"last dim {D} must be a positive multiple of 8")
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    elif out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous() or out.data_ptr() % 16:
+        raise _err(op, "`out` must be contiguous, 16-byte aligned and match input shape and dtype")
+    groups = -(-D // BLOCK) if per_block else 1
+    codes = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty((*x.shape[:-1], groups), dtype=torch.float32, device=x.device)
+    if M == 0:
+        return codes, scale, out
+    with _device_of(x.device):
+        rc = _lib.load().phyai_layer_add_rmsnorm_quant(
+            x2.data_ptr(), x2.stride(0) if M > 1 else D, r2.data_ptr(), r2.stride(0) if M > 1 else D, weight.data_ptr(), 1 if gemma else 0,
+            float(eps), M, D, out.data_ptr(), D, codes.data_ptr(), scale.data_ptr(), groups, 1 if per_block else 0, _stream_ptr())
+    _lib.check_layer(rc, op)
+    return codes, scale, out
+
+
 def _page_strides(t: torch.Tensor) -> tuple[int, ...]:
     """Elements between pages, tokens and heads (0 where there is only one: what torch says there means nothing)."""
     return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3]))
@@ -832,15 +874,46 @@ def _page_strides(t: torch.Tensor) -> tuple[int, ...]:
 
 def _check_pages(op: str, k_pages, v_pages, dtype, head_dim: int, device) -> None:
     _same_device(op, device, k_pages=k_pages, v_pages=v_pages)
+    step = 16 // dtype.itemsize
     for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
         if t is None or t.dim() != 4 or t.dtype != dtype or t.shape[3] != head_dim:
             raise _err(op, f"{name} must be a {dtype} GPU tensor of shape (pages, page_size, kv_heads, {head_dim})")
-        if t.numel() and (t.stride(3) != 1 or any(s % 8 for s in _page_strides(t)) or t.data_ptr() % 16):
-            raise _err(op, f"{name} needs head_dim innermost, other strides that are multiples of 8 and a 16-byte aligned base")
+        if t.numel() and (t.stride(3) != 1 or any(s % step for s in _page_strides(t)) or t.data_ptr() % 16):
+            raise _err(op, f"{name} needs head_dim innermost, other strides that are multiples of {step} and a 16-byte aligned base")
     if k_pages.shape != v_pages.shape:
         raise _err(op, f"k_pages and v_pages must have one shape, got {tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
     if k_pages.shape[1] == 0 or k_pages.shape[2] == 0:
         raise _err(op, "a page must hold at least one token and one head")
+
+
+FP8_CACHE_DTYPE = torch.float8_e4m3fn
+FP8_CACHE_SCALE_DTYPE = torch.float8_e8m0fnu
+
+
+def fp8_cache(pages: int, page_size: int, num_kv_heads: int, head_dim: int, *, device=None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(k_pages, v_pages, k_scales, v_scales)`` of a paged cache in 8 bits, zeroed: codes ``[pages, page_size, num_kv_heads, head_dim]``
+    e4m3fn, and scales ``[pages, page_size, num_kv_heads]`` float8_e8m0fnu (a power of two for each token and head) that lie head by head in a page, as
+    attention reads them."""
+    dev = device if device is not None else "cuda"
+    codes = [torch.zeros(pages, page_size, num_kv_heads, head_dim, dtype=torch.uint8, device=dev).view(FP8_CACHE_DTYPE) for _ in range(2)]
+    scales = [torch.zeros(pages, num_kv_heads, page_size, dtype=torch.uint8, device=dev).transpose(1, 2).view(FP8_CACHE_SCALE_DTYPE) for _ in range(2)]
+    return (*codes, *scales)
+
+
+def _check_scales(op: str, k_scales, v_scales, pages: torch.Tensor, head_dim: int, device) -> None:
+    """The scales beside pages in 8 bits, whose codes have been looked at."""
+    if head_dim % 16 != 0:
+        raise _err(op, f"pages in 8 bits need head_dim to be a multiple of 16, got {head_dim}")
+    _same_device(op, device, k_scales=k_scales, v_scales=v_scales)
+    for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
+        if t is None or t.dtype not in (FP8_CACHE_SCALE_DTYPE, torch.uint8) or tuple(t.shape) != tuple(pages.shape[:3]):
+            raise _err(op, f"{name} must be a float8_e8m0fnu (or uint8) GPU tensor of shape {tuple(pages.shape[:3])} beside pages of float8_e4m3fn")
+
+
+def _strides3(t: torch.Tensor):
+    import ctypes
+
+    return (ctypes.c_int64 * 3)(*_page_strides(t))
 
 
 def _vector(op: str, name: str, t, dtype, n: int, device) -> int:
@@ -852,7 +925,8 @@ def _vector(op: str, name: str, t, dtype, n: int, device) -> int:
 def qk_norm_rope(qkv: torch.Tensor, cos_sin: torch.Tensor, positions: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int, *,
                  q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6, gemma: bool = False,
                  interleaved: bool = False, k_pages: torch.Tensor | None = None, v_pages: torch.Tensor | None = None,
-                 slots: torch.Tensor | None = None, out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
+                 slots: torch.Tensor | None = None, out: torch.Tensor | None = None, k_scales: torch.Tensor | None = None,
+                 v_scales: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
     """Norms of the query and key heads of a fused projection, the position rotation, and the write of keys and values
     into a paged cache, in one pass (bf16 or fp16, fp32 inside, one rounding).
 
@@ -865,10 +939,14 @@ def qk_norm_rope(qkv: torch.Tensor, cos_sin: torch.Tensor, positions: torch.Tens
     With ``k_pages`` / ``v_pages`` (``[pages, page_size, num_kv_heads, head_dim]``) and ``slots`` (``[T]`` int64, page *
     page_size + place) keys and values go into the cache and ``(q, None)`` is returned; a slot outside the cache (-1: padding)
     is not written, and slots must differ from each other.  Without pages the result is ``(q, k)``; values stay in ``qkv``.
-    ``out``: where q ``[T, num_heads, head_dim]`` goes."""
+    ``out``: where q ``[T, num_heads, head_dim]`` goes.
+
+    With ``k_scales`` / ``v_scales`` (``[pages, page_size, num_kv_heads]`` float8_e8m0fnu, :func:`fp8_cache`) the pages are e4m3fn:
+    every head of a token is divided by the smallest power of two that brings it within 448, rounded once, and the power written beside
+    it.  ``head_dim`` is a multiple of 16 then; finite values end at 1.875 times the type's largest power of two (fp16: 61440); a head with an infinity or a NaN becomes NaNs."""
     op = "qk_norm_rope"
     got = _native().qk_norm_rope(qkv, cos_sin, positions, num_heads, num_kv_heads, head_dim, q_weight, k_weight, eps, gemma, interleaved,
-                                 k_pages, v_pages, slots, out)
+                                 k_pages, v_pages, slots, out, k_scales, v_scales)
     if got is not None:
         return got
     if not (isinstance(qkv, torch.Tensor) and qkv.is_cuda and qkv.dim() == 2 and qkv.dtype in _HEAD_TYPES):
@@ -900,16 +978,19 @@ def qk_norm_rope(qkv: torch.Tensor, cos_sin: torch.Tensor, positions: torch.Tens
         out = torch.empty(T, H, D, dtype=dtype, device=dev)
     elif tuple(out.shape) != (T, H, D) or out.dtype != dtype or out.device != dev or not out.is_contiguous() or out.data_ptr() % 16:
         raise _err(op, f"out must be a contiguous {dtype} tensor of shape {(T, H, D)} on {dev}, 16-byte aligned")
-    paged = k_pages is not None or v_pages is not None or slots is not None
+    fp8 = k_scales is not None or v_scales is not None
+    paged = k_pages is not None or v_pages is not None or slots is not None or fp8
     k = ks = vs = slot_ptr = None
     n_pages = page_size = 0
     if paged:
         import ctypes
 
-        _check_pages(op, k_pages, v_pages, dtype, D, dev)
+        _check_pages(op, k_pages, v_pages, FP8_CACHE_DTYPE if fp8 else dtype, D, dev)
+        if fp8:
+            _check_scales(op, k_scales, v_scales, k_pages, D, dev)
         if k_pages.shape[2] != KV:
             raise _err(op, f"pages have {k_pages.shape[2]} heads, num_kv_heads is {KV}")
-        if any(s == 0 and n > 1 for t in (k_pages, v_pages) for s, n in zip(t.stride(), t.shape)):
+        if any(s == 0 and n > 1 for t in (k_pages, v_pages, *((k_scales, v_scales) if fp8 else ())) for s, n in zip(t.stride(), t.shape)):
             raise _err(op, "pages must not be expanded: several tokens or heads would be written to one place")
         slot_ptr = _vector(op, "slots", slots, torch.int64, T, dev)
         n_pages, page_size = k_pages.shape[:2]
@@ -918,6 +999,15 @@ def qk_norm_rope(qkv: torch.Tensor, cos_sin: torch.Tensor, positions: torch.Tens
         k = torch.empty(T, KV, D, dtype=dtype, device=dev)
     if T == 0:
         return out, k
+    if fp8:
+        with _device_of(dev):
+            rc = _lib.load().phyai_layer_head_rope_fp8(
+                qkv.data_ptr(), qkv.stride(0) if T > 1 else width, *weights, cos_sin.data_ptr(), cos_sin.shape[0], pos, out.data_ptr(),
+                k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, k_scales.data_ptr(), v_scales.data_ptr(), _strides3(k_scales), _strides3(v_scales),
+                slot_ptr, n_pages, page_size, T, H, KV, D, rot, float(eps), 1 if gemma else 0, 1 if interleaved else 0, _HEAD_TYPES[dtype],
+                _stream_ptr())
+        _lib.check_layer(rc, op)
+        return out, None
     with _device_of(dev):
         rc = _lib.load().phyai_layer_head_rope(
             qkv.data_ptr(), qkv.stride(0) if T > 1 else width, *weights, cos_sin.data_ptr(), cos_sin.shape[0], pos, out.data_ptr(),
@@ -928,9 +1018,45 @@ def qk_norm_rope(qkv: torch.Tensor, cos_sin: torch.Tensor, positions: torch.Tens
     return out, k
 
 
+def read_fp8_cache(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor, slots: torch.Tensor, *,
+                   dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values of single tokens of a cache in 8 bits (:func:`fp8_cache`, written by :func:`qk_norm_rope`), ``[T, kv_heads,
+    head_dim]`` each in ``dtype`` (bf16, which holds them exactly, or fp16): what :func:`paged_attention` sees of them.  ``slots``: ``[T]``
+    int64, page * page_size + place; one outside the cache reads as zeros."""
+    op = "read_fp8_cache"
+    got = _native().read_fp8_cache(k_pages, v_pages, k_scales, v_scales, slots, dtype)
+    if got is not None:
+        return got
+    if not (isinstance(k_pages, torch.Tensor) and k_pages.is_cuda and k_pages.dim() == 4):
+        raise _err(op, "k_pages must be a 4-D float8_e4m3fn GPU tensor (pages, page_size, kv_heads, head_dim)")
+    if dtype not in _HEAD_TYPES:
+        raise _err(op, f"dtype must be bfloat16 or float16, got {dtype}")
+    dev = k_pages.device
+    n_pages, page_size, KV, D = k_pages.shape
+    if D == 0 or D > 512:
+        raise _err(op, f"head_dim must be a multiple of 16 up to 512, got {D}")
+    _check_pages(op, k_pages, v_pages, FP8_CACHE_DTYPE, D, dev)
+    _check_scales(op, k_scales, v_scales, k_pages, D, dev)
+    if not isinstance(slots, torch.Tensor) or slots.dim() != 1:
+        raise _err(op, "slots must be a 1-D int64 tensor")
+    T = slots.shape[0]
+    slot_ptr = _vector(op, "slots", slots, torch.int64, T, dev)
+    k, v = (torch.empty(T, KV, D, dtype=dtype, device=dev) for _ in range(2))
+    if T == 0:
+        return k, v
+    with _device_of(dev):
+        rc = _lib.load().phyai_layer_cache_read(
+            k_pages.data_ptr(), v_pages.data_ptr(), _strides3(k_pages), _strides3(v_pages), k_scales.data_ptr(), v_scales.data_ptr(),
+            _strides3(k_scales), _strides3(v_scales), slot_ptr, n_pages, page_size, k.data_ptr(), v.data_ptr(), T, KV, D, _HEAD_TYPES[dtype],
+            _stream_ptr())
+    _lib.check_layer(rc, op)
+    return k, v
+
+
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, q_offsets: torch.Tensor,
                     kv_lens: torch.Tensor, *, scale: float | None = None, causal: bool = True, window: int | None = None,
-                    out: torch.Tensor | None = None) -> torch.Tensor:
+                    out: torch.Tensor | None = None, k_scales: torch.Tensor | None = None, v_scales: torch.Tensor | None = None,
+                    softcap: float | None = None, prefix_lens: torch.Tensor | None = None, shared_prefix: int = 0) -> torch.Tensor:
     """Attention of each sequence's new tokens - one, or a chunk - over its pages of a cache that holds their keys and
     values already.
 
@@ -942,6 +1068,14 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     table's width do not exist, which moves no token.  Query head h
     reads key head ``h // (heads // kv_heads)``.  ``scale`` defaults to ``head_dim ** -0.5``.
 
+    ``k_scales`` / ``v_scales``: the pages are a cache in 8 bits (:func:`fp8_cache`, written by :func:`qk_norm_rope`), whose keys and values
+    are taken as values of q's type.  ``softcap``: a scaled score s becomes ``softcap * tanh(s / softcap)``.  ``prefix_lens`` (``[B]`` int32):
+    a causal token sees the first ``prefix_lens[b]`` keys of its sequence as well, wherever it stands - a prompt whose tokens see each
+    other, with text behind it - and a window hides of them what it hides of others.  ``shared_prefix``: so many leading keys lie in the same pages for all sequences,
+    that is, the rows of ``page_table`` have their first ``shared_prefix // page_size`` entries in common (not checked: those of the
+    first row are taken); they are then read once for a batch of few tokens a sequence, not once for each, and nothing else changes
+    but the order of sums.
+
     Sums and maxima are fp32; probabilities are rounded to the element type for the second product and summed as rounded, which
     puts the result about half a step of the type further from exact (of the weighted values' magnitudes; relative 0.0022 against
     0.0017 over thousands of keys in bf16).
@@ -949,7 +1083,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     Returns ``[T, heads, head_dim]``; a row that sees nothing is zero, one whose scores are all -inf is NaN, rows outside every
     sequence are left as they were (of a fresh result: undefined), and rows that see keys of a page that does not exist are NaN."""
     op = "paged_attention"
-    got = _native().paged_attention(q, k_pages, v_pages, page_table, q_offsets, kv_lens, scale, causal, window, out)
+    got = _native().paged_attention(q, k_pages, v_pages, page_table, q_offsets, kv_lens, scale, causal, window, out, k_scales, v_scales, softcap,
+                                    prefix_lens, shared_prefix)
     if got is not None:
         return got
     if not (isinstance(q, torch.Tensor) and q.is_cuda and q.dim() == 3 and q.dtype in _HEAD_TYPES):
@@ -960,7 +1095,12 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         raise _err(op, f"needs at least one head and head_dim a multiple of 8 up to 256, got {H} heads of {D}")
     if q.numel() and (q.stride(2) != 1 or q.stride(0) % 8 != 0 or q.stride(1) % 8 != 0 or q.data_ptr() % 16 != 0):
         q = q.contiguous() if not q.is_contiguous() else q.clone()
-    _check_pages(op, k_pages, v_pages, dtype, D, dev)
+    fp8 = k_scales is not None or v_scales is not None
+    _check_pages(op, k_pages, v_pages, FP8_CACHE_DTYPE if fp8 else dtype, D, dev)
+    if fp8:
+        _check_scales(op, k_scales, v_scales, k_pages, D, dev)
+        if k_scales.numel() and _page_strides(k_scales) != _page_strides(v_scales):
+            raise _err(op, f"k_scales and v_scales must have the same strides, got {k_scales.stride()} and {v_scales.stride()}")
     if k_pages.numel() and _page_strides(k_pages) != _page_strides(v_pages):
         raise _err(op, f"k_pages and v_pages must have the same strides, got {k_pages.stride()} and {v_pages.stride()}")
     n_pages, page_size, KV, _ = k_pages.shape
@@ -976,6 +1116,11 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         raise _err(op, f"scale must be a positive number, got {scale}")
     if window is not None and window < 1:
         raise _err(op, f"window must be at least 1, got {window}")
+    if softcap is not None and not 0.0 < float(softcap) < float("inf"):
+        raise _err(op, f"softcap must be a positive number, got {softcap}")
+    if shared_prefix < 0:
+        raise _err(op, f"shared_prefix must not be negative, got {shared_prefix}")
+    prompts = _vector(op, "prefix_lens", prefix_lens, torch.int32, B, dev) if prefix_lens is not None else None
     if out is None:
         out = torch.empty(T, H, D, dtype=dtype, device=dev)
     elif tuple(out.shape) != (T, H, D) or out.dtype != dtype or out.device != dev or not out.is_contiguous() or out.data_ptr() % 16:
@@ -985,6 +1130,20 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     import ctypes
 
     lib = _lib.load()
+    if fp8 or softcap is not None or prompts is not None or shared_prefix:
+        options = _lib.AttentionOptions(prefix_lens=prompts, shared_prefix=int(shared_prefix), softcap=float(softcap or 0.0))
+        if fp8:
+            options.k_scales, options.v_scales, options.scale_strides = k_scales.data_ptr(), v_scales.data_ptr(), _strides3(k_scales)
+        with _device_of(dev):
+            need = lib.phyai_layer_paged_attention_more_workspace_bytes(T, B, H, KV, D, page_size, W, int(shared_prefix))
+            ws = reserve_workspace(need, dev) if need else None
+            rc = lib.phyai_layer_paged_attention_more(
+                q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), v_pages.data_ptr(), _strides3(k_pages), n_pages, page_size,
+                page_table.data_ptr(), page_table.stride(0), W, offsets, lens, out.data_ptr(), T, B, H, KV, D, scale, 1 if causal else 0,
+                min(int(window), (1 << 31) - 1) if window is not None else 0, _HEAD_TYPES[dtype], ctypes.byref(options),
+                ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, _stream_ptr())
+        _lib.check_layer(rc, op)
+        return out
     with _device_of(dev):
         need = lib.phyai_layer_paged_attention_workspace_bytes(T, B, H, KV, D, W * page_size)
         ws = reserve_workspace(need, dev) if need else None
