@@ -269,12 +269,21 @@ struct Widener {
     const Pool& s;
     const int begin, end, row;
     int page, lo, hi;                  // of the lane's key: its page in the turn to come; its offset
-    uint32_t k_power, v_power;
+    uint32_t k_power, v_power, powers; // its scales as they were asked for; both, of the turn being stored
     uint64_t odd;                      // lanes whose key's page does not exist
+    uint32_t at;                       // the lane's part of an address: its key of a load, its chunk
+    uint32_t k_to, v_to;               // where its first chunk of load 0 goes in a buffer
     v4i k[LOADS], v[LOADS];            // of the block to come
 
     __device__ __forceinline__ Widener(const Pool& pool, int first, int last, int first_row)
-        : s(pool), begin(first), end(last), row(first_row), page(0), lo(0), hi(0), k_power(0), v_power(0), odd(0) {}
+        : s(pool), begin(first), end(last), row(first_row), page(0), lo(0), hi(0), k_power(0), v_power(0), powers(0), odd(0) {
+        const uint32_t lane = threadIdx.x & 63, r = (uint32_t)row + lane / LANES, chunk = 2 * (lane % LANES) + turned();
+        at = lane / LANES * (uint32_t)s.token_bytes + lane % LANES * 16;
+        k_to = r * ROW + ((chunk ^ k_swizzle<DP>(r)) << 4);
+        v_to = r * ROW + ((chunk ^ v_swizzle<DP>(r)) << 4);
+    }
+    // Of eight lanes, which LDS takes at once, four write their first eight values first and four the others: all in different banks.
+    __device__ __forceinline__ static uint32_t turned() { return (threadIdx.x >> 2) & 1; }
     __device__ __forceinline__ int key(int turn) const {
         const int lane = threadIdx.x & 63, j = (begin + turn * BLOCKS + lane / N) * STEP + row + lane % N;
         return j < s.kv_len ? j : (s.kv_len - 1) & ~(RUN - 1);
@@ -296,15 +305,34 @@ struct Widener {
     }
     // Asks for block `blk` (below end; the blocks one after another, block `begin` after ask(0)).
     __device__ __forceinline__ void load(int blk) {
-        const int at = blk - begin;
-        if (at % BLOCKS == 0) {
-            look(at / BLOCKS);
-            if (blk + BLOCKS < end) ask(at / BLOCKS + 1);
+        const int nth = blk - begin, first = nth % BLOCKS * N;
+        if (nth % BLOCKS == 0) {
+            look(nth / BLOCKS);
+            if (blk + BLOCKS < end) ask(nth / BLOCKS + 1);
+        }
+        if (s.neat && ((odd >> first) & (N == 64 ? ~0ull : (1ull << (N & 63)) - 1)) == 0) {
+            // runs of eight keys share a base
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                const int from = first + i * PER / RUN * RUN, run = PER > RUN ? (int)((threadIdx.x & 63) / LANES) / RUN * RUN : 0;
+                if constexpr (PER > RUN) {   // (two runs a load: each lane its own)
+                    const int64_t off = (int64_t)(uint32_t)__shfl(lo, from + run) | (int64_t)__shfl(hi, from + run) << 32;
+                    const int64_t to = off + at - (int64_t)run * s.token_bytes;
+                    k[i] = *reinterpret_cast<const v4i*>(s.k + to);
+                    v[i] = *reinterpret_cast<const v4i*>(s.v + to);
+                } else {
+                    const int64_t off = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(lo, from) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, from) << 32) +
+                                        (int64_t)(i * PER % RUN) * s.token_bytes;
+                    k[i] = *reinterpret_cast<const v4i*>(s.k + off + at);
+                    v[i] = *reinterpret_cast<const v4i*>(s.v + off + at);
+                }
+            }
+            return;
         }
         const int lane = threadIdx.x & 63, chunk = lane % LANES;
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
-            const int from = at % BLOCKS * N + i * PER + lane / LANES;
+            const int from = first + i * PER + lane / LANES;
             const int64_t off = (int64_t)(uint32_t)__shfl(lo, from) | (int64_t)__shfl(hi, from) << 32;
             const int fill = chunk < s.d_chunks && ((odd >> from) & 1) ? (int)kNanCodes : 0;
             v4i a = {fill, fill, fill, fill}, b = a;
@@ -316,23 +344,24 @@ struct Widener {
             v[i] = b;
         }
     }
-    __device__ __forceinline__ static void put(uint8_t* to, uint32_t swizzle, uint32_t power, const v4i& codes) {
-        const uint32_t chunk = (threadIdx.x & 63) % LANES;
+    __device__ __forceinline__ static void put(uint8_t* lds, uint32_t to, uint32_t power, const v4i& codes) {
         v4i w[2];
-        widen16<TYPE>(codes, power, w);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) *reinterpret_cast<v4i*>(to + (((2 * chunk + x) ^ swizzle) << 4)) = w[x];
+        widen16<TYPE>(turned() ? v4i{codes[2], codes[3], codes[0], codes[1]} : codes, power, w);
+        *reinterpret_cast<v4i*>(lds + to) = w[0];
+        *reinterpret_cast<v4i*>(lds + (to ^ 16u)) = w[1];
     }
     // The block asked for last, which is `blk`, into the buffers.
     __device__ __forceinline__ void store(int blk, uint8_t* k_lds, uint8_t* v_lds) {
         const int lane = threadIdx.x & 63;
-        asm volatile("" ::: "memory");
+        if ((blk - begin) % BLOCKS == 0) powers = k_power | v_power << 8;
+        uint32_t kt = k_to, vt = v_to;
+        asm volatile("" : "+v"(kt), "+v"(vt) :: "memory");   // (worked out here, not kept for each load)
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
-            const uint32_t r = (uint32_t)(row + i * PER + lane / LANES);
-            const int from = (blk - begin) % BLOCKS * N + i * PER + lane / LANES;
-            put(k_lds + r * ROW, k_swizzle<DP>(r), (uint32_t)__shfl((int)k_power, from), k[i]);
-            put(v_lds + r * ROW, v_swizzle<DP>(r), (uint32_t)__shfl((int)v_power, from), v[i]);
+            const uint32_t both = (uint32_t)__shfl((int)powers, (blk - begin) % BLOCKS * N + i * PER + lane / LANES);
+            // (the swizzles of these keys are those of load 0's with the bits of i PER flipped)
+            put(k_lds, (kt ^ k_swizzle<DP>(i * PER) << 4) + i * PER * ROW, both & 255u, k[i]);
+            put(v_lds, (vt ^ v_swizzle<DP>(i * PER) << 4) + i * PER * ROW, both >> 8, v[i]);
         }
         asm volatile("" ::: "memory");
     }
@@ -481,17 +510,18 @@ __device__ __forceinline__ void raise_maximum(State<DP>& st, float mx) {
     }
     st.m = m;
 }
-// A score s to cap tanh(s / cap), in base 2: with e = 2^(s by), by = 2 log2(e) scale / cap, tanh = 1 - 2 / (e + 1), exact where the
-// power over- or underflows; cap: times log2(e).  Off by some 2^-22 of cap in all, which is what the score's own rounding is.
+// A score s to cap tanh(s / cap) in base 2: with e = 2^(s by), by = 2 log2(e) scale / cap, tanh = 1 - 2 / (e + 1), exact where the
+// power over- or underflows.  Kept is -1 / (e + 1), from which the score (less a maximum) is one multiply-add: times 2 cap log2(e), and cap log2(e)
+// left out, which all scores have in common.  Off by some 2^-22 of cap in all, which is what the score's own rounding is.
 struct Cap {
-    float by, cap;
+    float by;
 };
 template <int NB>
 __device__ __forceinline__ void cap_scores(v16f (&s)[NB], Cap c) {
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[n][i] = __builtin_fmaf(__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[n][i] * c.by) + 1.0f), -2.0f * c.cap, c.cap);
+        for (int i = 0; i < 16; ++i) s[n][i] = -__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[n][i] * c.by) + 1.0f);
 }
 // Scores to probabilities, as the second product's operand.  The sum is of the rounded ones, those that the product uses:
 // their common error cancels.
@@ -520,7 +550,7 @@ template <int DP, int TYPE, int NB, int MODE, typename Top>
 __device__ __forceinline__ void attend_steps(State<DP>& st, const v4i* qf, int step, int end, const Row& row, int whole_lo, int whole_hi, float c, Cap cap, Top top) {
     using S = Shape<DP>;
     // V is read while the scores are turned into probabilities; as much of it as there are registers for
-    constexpr int EARLY = DP == 64 ? 2 : NB == 1 || DP == 256 ? 4 : 2;
+    constexpr int EARLY = DP == 64 || (DP == 128 && (MODE & MODE_FP8) && (MODE & MODE_CAP)) ? 2 : NB == 1 || DP == 256 ? 4 : 2;
     while (step < end) {
         v16f s[NB];
         float mx = kNone;
@@ -666,26 +696,28 @@ __device__ __forceinline__ Pool make_pool(const PagedAttention& p, const Tile& t
 // workgroup's states meet in LDS; with more than one workgroup per tile they leave unnormalised sums for
 // attend_join_kernel.  Many sequences: bound by memory, 64 x 8192 keys of 8 heads of 128 in 254 us, 5.1 TB/s.  Few: by the chain of
 // sequence, page numbers, keys (64 bytes a cycle into a CU), products, sums: 50 tokens over 866 keys of 256 dims 15.3 us, 3 to 4 of them the join.
-template <int DP>
+template <int DP, int WAVES_OF>
 struct SplitShape {
-    static constexpr int WAVES = DP == 256 ? 4 : 8;
+    static constexpr int WAVES = WAVES_OF;
     static constexpr int STAGE = 2 * 32 * Shape<DP>::ROW;
     static constexpr int OLD = DP + 4;                            // floats of a row of O in LDS
     static constexpr int WAVE_BYTES = STAGE > 32 * OLD * 4 ? STAGE : 32 * OLD * 4;
 };
+template <int DP>
+constexpr int SPLIT_WAVES = DP == 256 ? 4 : 8;   // of a workgroup that has a CU to itself (64 dims: two fit)
 // What a row's O is divided by, inverted: a sum of zero is a row's that sees nothing, or only scores of -inf.
 __device__ __forceinline__ float one_over(float sum, bool sees) { return sum != 0.f ? 1.0f / sum : sees ? __builtin_nanf("") : 0.f; }
 // How much of a state with maximum m belongs into one with the larger maximum `all` (m = -inf: it has seen nothing, or NaN).
 __device__ __forceinline__ float share(float m, float l, float all) { return m == kNone ? (l != l ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(m - all); }
 
 // The rows of all sequences against the shared leading keys, which the first sequence's pages hold.
-__device__ __forceinline__ bool locate_shared(const PagedAttention& p, const Plan& g, int tile, Tile& o) {
+__device__ __forceinline__ bool locate_shared(const PagedAttention& p, const Plan& g, int rows_per_tile, int tile, Tile& o) {
     const int q0 = clamp_i(p.q_offsets[0], 0, p.T), q1 = clamp_i(p.q_offsets[p.B], q0, p.T);
     o.b = 0;
     o.q_begin = q0;
     o.q_len = q1 - q0;
     o.rows = o.q_len * g.group_size;
-    o.row0 = tile * ROWS;
+    o.row0 = tile * rows_per_tile;
     o.length = o.kv_len = g.shared;
     o.prompt = 0;
     return o.row0 < o.rows;
@@ -736,27 +768,27 @@ __device__ __forceinline__ Row row_of_shared(const PagedAttention& p, const Tile
     hi = __builtin_amdgcn_readfirstlane(hi);
     all_lo = __builtin_amdgcn_readfirstlane(all_lo);
     all_hi = __builtin_amdgcn_readfirstlane(all_hi);
-    if (lo >= hi) lo = hi = 0;
     return r;
 }
 
-template <int DP, int TYPE, int MODE>
-__global__ __launch_bounds__(SplitShape<DP>::WAVES * 64, 1) void attend_split_kernel(const PagedAttention p, const Plan g, float* __restrict__ part) {
+template <int DP, int TYPE, int MODE, int WAVES_OF>
+__global__ __launch_bounds__(WAVES_OF * 64, SPLIT_WAVES<DP> / WAVES_OF) void attend_split_kernel(const PagedAttention p, const Plan g, float* __restrict__ part) {
     using S = Shape<DP>;
-    using X = SplitShape<DP>;
+    using X = SplitShape<DP, WAVES_OF>;
     __shared__ __align__(16) uint8_t lds[X::WAVES * X::WAVE_BYTES];
     __shared__ uint32_t ids[X::WAVES][2][64];
     __shared__ float ml[X::WAVES][32][2], weight[X::WAVES][32];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int tile = blockIdx.x, kv_head = blockIdx.y, z = blockIdx.z;
+    const int tile = blockIdx.x, kv_head = blockIdx.y, z = blockIdx.z + (MODE & MODE_MORE ? g.z_first : 0);
     // (the shared keys' splits come first)
     const bool shared = (MODE & MODE_MORE) != 0 && z < g.shared_splits;
     Tile t;
     Row row;
     int lo, hi, all_lo, all_hi;
     if (shared) {   // (here and below: the same for the whole workgroup)
-        if (tile >= g.shared_tiles || !locate_shared(p, g, tile, t)) return;
+        if (tile >= g.shared_tiles || !locate_shared(p, g, ROWS, tile, t)) return;
         row = row_of_shared(p, t, g, kv_head, t.row0, lo, hi, all_lo, all_hi);
+        if (lo >= hi) lo = hi = 0;
     } else {
         if (!locate<MODE>(p, g.group_size, ROWS, tile, t)) return;
         row = row_of<MODE>(p, t, g, kv_head, t.row0 + (lane & 31));
@@ -766,11 +798,11 @@ __global__ __launch_bounds__(SplitShape<DP>::WAVES * 64, 1) void attend_split_ke
     // even shares, the first ones a block larger
     const int of = MODE & MODE_MORE ? (shared ? g.shared_splits : g.splits - g.shared_splits) : g.splits;
     const int me = (z - (shared || !(MODE & MODE_MORE) ? 0 : g.shared_splits)) * X::WAVES + wave;
-    const int each = divide(n, shared ? g.shared_workers : g.workers), rest = n - each * of * X::WAVES;
+    const int each = shared ? divide(n, g.shared_workers) : divide(n, g.workers), rest = n - each * of * X::WAVES;
     const int begin = b0 + me * each + (me < rest ? me : rest), end = begin + each + (me < rest ? 1 : 0);
     const Pool pool = make_pool<DP, TYPE, MODE>(p, t, kv_head, g);
-    const float c = MODE & MODE_CAP ? 1.0f : p.scale * 1.4426950408889634f;
-    const Cap cap = {p.cap_by, p.cap};
+    const float c = MODE & MODE_CAP ? 2.0f * p.cap : p.scale * 1.4426950408889634f;
+    const Cap cap = {p.cap_by};
 
     State<DP> st;
     st.m = kNone;
@@ -946,27 +978,71 @@ struct ManyShape {
     static constexpr int WAVES = 4, STEP = 64, MINE = STEP / WAVES, STAGE = 2 * STEP * Shape<DP>::ROW;
 };
 
+// Which tile and key head a workgroup has.  Key heads change fastest: workgroups go round the eight chiplets, so each of those has few heads'
+// keys in its cache.  Causal rows see the more keys the later they are: the last ones first, and where two workgroups share a CU and
+// all run at once, the second half the other way round, so that a long one has a short one beside it.
+template <int DP>
+__device__ __forceinline__ bool place(const PagedAttention& p, int tiles, int& tile, int& kv_head) {
+    int at = blockIdx.y * gridDim.x + blockIdx.x;
+    const int all = tiles * p.KV;
+    if (at >= all) return false;
+    if (p.causal && DP != 256 && all <= 512 && at >= 256) at = all - 1 - (at - 256);
+    tile = at / p.KV;
+    kv_head = at - tile * p.KV;
+    if (p.causal) tile = tiles - 1 - tile;
+    return true;
+}
+
 template <int DP, int TYPE, int MODE>
-__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(const PagedAttention p, const Plan g) {
+__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(const PagedAttention p, const Plan g, float* __restrict__ part) {
     using S = Shape<DP>;
     using X = ManyShape<DP>;
     __shared__ __align__(16) uint8_t lds[2 * X::STAGE];
     __shared__ uint32_t ids[X::WAVES][2][64];
-    __shared__ int specials[X::WAVES];
+    __shared__ int specials[X::WAVES], spans[X::WAVES][4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int kv_head = blockIdx.y;
+    const int z = MODE & MODE_MORE ? blockIdx.z + g.z_first : 0;
+    const bool shared = (MODE & MODE_MORE) != 0 && z < g.shared_splits;
+    int tile, kv_head;
     Tile t;
-    if (!locate<MODE>(p, g.group_size, ROWS * X::WAVES, blockIdx.x, t)) return;
+    if (!place<DP>(p, shared ? g.shared_tiles : g.tiles, tile, kv_head)) return;   // (here and below: the same for the whole workgroup)
+    if (shared ? !locate_shared(p, g, ROWS * X::WAVES, tile, t) : !locate<MODE>(p, g.group_size, ROWS * X::WAVES, tile, t)) return;
     const int row0 = t.row0 + wave * ROWS, row_last = t.rows - 1;
-    const Row row = row_of<MODE>(p, t, g, kv_head, row0 + (lane & 31));
-    int lo, hi, all_lo, all_hi;          // of the workgroup
-    span_of<MODE>(p, t, g, t.row0, t.row0 + ROWS * X::WAVES - 1 < row_last ? t.row0 + ROWS * X::WAVES - 1 : row_last, lo, hi, all_lo, all_hi);
+    Row row;
+    int lo, hi, all_lo, all_hi;                             // of the workgroup
     int my_lo = 0, my_hi = 0, whole_lo = 0, whole_hi = 0;   // of the wavefront
-    if (row0 <= row_last) span_of<MODE>(p, t, g, row0, row0 + ROWS - 1 < row_last ? row0 + ROWS - 1 : row_last, my_lo, my_hi, whole_lo, whole_hi);
-    const int begin = lo / X::STEP, end = (hi + X::STEP - 1) / X::STEP;
+    if (shared) {
+        row = row_of_shared(p, t, g, kv_head, row0, my_lo, my_hi, whole_lo, whole_hi);
+        if (lane == 0) {
+            spans[wave][0] = my_lo;
+            spans[wave][1] = my_hi;
+            spans[wave][2] = whole_lo;
+            spans[wave][3] = whole_hi;
+        }
+        __syncthreads();
+        lo = min(min(spans[0][0], spans[1][0]), min(spans[2][0], spans[3][0]));
+        hi = max(max(spans[0][1], spans[1][1]), max(spans[2][1], spans[3][1]));
+        all_lo = max(max(spans[0][2], spans[1][2]), max(spans[2][2], spans[3][2]));
+        all_hi = min(min(spans[0][3], spans[1][3]), min(spans[2][3], spans[3][3]));
+        lo = __builtin_amdgcn_readfirstlane(lo < hi ? lo : 0);
+        hi = __builtin_amdgcn_readfirstlane(lo < hi ? hi : 0);
+        all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+        all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+    } else {
+        row = row_of<MODE>(p, t, g, kv_head, row0 + (lane & 31));
+        span_of<MODE>(p, t, g, t.row0, t.row0 + ROWS * X::WAVES - 1 < row_last ? t.row0 + ROWS * X::WAVES - 1 : row_last, lo, hi, all_lo, all_hi);
+        if (row0 <= row_last) span_of<MODE>(p, t, g, row0, row0 + ROWS - 1 < row_last ? row0 + ROWS - 1 : row_last, my_lo, my_hi, whole_lo, whole_hi);
+    }
+    int begin = lo / X::STEP, end = (hi + X::STEP - 1) / X::STEP;
+    if constexpr (MODE & MODE_MORE) {   // the split's part of them, the first ones a step larger
+        const int of = shared ? g.shared_splits : g.splits - g.shared_splits, me = z - (shared ? 0 : g.shared_splits);
+        const int n = end - begin, each = shared ? divide(n, g.shared_workers) : divide(n, g.workers), rest = n - each * of;
+        begin += me * each + (me < rest ? me : rest);
+        end = begin + each + (me < rest ? 1 : 0);
+    }
     const Pool pool = make_pool<DP, TYPE, MODE>(p, t, kv_head, g);
-    const float c = MODE & MODE_CAP ? 1.0f : p.scale * 1.4426950408889634f;
-    const Cap cap = {p.cap_by, p.cap};
+    const float c = MODE & MODE_CAP ? 2.0f * p.cap : p.scale * 1.4426950408889634f;
+    const Cap cap = {p.cap_by};
     const uint32_t base = (uint32_t)(uintptr_t)lds;
     using Feed = Feeder<DP, X::STEP, X::MINE>;
     Feed feed(pool, begin, wave * X::MINE, ids[wave][0]);
@@ -1028,6 +1104,26 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
         }
     }
     const float l = other_half_sum(st.l);
+    if constexpr (MODE & MODE_MORE) {
+        if (g.splits > 1) {   // as attend_split_kernel leaves them
+            if (!row.valid) return;
+            const int64_t all = (int64_t)p.T * p.H, i = z * all + (int64_t)row.token * p.H + row.head;
+            const int from = row.lo > begin * X::STEP ? row.lo : begin * X::STEP, to = row.hi < end * X::STEP ? row.hi : end * X::STEP;
+            if (lane < 32)
+                *reinterpret_cast<float2*>(part + g.splits * all * DP + i * 2) = make_float2(st.m == kNone && l == 0.f && from < to ? kLowest : st.m, l);
+            float* o = part + i * DP + 4 * (lane >> 5);
+#pragma unroll
+            for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    v4f v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = st.o[b][4 * k + e];
+                    if (32 * b + 8 * k + 4 * (lane >> 5) < p.D) *reinterpret_cast<v4f*>(o + 32 * b + 8 * k) = v;
+                }
+            return;
+        }
+    }
     const float inv = one_over(l, row.lo < row.hi);
     if (!row.valid) return;
     uint16_t* out = p.out + ((int64_t)row.token * p.H + row.head) * p.D;
@@ -1045,10 +1141,27 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
 // ---- launches --------------------------------------------------------------------------------------------------------
 template <int DP, int TYPE, int MODE>
 hipError_t launch(const PagedAttention& p, const Plan& plan, hipStream_t stream) {
-    if (plan.many) return enqueue(attend_many_kernel<DP, TYPE, MODE>, dim3(plan.tiles, p.KV), dim3(256), stream, p, plan);
     float* part = static_cast<float*>(p.workspace);
-    const int tiles = plan.tiles > plan.shared_tiles ? plan.tiles : plan.shared_tiles;
-    const hipError_t e = enqueue(attend_split_kernel<DP, TYPE, MODE>, dim3(tiles, p.KV, plan.splits), dim3(SplitShape<DP>::WAVES * 64), stream, p, plan, part);
+    constexpr int WAVES = SPLIT_WAVES<DP>;
+    // splits first .. first + count - 1, with one kernel
+    auto run = [&](int many, int tiles, int first, int count) {
+        Plan g = plan;
+        g.z_first = first;
+        const dim3 grid(tiles, p.KV, count);
+        if (many) return enqueue(attend_many_kernel<DP, TYPE, MODE>, grid, dim3(256), stream, p, g, part);
+        if constexpr (MODE & MODE_MORE) {
+            if (plan.small) return enqueue(attend_split_kernel<DP, TYPE, MODE, WAVES / 2>, grid, dim3(WAVES * 32), stream, p, g, part);
+        }
+        return enqueue(attend_split_kernel<DP, TYPE, MODE, WAVES>, grid, dim3(WAVES * 64), stream, p, g, part);
+    };
+    const int own = plan.splits - plan.shared_splits;
+    hipError_t e;
+    if (plan.shared == 0 || plan.shared_many == plan.many)
+        e = run(plan.many, plan.tiles > plan.shared_tiles ? plan.tiles : plan.shared_tiles, 0, plan.splits);
+    else {
+        e = run(plan.shared_many, plan.shared_tiles, 0, plan.shared_splits);
+        if (e == hipSuccess) e = run(plan.many, plan.tiles, plan.shared_splits, own);
+    }
     if (e != hipSuccess || plan.splits == 1) return e;
     return enqueue(attend_join_kernel<DP, TYPE>, dim3((unsigned)(((int64_t)p.T * p.H + 1024 / DP - 1) / (1024 / DP))), dim3(256), stream, p, plan, (const float*)part);
 }

@@ -84,6 +84,7 @@ struct PagedAttention {
     int64_t scale_stride[3];  // between pages, tokens of a page, heads
     const int32_t* prefix_lens;            // [B]: keys that a causal row sees whatever its position
     float cap, cap_by;        // scores become cap tanh: the cap times log2(e); 2 log2(e) scale / cap
+    int more;                 // not a plain call (also where everything below is zero)
     int shared;               // leading keys that lie in the same pages for all sequences, as the caller says
 };
 // Division by a number known on the host: its magic number and shift (magic 0: by one).
@@ -95,10 +96,12 @@ struct AttentionPlan {
     AttentionDivision page, group, workers;
     int group_size, tiles, splits, many;
     // leading keys computed once for all, with tiles of all sequences' rows together; of the splits the first ones are theirs
-    int shared, shared_tiles, shared_splits;
+    int shared, shared_tiles, shared_splits, shared_many;
     AttentionDivision shared_workers;
+    int small;                // few rows: half the wavefronts a workgroup
+    int z_first;              // of a launch: its first split
 };
-size_t paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int64_t max_kv, int64_t shared);
+size_t paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int64_t max_kv, int64_t shared, bool more);
 hipError_t launch_paged_attention(const PagedAttention& p, hipStream_t stream);
 
 // ---- residual, norm, quantizer ---------------------------------------------------------------------------------------

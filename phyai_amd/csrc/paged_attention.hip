@@ -2,6 +2,8 @@
 #include "attention.h"
 #include "tuning.h"
 
+#include <stdio.h>
+
 namespace phyai {
 namespace {
 
@@ -16,7 +18,7 @@ Division division(uint32_t d) {
 int64_t tiles_bound(int64_t T, int64_t B, int64_t group, int64_t rows) {
     return T * group / rows + (B < T ? B : T);   // every sequence with tokens adds less than one tile of its own
 }
-Plan make_plan(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int64_t max_kv, int64_t page_size, int64_t shared) {
+Plan make_plan(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int64_t max_kv, int64_t page_size) {
     Plan r = {};
     const int64_t group = H / KV;
     r.group_size = (int)group;
@@ -40,42 +42,69 @@ Plan make_plan(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int64_t m
         if (forced != nullptr) s = atoi(forced);
         r.splits = (int)(s < 1 ? 1 : s < MAX_SPLITS ? s : MAX_SPLITS);
     }
-    if (!r.many && shared > 0 && B > 1) {
-        const int64_t once = (T * group + ROWS - 1) / ROWS;   // tiles of all rows together
-        if (once < r.tiles) {
-            // Workgroups with about as many keys each, as many as run at once, at least a block for every wavefront.
-            const int64_t own = max_kv > shared ? max_kv - shared : 0, least = 32 * waves, at_once = DP == 64 ? 512 : 256;
-            int64_t keys = (once * KV * shared + r.tiles * KV * own + at_once - 1) / at_once;
-            keys = keys < least ? least : keys;
-            int64_t s = (shared + keys - 1) / keys, o = (own + keys - 1) / keys;
-            s = s < 1 ? 1 : s > MAX_SPLITS / 2 ? MAX_SPLITS / 2 : s;
-            o = o < 1 ? 1 : o > MAX_SPLITS / 2 ? MAX_SPLITS / 2 : o;
-            r.shared = (int)shared;
-            r.shared_tiles = (int)once;
-            r.shared_splits = (int)s;
-            r.shared_workers = division((uint32_t)(s * waves));
-            r.splits = (int)(s + o);
+    r.workers = division((uint32_t)(r.many ? 1 : r.splits * waves));
+    return r;
+}
+
+// Calls that are more than plain ones.  PHYAI_LAYER_ATTEND_MORE = "many splits small shared_many shared_splits" (shared_splits 0: nothing is shared).
+Plan make_plan_more(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int64_t max_kv, int64_t page_size, int64_t shared) {
+    Plan r = make_plan(T, B, H, KV, D, max_kv, page_size);
+    const int64_t group = H / KV;
+    const int DP = padded_dim(D), waves = DP == 256 ? 4 : 8;
+    int many = r.many, splits = r.splits, small = 0, shared_many = 0, shared_splits = 0;
+    if (tuning_env("PHYAI_LAYER_ATTEND") == nullptr) {
+        const int64_t at_once = DP == 64 ? 512 : 256;
+        small = !many && r.tiles * KV >= at_once;
+        if (shared > 0 && B > 1 && !many) {
+            const int64_t once = (T * group + ROWS - 1) / ROWS;   // tiles of all rows together
+            if (once < r.tiles) {
+                // Workgroups with about as many keys each, as many as run at once, at least a block for every wavefront.
+                const int64_t own = max_kv > shared ? max_kv - shared : 0, least = 32 * waves;
+                int64_t keys = (once * KV * shared + r.tiles * KV * own + at_once - 1) / at_once;
+                keys = keys < least ? least : keys;
+                shared_splits = (int)((shared + keys - 1) / keys);
+                splits = (int)((own + keys - 1) / keys);
+            }
         }
     }
-    r.workers = division((uint32_t)((r.splits - r.shared_splits) * waves));
+    if (const char* forced = tuning_env("PHYAI_LAYER_ATTEND_MORE")) sscanf(forced, "%d %d %d %d %d", &many, &splits, &small, &shared_many, &shared_splits);
+    auto held = [](int v, int most) { return v < 1 ? 1 : v < most ? v : most; };
+    r.many = many != 0;
+    r.small = small != 0;
+    r.tiles = (int)tiles_bound(T, B, group, r.many ? 128 : ROWS);
+    if (shared > 0 && shared_splits > 0) {
+        r.shared = (int)shared;
+        r.shared_many = shared_many != 0;
+        r.shared_tiles = (int)((T * group + (r.shared_many ? 128 : ROWS) - 1) / (r.shared_many ? 128 : ROWS));
+        r.shared_splits = held(shared_splits, MAX_SPLITS / 2);
+        splits = held(splits, MAX_SPLITS / 2);
+    } else splits = held(splits, MAX_SPLITS);
+    r.splits = r.shared_splits + splits;
+    const int wide = r.small ? waves / 2 : waves;
+    r.workers = division((uint32_t)(splits * (r.many ? 1 : wide)));
+    if (r.shared > 0) r.shared_workers = division((uint32_t)(r.shared_splits * (r.shared_many ? 1 : wide)));
     return r;
 }
 
 }  // namespace
 
-size_t paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int64_t max_kv, int64_t shared) {
+size_t paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int64_t max_kv, int64_t shared, bool more) {
     if (T <= 0 || B <= 0) return 0;
-    const Plan plan = make_plan(T, B, H, KV, D, max_kv, 1, shared);
-    if (plan.many || plan.splits == 1) return 0;
+    const Plan plan = more ? make_plan_more(T, B, H, KV, D, max_kv, 1, shared) : make_plan(T, B, H, KV, D, max_kv, 1);
+    if (plan.splits == 1) return 0;
     return (size_t)plan.splits * T * H * (padded_dim(D) + 2) * sizeof(float);
 }
 
 hipError_t launch_paged_attention(const PagedAttention& p, hipStream_t stream) {
-    const Plan plan = make_plan(p.T, p.B, p.H, p.KV, p.D, (int64_t)p.table_width * p.page_size, p.page_size, p.shared);
     const bool bf16 = p.type == HEAD_BF16;
+    const int64_t max_kv = (int64_t)p.table_width * p.page_size;
+    if (!p.more) {
+        const Plan plan = make_plan(p.T, p.B, p.H, p.KV, p.D, max_kv, p.page_size);
+        return bf16 ? launch_d<HEAD_BF16, 0>(p, plan, stream) : launch_d<HEAD_F16, 0>(p, plan, stream);
+    }
+    const Plan plan = make_plan_more(p.T, p.B, p.H, p.KV, p.D, max_kv, p.page_size, p.shared);
     if (p.k_scales != nullptr) return bf16 ? launch_attention_bf16_fp8(p, plan, stream) : launch_attention_f16_fp8(p, plan, stream);
-    if (p.cap > 0.f || p.prefix_lens != nullptr || plan.shared > 0) return bf16 ? launch_attention_bf16(p, plan, stream) : launch_attention_f16(p, plan, stream);
-    return bf16 ? launch_d<HEAD_BF16, 0>(p, plan, stream) : launch_d<HEAD_F16, 0>(p, plan, stream);
+    return bf16 ? launch_attention_bf16(p, plan, stream) : launch_attention_f16(p, plan, stream);
 }
 
 }  // namespace phyai

@@ -312,6 +312,18 @@ def test_attention(dev, monkeypatch, case, dtype, bits, plan):
     within(out, want, bound, "attention")
 
 
+@pytest.mark.parametrize("case", ATTEND, ids=name_of)
+@pytest.mark.parametrize("dtype,bits", [(torch.bfloat16, 8), (torch.float16, 16)])
+@pytest.mark.parametrize("plan", ["1 3 0", "1 1 0", "0 3 1", "0 1 1"])
+def test_attention_of_other_splits(dev, monkeypatch, case, dtype, bits, plan):
+    """Many rows with the keys split (1 3), few rows with half the wavefronts a workgroup (0 n 1)."""
+    monkeypatch.setenv("PHYAI_LAYER_ATTEND_MORE", plan)
+    tensors, kw = attend_case(case, dtype, bits, q_scale=4.0 if case[9] else 1.0)
+    want, bound = oracle.attention(*tensors.values(), **kw)
+    within(attend(dev, tensors, kw | dict(shared_prefix=0, prefix_lens=kw["prefix_lens"] if kw["prefix_lens"] is not None else
+                                          torch.zeros(len(case[0]), dtype=torch.int32))), want, bound, "attention")
+
+
 # new tokens and keys per sequence, page, heads, key heads, head_dim, causal, window, prompts, cap, shared
 SHARED = [
     ([1, 1], [20, 18], 16, 8, 1, 256, True, None, None, None, 16),
@@ -336,6 +348,17 @@ def test_shared_prefix(dev, case, dtype, bits):
     one = tensors | dict(page_table=tensors["page_table"][:1].expand(len(case[0]), -1)) if max(case[1]) <= case[-1] else None
     if one is not None:
         within(attend(dev, one, kw | dict(shared_prefix=case[-1])), want, bound, "one row for all")
+
+
+@pytest.mark.parametrize("case", SHARED, ids=name_of)
+@pytest.mark.parametrize("dtype,bits", [(torch.bfloat16, 8), (torch.float16, 16)])
+@pytest.mark.parametrize("plan", ["0 2 0 0 3", "0 2 1 1 3", "1 2 0 1 3", "1 1 0 0 2", "0 1 0 1 1"])
+def test_shared_prefix_of_other_splits(dev, monkeypatch, case, dtype, bits, plan):
+    """Many or few rows a workgroup for the shared keys and for the sequences' own, each with splits of their own."""
+    monkeypatch.setenv("PHYAI_LAYER_ATTEND_MORE", plan)
+    tensors, kw = attend_case(case[:-1], dtype, bits, shared=case[-1])
+    want, bound = oracle.attention(*tensors.values(), **kw)
+    within(attend(dev, tensors, kw | dict(shared_prefix=case[-1])), want, bound, "shared")
 
 
 def test_shared_prefix_beyond_the_table_and_of_one_sequence(dev):
