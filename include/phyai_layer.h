@@ -154,7 +154,8 @@ typedef struct {
 } phyai_layer_attention_options;
 
 size_t phyai_layer_paged_attention_more_workspace_bytes(int64_t T, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
-                                                        int64_t page_size, int64_t table_width, int64_t shared_prefix);
+                                                        int64_t page_size, int64_t table_width, int64_t shared_prefix,
+                                                        int64_t window);
 int phyai_layer_paged_attention_more(const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *k_pages,
                                      const void *v_pages, const int64_t *kv_strides, int64_t n_pages, int64_t page_size,
                                      const int32_t *page_table, int64_t table_stride, int64_t table_width, const int32_t *q_offsets,

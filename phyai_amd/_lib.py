@@ -75,7 +75,7 @@ LAYER_SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                          _i64, _i64, _i64, _i64, _f32, _int, _int, _int, _vp]),
     "phyai_layer_cache_read": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _int, _vp]),
     "phyai_layer_add_rmsnorm_quant": (_int, [_vp, _i64, _vp, _i64, _vp, _int, _f32, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _vp]),
-    "phyai_layer_paged_attention_more_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "phyai_layer_paged_attention_more_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64]),
     "phyai_layer_paged_attention_more": (_int, [_vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64,
                                                 _i64, _i64, _f32, _int, _i64, _int, _vp, _vp, _sz, _vp]),
 }

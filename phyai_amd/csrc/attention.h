@@ -270,13 +270,15 @@ struct Widener {
     const int begin, end, row;
     int page, lo, hi;                  // of the lane's key: its page in the turn to come; its offset
     uint32_t k_power, v_power, powers; // its scales as they were asked for; both, of the turn being stored
+    uint32_t both[LOADS];              // the scales of the block being stored
+    bool unknown;                      // a scale of the turn is a NaN
     uint64_t odd;                      // lanes whose key's page does not exist
     uint32_t at;                       // the lane's part of an address: its key of a load, its chunk
     uint32_t k_to, v_to;               // where its first chunk of load 0 goes in a buffer
     v4i k[LOADS], v[LOADS];            // of the block to come
 
     __device__ __forceinline__ Widener(const Pool& pool, int first, int last, int first_row)
-        : s(pool), begin(first), end(last), row(first_row), page(0), lo(0), hi(0), k_power(0), v_power(0), powers(0), odd(0) {
+        : s(pool), begin(first), end(last), row(first_row), page(0), lo(0), hi(0), k_power(0), v_power(0), powers(0), unknown(false), odd(0) {
         const uint32_t lane = threadIdx.x & 63, r = (uint32_t)row + lane / LANES, chunk = 2 * (lane % LANES) + turned();
         at = lane / LANES * (uint32_t)s.token_bytes + lane % LANES * 16;
         k_to = r * ROW + ((chunk ^ k_swizzle<DP>(r)) << 4);
@@ -344,25 +346,43 @@ struct Widener {
             v[i] = b;
         }
     }
-    __device__ __forceinline__ static void put(uint8_t* lds, uint32_t to, uint32_t power, const v4i& codes) {
+    __device__ __forceinline__ void put(uint8_t* lds, uint32_t to, uint32_t power, const v4i& codes) const {
         v4i w[2];
         widen16<TYPE>(turned() ? v4i{codes[2], codes[3], codes[0], codes[1]} : codes, power, w);
         *reinterpret_cast<v4i*>(lds + to) = w[0];
         *reinterpret_cast<v4i*>(lds + (to ^ 16u)) = w[1];
     }
-    // The block asked for last, which is `blk`, into the buffers.
-    __device__ __forceinline__ void store(int blk, uint8_t* k_lds, uint8_t* v_lds) {
-        const int lane = threadIdx.x & 63;
-        if ((blk - begin) % BLOCKS == 0) powers = k_power | v_power << 8;
-        uint32_t kt = k_to, vt = v_to;
-        asm volatile("" : "+v"(kt), "+v"(vt) :: "memory");   // (worked out here, not kept for each load)
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            const uint32_t both = (uint32_t)__shfl((int)powers, (blk - begin) % BLOCKS * N + i * PER + lane / LANES);
-            // (the swizzles of these keys are those of load 0's with the bits of i PER flipped)
-            put(k_lds, (kt ^ k_swizzle<DP>(i * PER) << 4) + i * PER * ROW, both & 255u, k[i]);
-            put(v_lds, (vt ^ v_swizzle<DP>(i * PER) << 4) + i * PER * ROW, both >> 8, v[i]);
+    // The block asked for last, which is `blk`, into the buffers, piece by piece of 2 LOADS (work to be done beside matrix
+    // products); its scales first.  Codes of a scale that is a NaN become NaNs.
+    static constexpr int PIECES = 2 * LOADS;
+    __device__ __forceinline__ void scales(int blk) {
+        if ((blk - begin) % BLOCKS == 0) {
+            powers = k_power | v_power << 8;
+            unknown = __any(k_power == 255 || v_power == 255);
         }
+        const int from = (blk - begin) % BLOCKS * N + (int)(threadIdx.x & 63) / LANES;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) both[i] = (uint32_t)__builtin_amdgcn_ds_bpermute((from + i * PER) * 4, (int)powers);
+        if (unknown) {   // (apart, so that the pieces are without a branch)
+            constexpr int NANS = (int)kNanCodes;
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                if ((both[i] & 255u) == 255u) k[i] = v4i{NANS, NANS, NANS, NANS};
+                if ((both[i] >> 8) == 255u) v[i] = v4i{NANS, NANS, NANS, NANS};
+            }
+        }
+    }
+    __device__ __forceinline__ void piece(int p, uint8_t* k_lds, uint8_t* v_lds) const {
+        const int i = p >> 1;
+        // (the swizzles of these keys are those of load 0's with the bits of i PER flipped)
+        if ((p & 1) == 0) put(k_lds, (k_to ^ k_swizzle<DP>(i * PER) << 4) + i * PER * ROW, both[i] & 255u, k[i]);
+        else put(v_lds, (v_to ^ v_swizzle<DP>(i * PER) << 4) + i * PER * ROW, both[i] >> 8, v[i]);
+    }
+    __device__ __forceinline__ void store(int blk, uint8_t* k_lds, uint8_t* v_lds) {
+        asm volatile("" ::: "memory");
+        scales(blk);
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) piece(p, k_lds, v_lds);
         asm volatile("" ::: "memory");
     }
 };
@@ -516,12 +536,10 @@ __device__ __forceinline__ void raise_maximum(State<DP>& st, float mx) {
 struct Cap {
     float by;
 };
-template <int NB>
-__device__ __forceinline__ void cap_scores(v16f (&s)[NB], Cap c) {
+template <int N>
+__device__ __forceinline__ void cap_some(v16f& s, int first, Cap c) {
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[n][i] = -__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[n][i] * c.by) + 1.0f);
+    for (int i = first; i < first + N; ++i) s[i] = -__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[i] * c.by) + 1.0f);
 }
 // Scores to probabilities, as the second product's operand.  The sum is of the rounded ones, those that the product uses:
 // their common error cancels.
@@ -546,8 +564,25 @@ __device__ __forceinline__ float probabilities(v16f& s, v4i (&pf)[2], float m, f
 // no row of the wavefront sees any of it); all rows see whole_lo .. whole_hi.  The loop inside touches O by matrix products
 // alone; a step that raises a maximum leaves it, is finished outside, and the loop goes on behind it.  (With the rescaling
 // inside, 256 dims' O moved from the accumulation registers and back for every block: 256 instructions beside 32 products.)
-template <int DP, int TYPE, int NB, int MODE, typename Top>
-__device__ __forceinline__ void attend_steps(State<DP>& st, const v4i* qf, int step, int end, const Row& row, int whole_lo, int whole_hi, float c, Cap cap, Top top) {
+// beside: work of a step that has nothing to do with its keys, done between the products with its values, a piece at a time, and all at
+// once where the maximum rises.  (No step is left out then, also where a wavefront's rows see nothing of it: a way round the products
+// made the compiler keep O in memory.)
+struct Nothing {
+    static constexpr int PIECES = 0;
+    __device__ __forceinline__ void start(int) const {}
+    __device__ __forceinline__ void piece(int) const {}
+};
+template <typename Beside>
+__device__ __forceinline__ void all_pieces(const Beside& beside, int step) {
+    if constexpr (Beside::PIECES > 0) {
+        beside.start(step);
+#pragma unroll
+        for (int p = 0; p < Beside::PIECES; ++p) beside.piece(p);
+    }
+}
+template <int DP, int TYPE, int NB, int MODE, typename Top, typename Beside>
+__device__ __forceinline__ void attend_steps(State<DP>& st, const v4i* qf, int step, int end, const Row& row, int whole_lo, int whole_hi, float c, Cap cap, Top top,
+                                             const Beside& beside) {
     using S = Shape<DP>;
     // V is read while the scores are turned into probabilities; as much of it as there are registers for
     constexpr int EARLY = DP == 64 || (DP == 128 && (MODE & MODE_FP8) && (MODE & MODE_CAP)) ? 2 : NB == 1 || DP == 256 ? 4 : 2;
@@ -559,7 +594,9 @@ __device__ __forceinline__ void attend_steps(State<DP>& st, const v4i* qf, int s
 #pragma unroll 1
         for (; step < end; ++step) {
             k = top(step);
-            if (k == nullptr) continue;
+            if constexpr (Beside::PIECES == 0) {
+                if (k == nullptr) continue;
+            }
             v = k + NB * 32 * S::ROW;
             v4i kf[DP / 16], vf[EARLY][2], pf[NB][2];
             // a block's reads all together, during the products of the one before: left to itself the compiler reads two,
@@ -574,6 +611,9 @@ __device__ __forceinline__ void attend_steps(State<DP>& st, const v4i* qf, int s
 #pragma unroll
                 for (int kk = 0; kk < DP / 16; ++kk) {
                     s[n] = mfma<TYPE>(kf[kk], qf[kk], s[n]);
+                    if constexpr ((MODE & MODE_CAP) != 0) {   // the scores of the block before, meanwhile
+                        if (n > 0) cap_some<256 / DP>(s[n > 0 ? n - 1 : 0], kk * (256 / DP), cap);
+                    }
                     if (n + 1 < NB) kf[kk] = read_k<DP>(k, 32 * (n + 1), kk);
                 }
                 if (n + 1 == NB) {
@@ -584,7 +624,7 @@ __device__ __forceinline__ void attend_steps(State<DP>& st, const v4i* qf, int s
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
-            if constexpr (MODE & MODE_CAP) cap_scores<NB>(s, cap);
+            if constexpr (MODE & MODE_CAP) cap_some<16>(s[NB - 1], 0, cap);
             const int j0 = step * (32 * NB);
             if (j0 < whole_lo || j0 + 32 * NB > whole_hi) {
 #pragma unroll
@@ -593,6 +633,7 @@ __device__ __forceinline__ void attend_steps(State<DP>& st, const v4i* qf, int s
             mx = max_score<NB>(s) * c;
             rises = maximum_rises(st.m, mx);
             if (rises) break;
+            if constexpr (Beside::PIECES > 0) beside.start(step);
 #pragma unroll
             for (int n = 0; n < NB; ++n) st.l += probabilities<TYPE>(s[n], pf[n], st.m, c);
 #pragma unroll
@@ -600,9 +641,17 @@ __device__ __forceinline__ void attend_steps(State<DP>& st, const v4i* qf, int s
 #pragma unroll
                 for (int b = 0; b < DP / 32; ++b)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) st.o[b] = mfma<TYPE>(n == 0 && b < EARLY ? vf[b % EARLY][e] : read_v<DP>(v, 32 * n, b, e), pf[n][e], st.o[b]);
+                    for (int e = 0; e < 2; ++e) {
+                        st.o[b] = mfma<TYPE>(n == 0 && b < EARLY ? vf[b % EARLY][e] : read_v<DP>(v, 32 * n, b, e), pf[n][e], st.o[b]);
+                        if constexpr (Beside::PIECES > 0) {
+                            constexpr int EACH = NB * (DP / 16) / Beside::PIECES;
+                            const int at = (n * (DP / 32) + b) * 2 + e;
+                            if (at % EACH == 0) beside.piece(at / EACH);
+                        }
+                    }
         }
         if (!rises) break;
+        all_pieces(beside, step);
         raise_maximum<DP>(st, mx);
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
@@ -732,7 +781,7 @@ __device__ __forceinline__ Row row_of_shared(const PagedAttention& p, const Tile
     r.head = kv_head * g.group_size + (r.valid ? row - i * g.group_size : 0);
     // how many sequences end at or before the row's token, 64 of them and a token at a time
     const int last = first + ROWS < t.rows ? first + ROWS - 1 : t.rows - 1;
-    const int i0 = divide(first < t.rows ? first : 0, g.group), i1 = divide(last, g.group);
+    const int i0 = divide(first < t.rows ? first : 0, g.group), i1 = first < t.rows ? divide(last, g.group) : -1;   // (none: no row is there)
     int b = 0;
     for (int base = 0; base < p.B; base += 64) {
         const int end = base + lane < p.B ? p.q_offsets[base + lane + 1] : 0x7FFFFFFF;
@@ -825,7 +874,7 @@ __global__ __launch_bounds__(WAVES_OF * 64, SPLIT_WAVES<DP> / WAVES_OF) void att
                 if (blk + 1 < end) feed.load(blk + 1);
                 if (blk * 32 < all_lo || blk * 32 + 32 > all_hi) special |= clean_values<DP, TYPE, 32>(mine + 32 * S::ROW, t.kv_len - blk * 32);
                 return mine;
-            });
+            }, Nothing());
         }
     } else if (begin < end) {
         const uint32_t base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)mine);
@@ -843,7 +892,7 @@ __global__ __launch_bounds__(WAVES_OF * 64, SPLIT_WAVES<DP> / WAVES_OF) void att
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             if (blk * 32 < all_lo || blk * 32 + 32 > all_hi) special |= clean_values<DP, TYPE, 32>(mine + 32 * S::ROW, t.kv_len - blk * 32);
             return mine;
-        });
+        }, Nothing());
     }
     if (special) {
 #pragma unroll 1
@@ -993,6 +1042,19 @@ __device__ __forceinline__ bool place(const PagedAttention& p, int tiles, int& t
     return true;
 }
 
+// The step behind the one that is worked on, widened beside its products into the buffers at `next` (V: V_AT bytes further).
+template <typename W, int V_AT>
+struct Widening {
+    static constexpr int PIECES = W::PIECES;
+    W& wide;
+    uint8_t*& next;
+    const int end;
+    __device__ __forceinline__ void start(int step) const {
+        if (step + 1 < end) wide.scales(step + 1);
+    }
+    __device__ __forceinline__ void piece(int p) const { wide.piece(p, next, next + V_AT); }
+};
+
 template <int DP, int TYPE, int MODE>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(const PagedAttention p, const Plan g, float* __restrict__ part) {
     using S = Shape<DP>;
@@ -1059,16 +1121,12 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
     v4i qf[DP / 16];
     load_q<DP>(p, row, qf);
     bool special = false;
-    auto widen = [&](int step) {
-        uint8_t* to = lds + (uint32_t)((step - begin) & 1) * X::STAGE;
-        wide.store(step, to, to + X::STEP * S::ROW);
-        if (step + 1 < end) wide.load(step + 1);
-    };
     if (begin < end) {
         if constexpr (MODE & MODE_FP8) {
             wide.ask(0);
             wide.load(begin);
-            widen(begin);
+            wide.store(begin, lds, lds + X::STEP * S::ROW);
+            if (DP == 128 && begin + 1 < end) wide.load(begin + 1);
         } else {
             feed.ask(0);
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -1082,18 +1140,30 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
     for (int b = 0; b < DP / 32; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i) st.o[b][i] = 0.f;
-    attend_steps<DP, TYPE, X::STEP / 32, MODE>(st, qf, begin, end, row, whole_lo, whole_hi, c, cap, [&](int step) -> const uint8_t* {
+    // Pages in 8 bits: the step to come is asked for at the top of this one and widened beside its products.  (In the last step
+    // what is there is stored once more, where nobody reads it.)  At 128 dims, where two wavefronts share a SIMD and their registers
+    // do not reach for that, it is widened at the top and the one behind it asked for.
+    constexpr bool BESIDE = (MODE & MODE_FP8) != 0 && DP != 128;
+    uint8_t* next = lds;
+    auto top = [&](int step) -> const uint8_t* {
         if constexpr (!(MODE & MODE_FP8)) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this step has landed; behind the barrier everybody has read the one before it
         uint8_t* k = lds + (uint32_t)((step - begin) & 1) * X::STAGE;
         const int j0 = step * X::STEP;
         if (j0 < all_lo || j0 + X::STEP > all_hi) special |= clean_values<DP, TYPE, X::MINE>(k + (X::STEP + wave * X::MINE) * S::ROW, t.kv_len - j0 - wave * X::MINE);
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (step + 1 < end) {
-            if constexpr (MODE & MODE_FP8) widen(step + 1);
-            else copy(step + 1);
-        }
-        return j0 >= my_hi || j0 + X::STEP <= my_lo ? nullptr : k;
-    });
+        if constexpr (MODE & MODE_FP8) {
+            next = lds + (uint32_t)((step + 1 - begin) & 1) * X::STAGE;
+            if constexpr (BESIDE) {
+                if (step + 1 < end) wide.load(step + 1);
+            } else if (step + 1 < end) {
+                wide.store(step + 1, next, next + X::STEP * S::ROW);
+                if (step + 2 < end) wide.load(step + 2);
+            }
+        } else if (step + 1 < end) copy(step + 1);
+        return !BESIDE && (j0 >= my_hi || j0 + X::STEP <= my_lo) ? nullptr : k;
+    };
+    if constexpr (BESIDE) attend_steps<DP, TYPE, X::STEP / 32, MODE>(st, qf, begin, end, row, whole_lo, whole_hi, c, cap, top, Widening<decltype(wide), X::STEP * S::ROW>{wide, next, end});
+    else attend_steps<DP, TYPE, X::STEP / 32, MODE>(st, qf, begin, end, row, whole_lo, whole_hi, c, cap, top, Nothing());
     if (lane == 0) specials[wave] = special ? 1 : 0;
     __syncthreads();
     if ((specials[0] | specials[1] | specials[2] | specials[3]) != 0) {

@@ -24,6 +24,7 @@ __global__ __launch_bounds__(256) void cache_read_kernel(const CacheRead p, int 
         codes = *reinterpret_cast<const v4i*>((value ? p.v_pages : p.k_pages) + page * s[0] + at * s[1] + h * s[2] + chunk * 16);
         power = (value ? p.v_scales : p.k_scales)[page * b[0] + at * b[1] + h * b[2]];
     }
+    if (power == 255) codes = v4i{(int)kNanCodes, (int)kNanCodes, (int)kNanCodes, (int)kNanCodes};
     v4i out[2];
     widen16<TYPE>(codes, power, out);
     uint16_t* o = (value ? p.v_out : p.k_out) + (t * p.KV + h) * p.D + chunk * 16;

@@ -993,7 +993,7 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     } else o = fresh3(T, H, D, dtype, at_.dev);
     Scratch ws = {nullptr, 0};
     if (fp8 || more.softcap > 0.f || more.prefix_lens || more.shared_prefix > 0) {
-        const size_t need = lib.attention_more_ws(T, B, H, kp->size(2), D, kp->size(1), W, more.shared_prefix);
+        const size_t need = lib.attention_more_ws(T, B, H, kp->size(2), D, kp->size(1), W, more.shared_prefix, window);
         if (need > 0 && !workspace(need, at_, &ws)) return declined();
         if (lib.attention_more(q->const_data_ptr(), q->stride(0), q->stride(1), kp->const_data_ptr(), vp->const_data_ptr(), ks, kp->size(0), kp->size(1),
                                table->const_data_ptr<int32_t>(), table->stride(0), W, offsets->const_data_ptr<int32_t>(), lens->const_data_ptr<int32_t>(),

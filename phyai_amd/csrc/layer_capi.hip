@@ -85,9 +85,9 @@ int64_t whole_pages(int64_t shared, int64_t page_size, int64_t table_width) {
     const int64_t pages = shared / page_size;
     return (pages < table_width ? pages : table_width) * page_size;
 }
-size_t attention_workspace(int64_t T, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_kv, int64_t shared, bool more) {
+size_t attention_workspace(int64_t T, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_kv, int64_t shared, int64_t window, bool more) {
     if (T <= 0 || batch <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || heads % kv_heads != 0 || T >= kMost || T * heads >= kMost) return 0;
-    const size_t n = phyai::paged_attention_workspace_bytes(T, batch, heads, kv_heads, head_dim, max_kv, shared, more);
+    const size_t n = phyai::paged_attention_workspace_bytes(T, batch, heads, kv_heads, head_dim, max_kv, shared, window, more);
     return n == 0 ? 0 : PHYAI_FP8_WORKSPACE_HEADER_BYTES + n;
 }
 
@@ -203,7 +203,7 @@ int attention(const char* fn, const void* q, int64_t q_token_stride, int64_t q_h
             if (more->scale_strides[i] < 0) return fail(PHYAI_FP8_EINVAL, "%s: strides of the scales must not be negative", fn);
         }
     const int64_t shared = more ? whole_pages(more->shared_prefix, page_size, table_width) : 0;
-    const size_t need = attention_workspace(T, batch, heads, kv_heads, head_dim, table_width * page_size, shared, more != nullptr);
+    const size_t need = attention_workspace(T, batch, heads, kv_heads, head_dim, table_width * page_size, shared, window, more != nullptr);
     if (need > 0 && (!workspace || !aligned(workspace, 256) || workspace_bytes < need))
         return fail(PHYAI_FP8_EWORKSPACE, "%s: workspace of %zu bytes is missing, unaligned or smaller than %zu", fn, workspace ? workspace_bytes : (size_t)0, need);
     phyai::PagedAttention p = {};
@@ -425,13 +425,13 @@ int phyai_layer_add_rmsnorm_quant(const void* x, int64_t ldx, const void* residu
 }
 
 size_t phyai_layer_paged_attention_workspace_bytes(int64_t T, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_kv) {
-    return attention_workspace(T, batch, heads, kv_heads, head_dim, max_kv, 0, false);
+    return attention_workspace(T, batch, heads, kv_heads, head_dim, max_kv, 0, 0, false);
 }
 
 size_t phyai_layer_paged_attention_more_workspace_bytes(int64_t T, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t page_size,
-                                                        int64_t table_width, int64_t shared_prefix) {
-    if (page_size <= 0 || table_width < 0 || page_size >= kMost || table_width >= kMost) return 0;
-    return attention_workspace(T, batch, heads, kv_heads, head_dim, table_width * page_size, whole_pages(shared_prefix, page_size, table_width), true);
+                                                        int64_t table_width, int64_t shared_prefix, int64_t window) {
+    if (page_size <= 0 || table_width < 0 || page_size >= kMost || table_width >= kMost || shared_prefix < 0) return 0;
+    return attention_workspace(T, batch, heads, kv_heads, head_dim, table_width * page_size, whole_pages(shared_prefix, page_size, table_width), window, true);
 }
 
 int phyai_layer_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_pages, const void* v_pages,

@@ -101,7 +101,8 @@ struct AttentionPlan {
     int small;                // few rows: half the wavefronts a workgroup
     int z_first;              // of a launch: its first split
 };
-size_t paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int64_t max_kv, int64_t shared, bool more);
+size_t paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int64_t max_kv, int64_t shared, int64_t window,
+                                       bool more);
 hipError_t launch_paged_attention(const PagedAttention& p, hipStream_t stream);
 
 // ---- residual, norm, quantizer ---------------------------------------------------------------------------------------

@@ -46,25 +46,77 @@ Plan make_plan(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int64_t m
     return r;
 }
 
-// Calls that are more than plain ones.  PHYAI_LAYER_ATTEND_MORE = "many splits small shared_many shared_splits" (shared_splits 0: nothing is shared).
-Plan make_plan_more(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int64_t max_kv, int64_t page_size, int64_t shared) {
+// What a launch is expected to take, in us: workgroups of one kind, `n` of them with `keys` each, of which `at_once` run together.
+struct Part {
+    int64_t n;
+    double each;
+};
+double together(const Part* parts, int count, int64_t at_once) {
+    int64_t n = 0;
+    double sum = 0, longest = 0;
+    for (int i = 0; i < count; ++i) {
+        n += parts[i].n;
+        sum += (double)parts[i].n * parts[i].each;
+        longest = longest > parts[i].each ? longest : parts[i].each;
+    }
+    return n <= at_once ? longest : sum / (double)at_once + 0.3 * longest > longest ? sum / (double)at_once + 0.3 * longest : longest;
+}
+
+// Calls that are more than plain ones: few rows a workgroup with all its wavefronts or half of them (two of those a CU), or many rows, each
+// with the keys split or not, and shared keys in one launch with the sequences' own (both few rows) or in one before it (many rows).  The
+// choice with the least expected time; a workgroup takes its start (9 us for few rows, 12 for many: most of it instructions that a cold
+// cache does not have, and three turns of memory) and its blocks of 32 keys a wavefront, or steps of 64, at what they take where the
+// CU is full; sums to be joined take 4.5.  Measured, few rows with all wavefronts / half of them / many rows, best number of splits each, 8 bits and
+// 32 heads on 8 of 128 dims unless said: 64 single tokens of 8192 keys 177 / 169 / -, 16 of them 53 / 48, 4 of them 20 / 22, 32 of 400 11 / 14, 256 of
+// 1000 114 / 94; 256 tokens of 1024 20 / 27 / 31, 512 of 512 26 / 19 / 26, 512 of 4096 79 / 71 / 63, 2048 of 8192 625 / 567 / 360; 1000 of 1000 of 64
+// dims 39 / 29 / 38; 16 x 816 of 816 of 256 dims in 16 bits 149 / 124 / 103.  64 tokens behind 8192 shared keys and up to 512 of their
+// own: few and few rows 67, many and few 53, nothing shared 180; 16 of them 28 and 35.
+// PHYAI_LAYER_ATTEND_MORE = "many splits small shared_many shared_splits" (shared_splits 0: nothing is shared) forces one.
+Plan make_plan_more(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int64_t max_kv, int64_t page_size, int64_t shared, int64_t window) {
     Plan r = make_plan(T, B, H, KV, D, max_kv, page_size);
     const int64_t group = H / KV;
     const int DP = padded_dim(D), waves = DP == 256 ? 4 : 8;
     int many = r.many, splits = r.splits, small = 0, shared_many = 0, shared_splits = 0;
     if (tuning_env("PHYAI_LAYER_ATTEND") == nullptr) {
-        const int64_t at_once = DP == 64 ? 512 : 256;
-        small = !many && r.tiles * KV >= at_once;
-        if (shared > 0 && B > 1 && !many) {
-            const int64_t once = (T * group + ROWS - 1) / ROWS;   // tiles of all rows together
-            if (once < r.tiles) {
-                // Workgroups with about as many keys each, as many as run at once, at least a block for every wavefront.
-                const int64_t own = max_kv > shared ? max_kv - shared : 0, least = 32 * waves;
-                int64_t keys = (once * KV * shared + r.tiles * KV * own + at_once - 1) / at_once;
-                keys = keys < least ? least : keys;
-                shared_splits = (int)((shared + keys - 1) / keys);
-                splits = (int)((own + keys - 1) / keys);
+        const double block = DP == 256 ? 3.0 : 2.4, join = 4.5;
+        const int64_t few = tiles_bound(T, B, group, ROWS) * KV, wide = tiles_bound(T, B, group, 128) * KV;
+        const int64_t seen = window > 0 && window + T / B + 64 < max_kv ? window + T / B + 64 : max_kv;   // keys of a tile
+        auto ceiling = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+        auto few_rows = [&](int64_t tiles, int64_t keys, int s, int half) {
+            return Part{tiles * s, 9.0 + (double)ceiling(keys, 32 * (half ? waves / 2 : waves) * s) * block};
+        };
+        auto many_rows = [&](int64_t tiles, int64_t keys, int s) {
+            const double step = DP == 256 ? 3.5 : DP == 128 ? (tiles * s <= 256 ? 1.9 : 2.5) : tiles * s <= 256 ? 1.6 : 2.2;
+            return Part{tiles * s, 12.0 + (double)ceiling(keys, 64 * s) * step};
+        };
+        const int64_t at_once_few = DP == 64 ? 512 : 256, at_once_many = DP == 256 ? 256 : 512;
+        auto moved = [&](int s) { return s > 1 ? join + (double)(T * H) * DP * s / 1.5e6 : 0.0; };   // (the sums of all splits)
+        double best = 1e30;
+        auto take = [&](double t, int m, int s, int h, int sm, int ss) {
+            if (t >= best) return;
+            best = t;
+            many = m; splits = s; small = h; shared_many = sm; shared_splits = ss;
+        };
+        for (int s = 1; s <= MAX_SPLITS; s = s < 8 ? s + 1 : s + s / 4) {
+            for (int h = 0; h < 2; ++h) {
+                const Part p = few_rows(few, seen, s, h);
+                if (s == 1 || seen >= 32 * (h ? waves / 2 : waves) * (s - 1)) take(together(&p, 1, at_once_few << h) + moved(s), 0, s, h, 0, 0);
             }
+            const Part p = many_rows(wide, seen, s);
+            if (s == 1 || seen >= 128 * s) take(together(&p, 1, at_once_many) + moved(s), 1, s, 0, 0, 0);
+        }
+        if (shared > 0 && B > 1) {
+            const int64_t own = max_kv > shared ? max_kv - shared : 1, once = ceiling(T * group, ROWS) * KV, once_wide = ceiling(T * group, 128) * KV;
+            for (int ss = 1; ss <= MAX_SPLITS / 2; ss *= 2)
+                for (int s = 1; s <= 4; s *= 2)
+                    for (int h = 0; h < 2; ++h) {
+                        const Part both[2] = {few_rows(once, shared, ss, h), few_rows(few, own, s, h)};
+                        const Part before = many_rows(once_wide, shared, ss), wide_own = many_rows(wide, own, s);
+                        const Part all_many[2] = {before, wide_own};
+                        take(together(both, 2, at_once_few << h) + moved(ss + s), 0, s, h, 0, ss);
+                        if (shared >= 128 * ss) take(together(&before, 1, at_once_many) + together(both + 1, 1, at_once_few << h) + moved(ss + s), 0, s, h, 1, ss);
+                        if (shared >= 128 * ss && h == 0) take(together(all_many, 2, at_once_many) + moved(ss + s), 1, s, 0, 1, ss);
+                    }
         }
     }
     if (const char* forced = tuning_env("PHYAI_LAYER_ATTEND_MORE")) sscanf(forced, "%d %d %d %d %d", &many, &splits, &small, &shared_many, &shared_splits);
@@ -88,9 +140,9 @@ Plan make_plan_more(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int6
 
 }  // namespace
 
-size_t paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int64_t max_kv, int64_t shared, bool more) {
+size_t paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int64_t max_kv, int64_t shared, int64_t window, bool more) {
     if (T <= 0 || B <= 0) return 0;
-    const Plan plan = more ? make_plan_more(T, B, H, KV, D, max_kv, 1, shared) : make_plan(T, B, H, KV, D, max_kv, 1);
+    const Plan plan = more ? make_plan_more(T, B, H, KV, D, max_kv, 1, shared, window) : make_plan(T, B, H, KV, D, max_kv, 1);
     if (plan.splits == 1) return 0;
     return (size_t)plan.splits * T * H * (padded_dim(D) + 2) * sizeof(float);
 }
@@ -102,7 +154,7 @@ hipError_t launch_paged_attention(const PagedAttention& p, hipStream_t stream) {
         const Plan plan = make_plan(p.T, p.B, p.H, p.KV, p.D, max_kv, p.page_size);
         return bf16 ? launch_d<HEAD_BF16, 0>(p, plan, stream) : launch_d<HEAD_F16, 0>(p, plan, stream);
     }
-    const Plan plan = make_plan_more(p.T, p.B, p.H, p.KV, p.D, max_kv, p.page_size, p.shared);
+    const Plan plan = make_plan_more(p.T, p.B, p.H, p.KV, p.D, max_kv, p.page_size, p.shared, p.window);
     if (p.k_scales != nullptr) return bf16 ? launch_attention_bf16_fp8(p, plan, stream) : launch_attention_f16_fp8(p, plan, stream);
     return bf16 ? launch_attention_bf16(p, plan, stream) : launch_attention_f16(p, plan, stream);
 }

@@ -21,14 +21,13 @@ __device__ __forceinline__ uint32_t widen2(uint32_t codes, float power, bool upp
         return __builtin_bit_cast(uint32_t, v);
     }
 }
-// Sixteen codes, as two chunks of eight values.
+// Sixteen codes, as two chunks of eight values; of a known power.
 template <int TYPE>
 __device__ __forceinline__ void widen16(const v4i& codes, uint32_t power, v4i* out) {
     const float by = __uint_as_float(power << 23);
-    const bool unknown = power == 255;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-        const uint32_t a = unknown ? kNanCodes : (uint32_t)codes[2 * x], b = unknown ? kNanCodes : (uint32_t)codes[2 * x + 1];
+        const uint32_t a = (uint32_t)codes[2 * x], b = (uint32_t)codes[2 * x + 1];
         out[x] = v4i{(int)widen2<TYPE>(a, by, false), (int)widen2<TYPE>(a, by, true), (int)widen2<TYPE>(b, by, false), (int)widen2<TYPE>(b, by, true)};
     }
 }

@@ -1135,12 +1135,13 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         if fp8:
             options.k_scales, options.v_scales, options.scale_strides = k_scales.data_ptr(), v_scales.data_ptr(), _strides3(k_scales)
         with _device_of(dev):
-            need = lib.phyai_layer_paged_attention_more_workspace_bytes(T, B, H, KV, D, page_size, W, int(shared_prefix))
+            held = min(int(window), (1 << 31) - 1) if window is not None else 0
+            need = lib.phyai_layer_paged_attention_more_workspace_bytes(T, B, H, KV, D, page_size, W, int(shared_prefix), held)
             ws = reserve_workspace(need, dev) if need else None
             rc = lib.phyai_layer_paged_attention_more(
                 q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), v_pages.data_ptr(), _strides3(k_pages), n_pages, page_size,
                 page_table.data_ptr(), page_table.stride(0), W, offsets, lens, out.data_ptr(), T, B, H, KV, D, scale, 1 if causal else 0,
-                min(int(window), (1 << 31) - 1) if window is not None else 0, _HEAD_TYPES[dtype], ctypes.byref(options),
+                held, _HEAD_TYPES[dtype], ctypes.byref(options),
                 ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, _stream_ptr())
         _lib.check_layer(rc, op)
         return out
