@@ -6,10 +6,13 @@
 //     codes = e4m3(n / scale_g)                              (round to nearest even)
 //
 // A workgroup has a row, in registers: both inputs are read once, the sum and the codes written once.  Sixteen lanes of eight
-// elements are a group of 128, so its maximum takes four steps inside a row of lanes; a row's goes through LDS.
+// elements are a group of 128, so its maximum takes four steps inside a row of lanes; a row's goes through LDS.  Bound by memory, seven
+// bytes an element: 13056 x 2048 in 31.4 us, 6.0 TB/s (the last states of a loop are still in the caches; 34.8, 5.4, where three take
+// turns), where a large copy runs at 4.9; one row 2.6 us, the launch and a turn of memory.
 #include "fp8_device.h"
 #include "layer_kernels.h"
 #include "quant_device.h"
+#include "tuning.h"
 
 namespace phyai {
 namespace {
@@ -71,43 +74,41 @@ __device__ __forceinline__ void normed8(const v4i& t, const v4i& w, float r, flo
     for (int i = 0; i < 8; ++i) n[i] = n[i] * r * (wf[i] + more);
 }
 
-template <int THREADS>
+// Over the workgroup's wavefronts, whose words are in LDS, in their order.
 __device__ __forceinline__ float sum_of_all(float v, float* words) {
+    const int waves = blockDim.x / kWave;
     v = wave_sum_f32(v);
-    if constexpr (THREADS > kWave) {
-        constexpr int WAVES = THREADS / kWave;
+    if (waves > 1) {
         if (threadIdx.x % kWave == 0) words[threadIdx.x / kWave] = v;
         __syncthreads();
         v = words[0];
-#pragma unroll
-        for (int i = 1; i < WAVES; ++i) v += words[i];
+        for (int i = 1; i < waves; ++i) v += words[i];
     }
     return v;
 }
-template <int THREADS>
 __device__ __forceinline__ uint32_t max_of_all(uint32_t v, uint32_t* words) {
+    const int waves = blockDim.x / kWave;
     v = wave_max_u32(v);
-    if constexpr (THREADS > kWave) {
-        constexpr int WAVES = THREADS / kWave;
+    if (waves > 1) {
         if (threadIdx.x % kWave == 0) words[threadIdx.x / kWave] = v;
         __syncthreads();
         v = words[0];
-#pragma unroll
-        for (int i = 1; i < WAVES; ++i) v = words[i] > v ? words[i] : v;
+        for (int i = 1; i < waves; ++i) v = words[i] > v ? words[i] : v;
     }
     return v;
 }
 
-template <int THREADS, int CHUNKS, bool BLOCKS>
-__global__ __launch_bounds__(THREADS) void add_norm_kernel(const AddNorm p) {
-    __shared__ float sums[THREADS / kWave];
-    __shared__ uint32_t maxima[THREADS / kWave];
+template <int CHUNKS, bool BLOCKS>
+__global__ __launch_bounds__(1024) void add_norm_kernel(const AddNorm p) {
+    __shared__ float sums[1024 / kWave];
+    __shared__ uint32_t maxima[1024 / kWave];
+    const int threads = blockDim.x;
     const int64_t row = blockIdx.x;
     const uint16_t *x = p.x + row * p.ldx, *residual = p.residual + row * p.ldr;
     v4i t[CHUNKS], w[CHUNKS];
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
-        const int k = (c * THREADS + threadIdx.x) * 8;
+        const int k = (c * threads + threadIdx.x) * 8;
         t[c] = v4i{0, 0, 0, 0};
         w[c] = v4i{0, 0, 0, 0};
         if (k < p.D) {
@@ -118,21 +119,21 @@ __global__ __launch_bounds__(THREADS) void add_norm_kernel(const AddNorm p) {
     float ss = 0.f;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
-        const int k = (c * THREADS + threadIdx.x) * 8;
+        const int k = (c * threads + threadIdx.x) * 8;
         if (k < p.D) *reinterpret_cast<v4i*>(p.total + row * p.ldt + k) = t[c];
         float f[8];
         unpack8(t[c], f);
 #pragma unroll
         for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(f[i], f[i], ss);
     }
-    ss = sum_of_all<THREADS>(ss, sums);
+    ss = sum_of_all(ss, sums);
     const float r = 1.0f / __builtin_sqrtf(ss / (float)p.D + p.eps), more = p.gemma ? 1.0f : 0.0f;
     uint8_t* codes = p.xq + row * (int64_t)p.D;
     float* scale = p.scale + row * p.xs_row;
     if constexpr (BLOCKS) {
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
-            const int k = (c * THREADS + threadIdx.x) * 8;
+            const int k = (c * threads + threadIdx.x) * 8;
             float n[8];
             normed8(t[c], w[c], r, more, n);
             const float s = scale_of(max_of_16_lanes(amax8(n)));
@@ -149,12 +150,12 @@ __global__ __launch_bounds__(THREADS) void add_norm_kernel(const AddNorm p) {
             const uint32_t a = amax8(n);
             m = a > m ? a : m;
         }
-        const float s = scale_of(max_of_all<THREADS>(m, maxima));
+        const float s = scale_of(max_of_all(m, maxima));
         if (threadIdx.x == 0) scale[0] = s;
         const StaticDivisor d = make_static_divisor(s);
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
-            const int k = (c * THREADS + threadIdx.x) * 8;
+            const int k = (c * threads + threadIdx.x) * 8;
             float n[8];
             normed8(t[c], w[c], r, more, n);
             if (k < p.D) *reinterpret_cast<uint2*>(codes + k) = encode8(n, d);
@@ -179,7 +180,7 @@ __global__ __launch_bounds__(512) void add_norm_long_kernel(const AddNorm p) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(f[i], f[i], ss);
     }
-    ss = sum_of_all<512>(ss, sums);
+    ss = sum_of_all(ss, sums);
     const float r = 1.0f / __builtin_sqrtf(ss / (float)p.D + p.eps), more = p.gemma ? 1.0f : 0.0f;
     uint8_t* codes = p.xq + row * (int64_t)p.D;
     float* scale = p.scale + row * p.xs_row;
@@ -192,7 +193,7 @@ __global__ __launch_bounds__(512) void add_norm_long_kernel(const AddNorm p) {
             const uint32_t a = amax8(n);
             m = a > m ? a : m;
         }
-        const float s = scale_of(max_of_all<512>(m, maxima));
+        const float s = scale_of(max_of_all(m, maxima));
         if (threadIdx.x == 0) scale[0] = s;
         d = make_static_divisor(s);
     }
@@ -213,13 +214,25 @@ __global__ __launch_bounds__(512) void add_norm_long_kernel(const AddNorm p) {
 template <bool BLOCKS>
 hipError_t launch_blocks(const AddNorm& p, hipStream_t stream) {
     const dim3 grid((uint32_t)p.M);
-    if (p.D <= 512) return enqueue(add_norm_kernel<64, 1, BLOCKS>, grid, dim3(64), stream, p);
-    if (p.D <= 1024) return enqueue(add_norm_kernel<128, 1, BLOCKS>, grid, dim3(128), stream, p);
-    if (p.D <= 2048) return enqueue(add_norm_kernel<256, 1, BLOCKS>, grid, dim3(256), stream, p);
-    if (p.D <= 4096) return enqueue(add_norm_kernel<256, 2, BLOCKS>, grid, dim3(256), stream, p);
-    if (p.D <= 8192) return enqueue(add_norm_kernel<512, 2, BLOCKS>, grid, dim3(512), stream, p);
-    if (p.D <= 16384) return enqueue(add_norm_kernel<512, 4, BLOCKS>, grid, dim3(512), stream, p);
-    return enqueue(add_norm_long_kernel<BLOCKS>, grid, dim3(512), stream, p);
+    // One chunk of eight elements a thread where few rows leave most of the chip empty: a row is then one turn of memory.  With more, two or
+    // three, whichever leaves fewer lanes without work: wavefronts of a row wait for each other less.  us with 1 / 2 / 3 chunks: 1 x
+    // 2048 2.6 / 3.2 / 3.3, 816 x 2048 4.4 / 4.6 / 4.8, 777 x 4304 8.7 / 8.3 / 7.8, 6000 x 1152 11.6 / 11.7 / 11.1, 3264 x 8192 37.2 / 32.4 / 33.2, 13056 x 2048
+    // 32.7 / 31.4 / 31.9.
+    const int lanes = (p.D + 7) / 8;
+    auto threads_of = [&](int c) { return ((lanes + c - 1) / c + kWave - 1) / kWave * kWave; };
+    int chunks = 1;
+    if (p.M * threads_of(1) > 4096 * kWave) chunks = threads_of(3) * 3 < threads_of(2) * 2 ? 3 : 2;
+    if (lanes <= kWave) chunks = 1;
+    if (const char* forced = tuning_env("PHYAI_LAYER_ADD_NORM")) chunks = atoi(forced);
+    while (threads_of(chunks) > 1024) ++chunks;
+    const dim3 threads((uint32_t)threads_of(chunks));
+    if (lanes > 4096) return enqueue(add_norm_long_kernel<BLOCKS>, grid, dim3(512), stream, p);
+    switch (chunks) {
+        case 1: return enqueue(add_norm_kernel<1, BLOCKS>, grid, threads, stream, p);
+        case 2: return enqueue(add_norm_kernel<2, BLOCKS>, grid, threads, stream, p);
+        case 3: return enqueue(add_norm_kernel<3, BLOCKS>, grid, threads, stream, p);
+        default: return enqueue(add_norm_kernel<4, BLOCKS>, grid, threads, stream, p);
+    }
 }
 
 }  // namespace
