@@ -751,6 +751,7 @@ struct SplitShape {
     static constexpr int STAGE = 2 * 32 * Shape<DP>::ROW;
     static constexpr int OLD = DP + 4;                            // floats of a row of O in LDS
     static constexpr int WAVE_BYTES = STAGE > 32 * OLD * 4 ? STAGE : 32 * OLD * 4;
+    static constexpr int LDS = WAVES * (WAVE_BYTES + 512 + 256 + 128);   // and page numbers, maxima and sums, shares
 };
 template <int DP>
 constexpr int SPLIT_WAVES = DP == 256 ? 4 : 8;   // of a workgroup that has a CU to itself (64 dims: two fit)
@@ -821,14 +822,13 @@ __device__ __forceinline__ Row row_of_shared(const PagedAttention& p, const Tile
 }
 
 template <int DP, int TYPE, int MODE, int WAVES_OF>
-__global__ __launch_bounds__(WAVES_OF * 64, SPLIT_WAVES<DP> / WAVES_OF) void attend_split_kernel(const PagedAttention p, const Plan g, float* __restrict__ part) {
+__device__ __forceinline__ void attend_split(const PagedAttention& p, const Plan& g, float* __restrict__ part, uint8_t* lds, int tile, int kv_head, int z) {
     using S = Shape<DP>;
     using X = SplitShape<DP, WAVES_OF>;
-    __shared__ __align__(16) uint8_t lds[X::WAVES * X::WAVE_BYTES];
-    __shared__ uint32_t ids[X::WAVES][2][64];
-    __shared__ float ml[X::WAVES][32][2], weight[X::WAVES][32];
+    auto ids = reinterpret_cast<uint32_t (*)[2][64]>(lds + X::WAVES * X::WAVE_BYTES);
+    auto ml = reinterpret_cast<float (*)[32][2]>(lds + X::WAVES * (X::WAVE_BYTES + 512));
+    auto weight = reinterpret_cast<float (*)[32]>(lds + X::WAVES * (X::WAVE_BYTES + 512 + 256));
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int tile = blockIdx.x, kv_head = blockIdx.y, z = blockIdx.z + (MODE & MODE_MORE ? g.z_first : 0);
     // (the shared keys' splits come first)
     const bool shared = (MODE & MODE_MORE) != 0 && z < g.shared_splits;
     Tile t;
@@ -956,6 +956,12 @@ __global__ __launch_bounds__(WAVES_OF * 64, SPLIT_WAVES<DP> / WAVES_OF) void att
     }
 }
 
+template <int DP, int TYPE, int MODE, int WAVES_OF>
+__global__ __launch_bounds__(WAVES_OF * 64, SPLIT_WAVES<DP> / WAVES_OF) void attend_split_kernel(const PagedAttention p, const Plan g, float* __restrict__ part) {
+    __shared__ __align__(16) uint8_t lds[SplitShape<DP, WAVES_OF>::LDS];
+    attend_split<DP, TYPE, MODE, WAVES_OF>(p, g, part, lds, blockIdx.x, blockIdx.y, blockIdx.z);
+}
+
 // The workgroups' sums of a row joined, in the order of the splits; DP / 4 lanes a row, four value dims each.  Rows lie as in
 // out, so that nothing has to be looked up before the loads: the first splits' sums, all maxima and weights and the ends of
 // the sequences come in one turn of memory's latency (found by its tile, a row took three).
@@ -1025,14 +1031,14 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const PagedAttention p
 template <int DP>
 struct ManyShape {
     static constexpr int WAVES = 4, STEP = 64, MINE = STEP / WAVES, STAGE = 2 * STEP * Shape<DP>::ROW;
+    static constexpr int LDS = 2 * STAGE + WAVES * 512 + 128;   // and page numbers, words between wavefronts
 };
 
 // Which tile and key head a workgroup has.  Key heads change fastest: workgroups go round the eight chiplets, so each of those has few heads'
 // keys in its cache.  Causal rows see the more keys the later they are: the last ones first, and where two workgroups share a CU and
 // all run at once, the second half the other way round, so that a long one has a short one beside it.
 template <int DP>
-__device__ __forceinline__ bool place(const PagedAttention& p, int tiles, int& tile, int& kv_head) {
-    int at = blockIdx.y * gridDim.x + blockIdx.x;
+__device__ __forceinline__ bool place(const PagedAttention& p, int at, int tiles, int& tile, int& kv_head) {
     const int all = tiles * p.KV;
     if (at >= all) return false;
     if (p.causal && DP != 256 && all <= 512 && at >= 256) at = all - 1 - (at - 256);
@@ -1056,18 +1062,17 @@ struct Widening {
 };
 
 template <int DP, int TYPE, int MODE>
-__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(const PagedAttention p, const Plan g, float* __restrict__ part) {
+__device__ __forceinline__ void attend_many(const PagedAttention& p, const Plan& g, float* __restrict__ part, uint8_t* lds, int at, int z) {
     using S = Shape<DP>;
     using X = ManyShape<DP>;
-    __shared__ __align__(16) uint8_t lds[2 * X::STAGE];
-    __shared__ uint32_t ids[X::WAVES][2][64];
-    __shared__ int specials[X::WAVES], spans[X::WAVES][4];
+    auto ids = reinterpret_cast<uint32_t (*)[2][64]>(lds + 2 * X::STAGE);
+    auto specials = reinterpret_cast<int*>(lds + 2 * X::STAGE + X::WAVES * 512);
+    auto spans = reinterpret_cast<int (*)[4]>(lds + 2 * X::STAGE + X::WAVES * 512 + 64);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int z = MODE & MODE_MORE ? blockIdx.z + g.z_first : 0;
     const bool shared = (MODE & MODE_MORE) != 0 && z < g.shared_splits;
     int tile, kv_head;
     Tile t;
-    if (!place<DP>(p, shared ? g.shared_tiles : g.tiles, tile, kv_head)) return;   // (here and below: the same for the whole workgroup)
+    if (!place<DP>(p, at, shared ? g.shared_tiles : g.tiles, tile, kv_head)) return;   // (here and below: the same for the whole workgroup)
     if (shared ? !locate_shared(p, g, ROWS * X::WAVES, tile, t) : !locate<MODE>(p, g.group_size, ROWS * X::WAVES, tile, t)) return;
     const int row0 = t.row0 + wave * ROWS, row_last = t.rows - 1;
     Row row;
@@ -1208,29 +1213,49 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
         }
 }
 
+template <int DP, int TYPE, int MODE>
+__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(const PagedAttention p, const Plan g, float* __restrict__ part) {
+    __shared__ __align__(16) uint8_t lds[ManyShape<DP>::LDS];
+    attend_many<DP, TYPE, MODE>(p, g, part, lds, blockIdx.y * gridDim.x + blockIdx.x, blockIdx.z);
+}
+
+// The shared keys for many rows a workgroup, bound by arithmetic, and the sequences' own for few, bound by memory, in one launch: first
+// come the workgroups of the shared ones.
+template <int DP, int TYPE, int MODE>
+__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_both_kernel(const PagedAttention p, const Plan g, float* __restrict__ part) {
+    using X = SplitShape<DP, 4>;
+    __shared__ __align__(16) uint8_t lds[X::LDS > ManyShape<DP>::LDS ? X::LDS : ManyShape<DP>::LDS];
+    const int once = g.shared_tiles * p.KV, before = once * g.shared_splits;
+    int at = blockIdx.x;
+    if (at < before) {
+        const int z = at / once;
+        attend_many<DP, TYPE, MODE>(p, g, part, lds, at - z * once, z);
+    } else {
+        at -= before;
+        const int z = at / (g.tiles * p.KV), rest = at - z * (g.tiles * p.KV), kv_head = rest / g.tiles;
+        attend_split<DP, TYPE, MODE, 4>(p, g, part, lds, rest - kv_head * g.tiles, kv_head, g.shared_splits + z);
+    }
+}
+
 // ---- launches --------------------------------------------------------------------------------------------------------
 template <int DP, int TYPE, int MODE>
 hipError_t launch(const PagedAttention& p, const Plan& plan, hipStream_t stream) {
     float* part = static_cast<float*>(p.workspace);
     constexpr int WAVES = SPLIT_WAVES<DP>;
-    // splits first .. first + count - 1, with one kernel
-    auto run = [&](int many, int tiles, int first, int count) {
-        Plan g = plan;
-        g.z_first = first;
-        const dim3 grid(tiles, p.KV, count);
-        if (many) return enqueue(attend_many_kernel<DP, TYPE, MODE>, grid, dim3(256), stream, p, g, part);
-        if constexpr (MODE & MODE_MORE) {
-            if (plan.small) return enqueue(attend_split_kernel<DP, TYPE, MODE, WAVES / 2>, grid, dim3(WAVES * 32), stream, p, g, part);
-        }
-        return enqueue(attend_split_kernel<DP, TYPE, MODE, WAVES>, grid, dim3(WAVES * 64), stream, p, g, part);
-    };
-    const int own = plan.splits - plan.shared_splits;
-    hipError_t e;
-    if (plan.shared == 0 || plan.shared_many == plan.many)
-        e = run(plan.many, plan.tiles > plan.shared_tiles ? plan.tiles : plan.shared_tiles, 0, plan.splits);
-    else {
-        e = run(plan.shared_many, plan.shared_tiles, 0, plan.shared_splits);
-        if (e == hipSuccess) e = run(plan.many, plan.tiles, plan.shared_splits, own);
+    const dim3 grid(plan.tiles > plan.shared_tiles ? plan.tiles : plan.shared_tiles, p.KV, plan.splits);
+    hipError_t e = hipSuccess;
+    bool done = false;
+    if constexpr (MODE & MODE_MORE) {
+        done = true;
+        if (plan.shared > 0 && plan.shared_many && !plan.many) {
+            const int64_t all = ((int64_t)plan.shared_tiles * plan.shared_splits + (int64_t)plan.tiles * (plan.splits - plan.shared_splits)) * p.KV;
+            e = enqueue(attend_both_kernel<DP, TYPE, MODE>, dim3((uint32_t)all), dim3(256), stream, p, plan, part);
+        } else if (!plan.many && plan.small) e = enqueue(attend_split_kernel<DP, TYPE, MODE, WAVES / 2>, grid, dim3(WAVES * 32), stream, p, plan, part);
+        else done = false;
+    }
+    if (!done) {
+        e = plan.many ? enqueue(attend_many_kernel<DP, TYPE, MODE>, grid, dim3(256), stream, p, plan, part)
+                      : enqueue(attend_split_kernel<DP, TYPE, MODE, WAVES>, grid, dim3(WAVES * 64), stream, p, plan, part);
     }
     if (e != hipSuccess || plan.splits == 1) return e;
     return enqueue(attend_join_kernel<DP, TYPE>, dim3((unsigned)(((int64_t)p.T * p.H + 1024 / DP - 1) / (1024 / DP))), dim3(256), stream, p, plan, (const float*)part);

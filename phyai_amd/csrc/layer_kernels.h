@@ -99,7 +99,6 @@ struct AttentionPlan {
     int shared, shared_tiles, shared_splits, shared_many;
     AttentionDivision shared_workers;
     int small;                // few rows: half the wavefronts a workgroup
-    int z_first;              // of a launch: its first split
 };
 size_t paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int64_t max_kv, int64_t shared, int64_t window,
                                        bool more);

@@ -63,7 +63,7 @@ double together(const Part* parts, int count, int64_t at_once) {
 }
 
 // Calls that are more than plain ones: few rows a workgroup with all its wavefronts or half of them (two of those a CU), or many rows, each
-// with the keys split or not, and shared keys in one launch with the sequences' own (both few rows) or in one before it (many rows).  The
+// with the keys split or not, and shared keys beside the sequences' own, for few rows or many.  The
 // choice with the least expected time; a workgroup takes its start (9 us for few rows, 12 for many: most of it instructions that a cold
 // cache does not have, and three turns of memory) and its blocks of 32 keys a wavefront, or steps of 64, at what they take where the
 // CU is full; sums to be joined take 4.5.  Measured, few rows with all wavefronts / half of them / many rows, best number of splits each, 8 bits and
@@ -89,7 +89,8 @@ Plan make_plan_more(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int6
             const double step = DP == 256 ? 3.5 : DP == 128 ? (tiles * s <= 256 ? 1.9 : 2.5) : tiles * s <= 256 ? 1.6 : 2.2;
             return Part{tiles * s, 12.0 + (double)ceiling(keys, 64 * s) * step};
         };
-        const int64_t at_once_few = DP == 64 ? 512 : 256, at_once_many = DP == 256 ? 256 : 512;
+        const int64_t at_once_many = DP == 256 ? 256 : 512, at_once_mixed = DP == 64 ? 768 : at_once_many;
+        auto at_once_few = [&](int half) -> int64_t { return DP == 64 ? (half ? 768 : 512) : half ? 512 : 256; };
         auto moved = [&](int s) { return s > 1 ? join + (double)(T * H) * DP * s / 1.5e6 : 0.0; };   // (the sums of all splits)
         double best = 1e30;
         auto take = [&](double t, int m, int s, int h, int sm, int ss) {
@@ -100,21 +101,21 @@ Plan make_plan_more(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int6
         for (int s = 1; s <= MAX_SPLITS; s = s < 8 ? s + 1 : s + s / 4) {
             for (int h = 0; h < 2; ++h) {
                 const Part p = few_rows(few, seen, s, h);
-                if (s == 1 || seen >= 32 * (h ? waves / 2 : waves) * (s - 1)) take(together(&p, 1, at_once_few << h) + moved(s), 0, s, h, 0, 0);
+                if (s == 1 || seen >= 32 * (h ? waves / 2 : waves) * (s - 1)) take(together(&p, 1, at_once_few(h)) + moved(s), 0, s, h, 0, 0);
             }
             const Part p = many_rows(wide, seen, s);
             if (s == 1 || seen >= 128 * s) take(together(&p, 1, at_once_many) + moved(s), 1, s, 0, 0, 0);
         }
-        if (shared > 0 && B > 1) {
+        if (shared > 0 && B > 1 && few < (1 << 24)) {   // (beyond, everything is full as it is)
             const int64_t own = max_kv > shared ? max_kv - shared : 1, once = ceiling(T * group, ROWS) * KV, once_wide = ceiling(T * group, 128) * KV;
             for (int ss = 1; ss <= MAX_SPLITS / 2; ss *= 2)
                 for (int s = 1; s <= 4; s *= 2)
                     for (int h = 0; h < 2; ++h) {
                         const Part both[2] = {few_rows(once, shared, ss, h), few_rows(few, own, s, h)};
                         const Part before = many_rows(once_wide, shared, ss), wide_own = many_rows(wide, own, s);
-                        const Part all_many[2] = {before, wide_own};
-                        take(together(both, 2, at_once_few << h) + moved(ss + s), 0, s, h, 0, ss);
-                        if (shared >= 128 * ss) take(together(&before, 1, at_once_many) + together(both + 1, 1, at_once_few << h) + moved(ss + s), 0, s, h, 1, ss);
+                        const Part all_many[2] = {before, wide_own}, mixed[2] = {before, both[1]};
+                        take(together(both, 2, at_once_few(h)) + moved(ss + s), 0, s, h, 0, ss);
+                        if (shared >= 128 * ss && h == (DP != 256)) take(together(mixed, 2, at_once_mixed) + moved(ss + s), 0, s, h, 1, ss);
                         if (shared >= 128 * ss && h == 0) take(together(all_many, 2, at_once_many) + moved(ss + s), 1, s, 0, 1, ss);
                     }
         }
@@ -122,11 +123,11 @@ Plan make_plan_more(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int6
     if (const char* forced = tuning_env("PHYAI_LAYER_ATTEND_MORE")) sscanf(forced, "%d %d %d %d %d", &many, &splits, &small, &shared_many, &shared_splits);
     auto held = [](int v, int most) { return v < 1 ? 1 : v < most ? v : most; };
     r.many = many != 0;
-    r.small = small != 0;
+    r.small = shared > 0 && shared_splits > 0 && shared_many != 0 && many == 0 ? DP != 256 : small != 0;   // (in one launch: four wavefronts)
     r.tiles = (int)tiles_bound(T, B, group, r.many ? 128 : ROWS);
     if (shared > 0 && shared_splits > 0) {
         r.shared = (int)shared;
-        r.shared_many = shared_many != 0;
+        r.shared_many = shared_many != 0 || many != 0;   // (nobody has many rows of his own and few with the others)
         r.shared_tiles = (int)((T * group + (r.shared_many ? 128 : ROWS) - 1) / (r.shared_many ? 128 : ROWS));
         r.shared_splits = held(shared_splits, MAX_SPLITS / 2);
         splits = held(splits, MAX_SPLITS / 2);

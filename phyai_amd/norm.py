@@ -56,6 +56,13 @@ class RMSNorm(nn.Module):
         xq, xs = ops.rmsnorm_fp8(x, self.weight, self.variance_epsilon, gemma=self._gemma)
         return ActivationView(xq, xs, Granularity.PER_CHANNEL)
 
+    def forward_add_fp8(self, x: torch.Tensor, residual: torch.Tensor, *, per_block: bool = False,
+                        out: torch.Tensor | None = None) -> tuple[ActivationView, torch.Tensor]:
+        """The residual's addition, the norm of the sum and its quantization in one kernel: ``(view, x + residual)``.  The view has
+        one scale per token or, with ``per_block``, one per 128 elements of it, as layers of ``fp8_block_128_128`` take them."""
+        xq, xs, total = ops.add_rmsnorm_fp8(x, residual, self.weight, self.variance_epsilon, gemma=self._gemma, per_block=per_block, out=out)
+        return ActivationView(xq, xs, Granularity.BLOCK if per_block else Granularity.PER_CHANNEL), total
+
     def extra_repr(self) -> str:
         return f"{self.hidden_size}, eps={self.variance_epsilon}, backend={self.backend!r}"
 
