@@ -38,6 +38,7 @@ enum Mode : int {
     MODE_MORE = 1,   // prompts that causal rows see the whole of, shared leading keys
     MODE_FP8 = 2,    // pages in 8 bits
     MODE_CAP = 4,    // scores capped by a tanh
+    MODE_WIDE = 8,   // the same with a cap that scores may be far below (above 256)
 };
 
 constexpr int ROWS = 32;               // rows of a wavefront's tile
@@ -534,12 +535,28 @@ __device__ __forceinline__ void raise_maximum(State<DP>& st, float mx) {
 // power over- or underflows.  Kept is -1 / (e + 1), from which the score (less a maximum) is one multiply-add: times 2 cap log2(e), and cap log2(e)
 // left out, which all scores have in common.  Off by some 2^-22 of cap in all, which is what the score's own rounding is.
 struct Cap {
-    float by;
+    float by, most;
 };
 template <int N>
 __device__ __forceinline__ void cap_some(v16f& s, int first, Cap c) {
 #pragma unroll
     for (int i = first; i < first + N; ++i) s[i] = -__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[i] * c.by) + 1.0f);
+}
+// That rounding is 2^-22 of the cap also for scores far below it, which large caps are there to leave alone.  So for those: with y = s by,
+// by = scale / cap, s times the first terms of tanh(y) / y = 1 - y^2 / 3 + ..., the one left out 6e-8 of it at the border, and beyond
+// cap / scale times 1 - 2 / (e^2y + 1).  The result is a score as it was.  Three times the instructions: only in kernels of its own.
+__device__ __forceinline__ void cap_wide(v16f& s, Cap c) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float y = s[i] * c.by, u = y * y;
+        float f = __builtin_fmaf(u, -1382.0f / 155925, 62.0f / 2835);
+        f = __builtin_fmaf(u, f, -17.0f / 315);
+        f = __builtin_fmaf(u, f, 2.0f / 15);
+        f = __builtin_fmaf(u, f, -1.0f / 3);
+        const float small = __builtin_fmaf(s[i] * u, f, s[i]);
+        const float t = 1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(__builtin_fabsf(y) * 2.8853900817779268f) + 1.0f);
+        s[i] = __builtin_fabsf(y) > 0.4f ? __builtin_copysignf(t * c.most, s[i]) : small;
+    }
 }
 // Scores to probabilities, as the second product's operand.  The sum is of the rounded ones, those that the product uses:
 // their common error cancels.
@@ -625,6 +642,10 @@ __device__ __forceinline__ void attend_steps(State<DP>& st, const v4i* qf, int s
             }
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (MODE & MODE_CAP) cap_some<16>(s[NB - 1], 0, cap);
+            if constexpr ((MODE & MODE_WIDE) != 0) {
+#pragma unroll
+                for (int n = 0; n < NB; ++n) cap_wide(s[n], cap);
+            }
             const int j0 = step * (32 * NB);
             if (j0 < whole_lo || j0 + 32 * NB > whole_hi) {
 #pragma unroll
@@ -851,7 +872,7 @@ __device__ __forceinline__ void attend_split(const PagedAttention& p, const Plan
     const int begin = b0 + me * each + (me < rest ? me : rest), end = begin + each + (me < rest ? 1 : 0);
     const Pool pool = make_pool<DP, TYPE, MODE>(p, t, kv_head, g);
     const float c = MODE & MODE_CAP ? 2.0f * p.cap : p.scale * 1.4426950408889634f;
-    const Cap cap = {p.cap_by};
+    const Cap cap = {p.cap_by, p.cap_most};
 
     State<DP> st;
     st.m = kNone;
@@ -1109,7 +1130,7 @@ __device__ __forceinline__ void attend_many(const PagedAttention& p, const Plan&
     }
     const Pool pool = make_pool<DP, TYPE, MODE>(p, t, kv_head, g);
     const float c = MODE & MODE_CAP ? 2.0f * p.cap : p.scale * 1.4426950408889634f;
-    const Cap cap = {p.cap_by};
+    const Cap cap = {p.cap_by, p.cap_most};
     const uint32_t base = (uint32_t)(uintptr_t)lds;
     using Feed = Feeder<DP, X::STEP, X::MINE>;
     Feed feed(pool, begin, wave * X::MINE, ids[wave][0]);
@@ -1245,7 +1266,7 @@ hipError_t launch(const PagedAttention& p, const Plan& plan, hipStream_t stream)
     const dim3 grid(plan.tiles > plan.shared_tiles ? plan.tiles : plan.shared_tiles, p.KV, plan.splits);
     hipError_t e = hipSuccess;
     bool done = false;
-    if constexpr (MODE & MODE_MORE) {
+    if constexpr ((MODE & MODE_MORE) != 0 && (MODE & MODE_WIDE) == 0) {
         done = true;
         if (plan.shared > 0 && plan.shared_many && !plan.many) {
             const int64_t all = ((int64_t)plan.shared_tiles * plan.shared_splits + (int64_t)plan.tiles * (plan.splits - plan.shared_splits)) * p.KV;
@@ -1253,7 +1274,8 @@ hipError_t launch(const PagedAttention& p, const Plan& plan, hipStream_t stream)
         } else if (!plan.many && plan.small) e = enqueue(attend_split_kernel<DP, TYPE, MODE, WAVES / 2>, grid, dim3(WAVES * 32), stream, p, plan, part);
         else done = false;
     }
-    if (!done) {
+    if constexpr (MODE & MODE_WIDE) e = enqueue(attend_split_kernel<DP, TYPE, MODE, WAVES>, grid, dim3(WAVES * 64), stream, p, plan, part);
+    else if (!done) {
         e = plan.many ? enqueue(attend_many_kernel<DP, TYPE, MODE>, grid, dim3(256), stream, p, plan, part)
                       : enqueue(attend_split_kernel<DP, TYPE, MODE, WAVES>, grid, dim3(WAVES * 64), stream, p, plan, part);
     }

@@ -5,6 +5,7 @@ namespace phyai {
 
 hipError_t launch_attention_bf16(const PagedAttention& p, const AttentionPlan& plan, hipStream_t stream) {
     constexpr int MODE = MODE_MORE;
+    if (p.cap > kWideCap) return launch_d<HEAD_BF16, MODE | MODE_WIDE>(p, plan, stream);
     return p.cap > 0.f ? launch_d<HEAD_BF16, MODE | MODE_CAP>(p, plan, stream) : launch_d<HEAD_BF16, MODE>(p, plan, stream);
 }
 

@@ -87,6 +87,7 @@ int64_t whole_pages(int64_t shared, int64_t page_size, int64_t table_width) {
 }
 size_t attention_workspace(int64_t T, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_kv, int64_t shared, int64_t window, bool more) {
     if (T <= 0 || batch <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || heads % kv_heads != 0 || T >= kMost || T * heads >= kMost) return 0;
+    window = window < 0 ? 0 : window > kMost - 1 ? kMost - 1 : window;   // (as the call takes it)
     const size_t n = phyai::paged_attention_workspace_bytes(T, batch, heads, kv_heads, head_dim, max_kv, shared, window, more);
     return n == 0 ? 0 : PHYAI_FP8_WORKSPACE_HEADER_BYTES + n;
 }
@@ -233,7 +234,11 @@ int attention(const char* fn, const void* q, int64_t q_token_stride, int64_t q_h
         }
         p.prefix_lens = causal ? more->prefix_lens : nullptr;
         p.cap = more->softcap * 1.4426950408889634f;
-        p.cap_by = more->softcap > 0.f ? (float)(2.0 * scale * 1.4426950408889634 / more->softcap) : 0.f;
+        if (more->softcap > 0.f) {
+            const double most = (double)more->softcap / scale;
+            p.cap_by = (float)(p.cap > phyai::kWideCap ? 1.0 / most : 2.0 * 1.4426950408889634 / most);
+            p.cap_most = most < 3.4028234663852886e38 ? (float)most : 3.40282347e38f;
+        }
         p.more = 1;
         p.shared = (int)shared;
     }
@@ -364,8 +369,8 @@ int phyai_layer_cache_read(const void* k_pages, const void* v_pages, const int64
         return fail(PHYAI_FP8_EINVAL, "%s: null pointer", fn);
     if (!aligned(k_pages, 16) || !aligned(v_pages, 16) || !aligned(k_out, 16) || !aligned(v_out, 16) || !aligned(slots, 8))
         return fail(PHYAI_FP8_EINVAL, "%s: operands must be 16-byte aligned (slots 8-byte)", fn);
-    if (T >= kMost || T * kv_heads >= kMost || T * kv_heads * (head_dim / 16) >= kMost * 64)
-        return fail(PHYAI_FP8_EUNSUPPORTED, "%s: T * kv_heads must be below 2^31", fn);
+    if (T >= kMost || T * kv_heads >= kMost || T * kv_heads * (head_dim / 16) >= kMost - 256)   // (threads for K and V: less than 2^32)
+        return fail(PHYAI_FP8_EUNSUPPORTED, "%s: T * kv_heads * head_dim / 16 must be below 2^31 - 256", fn);
     if (page_size >= kMost || (n_pages > 0 && page_size > (kMost - 1) / n_pages))
         return fail(PHYAI_FP8_EUNSUPPORTED, "%s: a cache of 2^31 tokens or more", fn);
     phyai::CacheRead p = {};
@@ -395,7 +400,9 @@ int phyai_layer_add_rmsnorm_quant(const void* x, int64_t ldx, const void* residu
     if (ldx < D || ldr < D || ldt < D || ldx % 8 != 0 || ldr % 8 != 0 || ldt % 8 != 0)
         return fail(PHYAI_FP8_EINVAL, "%s: row strides must be at least D and multiples of 8", fn);
     if (xs_row <= 0 || xs_block < 0) return fail(PHYAI_FP8_EINVAL, "%s: strides of x_scale must be positive (xs_block 0: one scale a row)", fn);
-    if (M >= kMost || D >= kMost / 4) return fail(PHYAI_FP8_EUNSUPPORTED, "%s: M must be below 2^31 and D below 2^29", fn);
+    // (a row has a workgroup of D / 8 threads, rounded up to wavefronts, at most 1024, and a launch less than 2^32 threads)
+    if (M >= kMost || D >= kMost / 4 || M * (D < 8192 ? (D / 8 + 63) / 64 * 64 : 1024) >= 2 * kMost)
+        return fail(PHYAI_FP8_EUNSUPPORTED, "%s: M=%lld rows of D=%lld are too many (2^22 of 8192 and more, 2^26 of 512 and less)", fn, (long long)M, (long long)D);
     // (in place is fine: a thread reads what it writes, before; anywhere else rows would be written that others still read)
     for (const void* in : {x, residual}) {
         const int64_t ld = in == x ? ldx : ldr;

@@ -83,10 +83,12 @@ struct PagedAttention {
     const uint8_t *k_scales, *v_scales;    // of pages in 8 bits: bytes b of powers 2^(b - 127)
     int64_t scale_stride[3];  // between pages, tokens of a page, heads
     const int32_t* prefix_lens;            // [B]: keys that a causal row sees whatever its position
-    float cap, cap_by;        // scores become cap tanh: the cap times log2(e); 2 log2(e) scale / cap
+    float cap, cap_by;        // scores become cap tanh: the cap times log2(e); 2 log2(e) scale / cap (above kWideCap: scale / cap)
+    float cap_most;           // cap / scale
     int more;                 // not a plain call (also where everything below is zero)
     int shared;               // leading keys that lie in the same pages for all sequences, as the caller says
 };
+constexpr float kWideCap = 256.0f * 1.4426950408889634f;   // (as cap above)
 // Division by a number known on the host: its magic number and shift (magic 0: by one).
 struct AttentionDivision {
     uint32_t magic, shift;

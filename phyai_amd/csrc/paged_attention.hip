@@ -71,8 +71,9 @@ double together(const Part* parts, int count, int64_t at_once) {
 // 1000 114 / 94; 256 tokens of 1024 20 / 27 / 31, 512 of 512 26 / 19 / 26, 512 of 4096 79 / 71 / 63, 2048 of 8192 625 / 567 / 360; 1000 of 1000 of 64
 // dims 39 / 29 / 38; 16 x 816 of 816 of 256 dims in 16 bits 149 / 124 / 103.  64 tokens behind 8192 shared keys and up to 512 of their
 // own: few and few rows 67, many and few 53, nothing shared 180; 16 of them 28 and 35.
+// (few_only: kernels for caps above kWideCap are there for few rows with all wavefronts.)
 // PHYAI_LAYER_ATTEND_MORE = "many splits small shared_many shared_splits" (shared_splits 0: nothing is shared) forces one.
-Plan make_plan_more(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int64_t max_kv, int64_t page_size, int64_t shared, int64_t window) {
+Plan make_plan_more(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int64_t max_kv, int64_t page_size, int64_t shared, int64_t window, bool few_only) {
     Plan r = make_plan(T, B, H, KV, D, max_kv, page_size);
     const int64_t group = H / KV;
     const int DP = padded_dim(D), waves = DP == 256 ? 4 : 8;
@@ -106,7 +107,7 @@ Plan make_plan_more(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int6
             const Part p = many_rows(wide, seen, s);
             if (s == 1 || seen >= 128 * s) take(together(&p, 1, at_once_many) + moved(s), 1, s, 0, 0, 0);
         }
-        if (shared > 0 && B > 1 && few < (1 << 24)) {   // (beyond, everything is full as it is)
+        if (shared > 0 && B > 1 && few < (1 << 20)) {   // (beyond, a launch of all of them could have 2^32 threads)
             const int64_t own = max_kv > shared ? max_kv - shared : 1, once = ceiling(T * group, ROWS) * KV, once_wide = ceiling(T * group, 128) * KV;
             for (int ss = 1; ss <= MAX_SPLITS / 2; ss *= 2)
                 for (int s = 1; s <= 4; s *= 2)
@@ -121,6 +122,7 @@ Plan make_plan_more(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int6
         }
     }
     if (const char* forced = tuning_env("PHYAI_LAYER_ATTEND_MORE")) sscanf(forced, "%d %d %d %d %d", &many, &splits, &small, &shared_many, &shared_splits);
+    if (few_only) many = small = shared_many = 0;   // (as many sums, so no other workspace)
     auto held = [](int v, int most) { return v < 1 ? 1 : v < most ? v : most; };
     r.many = many != 0;
     r.small = shared > 0 && shared_splits > 0 && shared_many != 0 && many == 0 ? DP != 256 : small != 0;   // (in one launch: four wavefronts)
@@ -143,7 +145,7 @@ Plan make_plan_more(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int6
 
 size_t paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int64_t max_kv, int64_t shared, int64_t window, bool more) {
     if (T <= 0 || B <= 0) return 0;
-    const Plan plan = more ? make_plan_more(T, B, H, KV, D, max_kv, 1, shared, window) : make_plan(T, B, H, KV, D, max_kv, 1);
+    const Plan plan = more ? make_plan_more(T, B, H, KV, D, max_kv, 1, shared, window, false) : make_plan(T, B, H, KV, D, max_kv, 1);
     if (plan.splits == 1) return 0;
     return (size_t)plan.splits * T * H * (padded_dim(D) + 2) * sizeof(float);
 }
@@ -155,7 +157,7 @@ hipError_t launch_paged_attention(const PagedAttention& p, hipStream_t stream) {
         const Plan plan = make_plan(p.T, p.B, p.H, p.KV, p.D, max_kv, p.page_size);
         return bf16 ? launch_d<HEAD_BF16, 0>(p, plan, stream) : launch_d<HEAD_F16, 0>(p, plan, stream);
     }
-    const Plan plan = make_plan_more(p.T, p.B, p.H, p.KV, p.D, max_kv, p.page_size, p.shared, p.window);
+    const Plan plan = make_plan_more(p.T, p.B, p.H, p.KV, p.D, max_kv, p.page_size, p.shared, p.window, p.cap > kWideCap);
     if (p.k_scales != nullptr) return bf16 ? launch_attention_bf16_fp8(p, plan, stream) : launch_attention_f16_fp8(p, plan, stream);
     return bf16 ? launch_attention_bf16(p, plan, stream) : launch_attention_f16(p, plan, stream);
 }

@@ -1082,6 +1082,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
     Returns ``[T, heads, head_dim]``; a row that sees nothing is zero, one whose scores are all -inf is NaN, rows outside every
     sequence are left as they were (of a fresh result: undefined), and rows that see keys of a page that does not exist are NaN."""
+    import ctypes
+
     op = "paged_attention"
     got = _native().paged_attention(q, k_pages, v_pages, page_table, q_offsets, kv_lens, scale, causal, window, out, k_scales, v_scales, softcap,
                                     prefix_lens, shared_prefix)
@@ -1116,8 +1118,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         raise _err(op, f"scale must be a positive number, got {scale}")
     if window is not None and window < 1:
         raise _err(op, f"window must be at least 1, got {window}")
-    if softcap is not None and not 0.0 < float(softcap) < float("inf"):
-        raise _err(op, f"softcap must be a positive number, got {softcap}")
+    if softcap is not None and not 0.0 < ctypes.c_float(softcap).value < float("inf"):
+        raise _err(op, f"softcap must be a positive number of fp32, got {softcap}")
     if shared_prefix < 0:
         raise _err(op, f"shared_prefix must not be negative, got {shared_prefix}")
     prompts = _vector(op, "prefix_lens", prefix_lens, torch.int32, B, dev) if prefix_lens is not None else None
@@ -1127,8 +1129,6 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         raise _err(op, f"out must be a contiguous {dtype} tensor of shape {(T, H, D)} on {dev}, 16-byte aligned")
     if T == 0 or B == 0:
         return out
-    import ctypes
-
     lib = _lib.load()
     if fp8 or softcap is not None or prompts is not None or shared_prefix:
         options = _lib.AttentionOptions(prefix_lens=prompts, shared_prefix=int(shared_prefix), softcap=float(softcap or 0.0))

@@ -448,6 +448,32 @@ def test_capped_scores_of_any_size(dev):
     within(attend(dev, tensors, kw), want, bound + 2.0 ** -7, "a high cap")
 
 
+WIDE = [
+    ([3, 40], [200, 90], 16, 4, 1, 64, True, None, None),
+    ([300], [700], 16, 8, 2, 64, True, 130, [500]),
+    ([1] * 9, [300 + 7 * i for i in range(9)], 16, 4, 2, 64, True, None, None),
+    ([5, 0, 33], [70, 20, 100], 8, 2, 2, 80, False, None, None),
+    ([20], [150], 16, 3, 1, 256, True, None, [60]),
+]
+
+
+@pytest.mark.parametrize("case", WIDE, ids=name_of)
+@pytest.mark.parametrize("cap", [257.0, 3e4, 1e6, 1e20, 2.3e38])
+@pytest.mark.parametrize("dtype,bits", [(torch.bfloat16, 8), (torch.float16, 16), (torch.bfloat16, 16), (torch.float16, 8)])
+def test_caps_that_scores_are_far_below(dev, case, cap, dtype, bits):
+    """Scores far below a cap are as exact as without one, those about it as its tanh, whatever their number.  The first token's are eight times
+    as large: 64 products and sums of at most 2^-23 / 2 of sum_d |q_d k_d| scale < 2^9 move a probability by 2^-8 at most, and the tanh by less
+    than 2^-10; the oracle's bound is at least 2^-9 of the same values, so three times that holds both."""
+    d = case[5]
+    tensors, kw = attend_case((*case, cap), dtype, bits, q_scale=8.0 if d == 64 else 1.0, shared=16 * 16 if len(case[0]) == 9 else 0)
+    if d == 64:
+        tensors["q"][0] *= 8
+    want, bound = oracle.attention(*tensors.values(), **kw)
+    within(attend(dev, tensors, kw), want, 3 * bound, f"cap {cap}")
+    if len(case[0]) == 9:
+        within(attend(dev, tensors, kw | dict(shared_prefix=256)), want, 3 * bound, f"cap {cap}, shared")
+
+
 def test_plain_calls_are_the_same_bits(dev):
     """What asks for nothing more is the plain kernel; a prompt of nothing and a prefix of nothing change no bit either."""
     tensors, kw = attend_case(([5, 1, 40], [60, 33, 90], 16, 4, 2, 128, True, None, None, None), torch.bfloat16, 16)

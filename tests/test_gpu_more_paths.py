@@ -231,7 +231,7 @@ def test_refused_calls(dev):
     offsets, lens = torch.tensor([0, 1, 2], dtype=torch.int32, device=dev), torch.tensor([5, 6], dtype=torch.int32, device=dev)
     good = dict(k_pages=k, v_pages=v, k_scales=ks, v_scales=vs)
     ops().paged_attention(q, page_table=table, q_offsets=offsets, kv_lens=lens, **good)
-    for bad in (dict(k_scales=None), dict(k_scales=None, v_scales=None), dict(k_pages=bf, v_pages=bf), dict(softcap=0.0), dict(softcap=-1.0), dict(softcap=float("nan")),
+    for bad in (dict(k_scales=None), dict(k_scales=None, v_scales=None), dict(k_pages=bf, v_pages=bf), dict(softcap=0.0), dict(softcap=-1.0), dict(softcap=float("nan")), dict(softcap=1e-60), dict(softcap=1e39),
                 dict(softcap=float("inf")), dict(shared_prefix=-1), dict(prefix_lens=lens.long()), dict(prefix_lens=lens[:1]), dict(prefix_lens=lens.cpu()),
                 dict(k_scales=raw(ks).contiguous())):
         with pytest.raises(RuntimeError):

@@ -48,6 +48,24 @@ def test_add_rmsnorm_quant(lib):
     assert b"overlaps" in lib.phyai_layer_last_error() or lib.phyai_layer_last_error()
 
 
+def test_calls_of_more_threads_than_a_launch_has(lib):
+    raw, p = buffer()
+    norm = [p, 64, p + 4096, 64, p, 0, 1e-6, 2 ** 26, 64, p + 8192, 64, p + 16384, p + 32768, 1, 1, None]
+    assert lib.phyai_layer_add_rmsnorm_quant(*norm) == EUNSUPPORTED
+    norm[7], norm[8] = 2 ** 22, 8192
+    norm[1] = norm[3] = norm[10] = 8192
+    assert lib.phyai_layer_add_rmsnorm_quant(*norm) == EUNSUPPORTED
+    s, b = three(64, 64, 64), three(4, 1, 1)
+    assert lib.phyai_layer_cache_read(p, p, s, s, p, p, b, b, p, 4, 4, p, p, 2 ** 26, 1, 512, 0, None) == EUNSUPPORTED
+
+
+def test_a_workspace_is_that_of_the_window_that_a_call_takes(lib):
+    need = lib.phyai_layer_paged_attention_more_workspace_bytes
+    for window in (2 ** 31, 2 ** 40, 2 ** 63 - 1):
+        for width in (400, 2 ** 30):
+            assert need(4, 2, 1, 1, 64, 16, width, 0, window) == need(4, 2, 1, 1, 64, 16, width, 0, 2 ** 31 - 1) > 0
+
+
 def test_head_rope_fp8(lib):
     raw, p = buffer()
     s, b = three(64, 64, 64), three(4, 1, 1)
