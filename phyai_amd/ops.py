@@ -840,8 +840,8 @@ def add_rmsnorm_fp8(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tenso
     got = _native().add_rmsnorm_fp8(x, residual, weight, eps, gemma, per_block, out)
     if got is not None:
         return got
-    x2 = _as_rows(op, x, "x", torch.bfloat16)
-    r2 = _as_rows(op, residual, "residual", torch.bfloat16)
+    x2, r2 = (t if t.shape[0] < 2 or t.stride(0) >= t.shape[1] else t.contiguous()   # (rows that are one, expanded: copied)
+              for t in (_as_rows(op, x, "x", torch.bfloat16), _as_rows(op, residual, "residual", torch.bfloat16)))
     if residual.shape != x.shape:
         raise _err(op, f"residual must have x's shape {tuple(x.shape)}, got {tuple(residual.shape)}")
     M, D = x2.shape

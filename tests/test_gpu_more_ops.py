@@ -83,6 +83,13 @@ def test_add_rmsnorm_in_place_and_strided(dev, d):
         again = ops().add_rmsnorm_fp8(*pair, weight, gemma=True, out=pair[which])
         assert again[2].data_ptr() == pair[which].data_ptr()
         assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(again, want))
+    same = x.contiguous()
+    for one in (ops().add_rmsnorm_fp8(same[:1].expand(m, d), residual, weight, gemma=True), ops().add_rmsnorm_fp8(residual, same[:1].expand(m, d), weight, gemma=True)):
+        repeated = ops().add_rmsnorm_fp8(same[:1].repeat(m, 1), residual.contiguous(), weight, gemma=True)
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(one, repeated))
+    twice = same.clone()
+    both = ops().add_rmsnorm_fp8(twice, twice, weight, gemma=True, out=twice)
+    assert torch.equal(both[2], same + same)
     three = ops().add_rmsnorm_fp8(x.contiguous().view(1, m, d), residual.contiguous().view(1, m, d), weight, gemma=True)
     assert three[0].shape == (1, m, d) and three[1].shape == (1, m, -(-d // 128)) and torch.equal(three[1][0], want[1])
 
@@ -415,6 +422,46 @@ def test_pages_that_do_not_exist(dev, shared):
             tensors["page_table"][1, 5] = bad                     # keys 80 .. 89 of the second sequence, whose tokens stand at 87 .. 89
             out = attend(dev, tensors, kw | dict(shared_prefix=shared)).cpu().double()
             assert out[1:4].isnan().all() and bool(((out - want).abs() <= bound)[[0, 4, 5]].all())
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("case,shared", [(([1] * 9, [70 + i for i in range(9)], 16, 4, 1, 128, True, None, None, 30.0), 64), (([260, 40], [300, 200], 16, 4, 2, 64, True, None, [50, 0], None), 0),
+                                         (([1, 2], [900, 1000], 16, 4, 2, 256, True, None, None, None), 0)])
+def test_results_in_the_place_of_the_queries(dev, case, shared, bits):
+    tensors, kw = attend_case(case, torch.bfloat16, bits, shared=shared)
+    want = attend(dev, tensors, kw | dict(shared_prefix=shared))
+    q = tensors["q"].to(dev)
+    again = attend(dev, tensors | dict(q=q), kw | dict(shared_prefix=shared), out=q)
+    assert again.data_ptr() == q.data_ptr() and torch.equal(again, want)
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_one_table_row_for_a_whole_batch(dev, bits):
+    """Sequences that have everything in common, their table one row expanded, queries a slice of a fused projection, and a prefix
+    length given as a numpy integer."""
+    import numpy
+
+    tensors, kw = attend_case(([2] * 5, [96] * 5, 16, 4, 2, 128, True, None, None, None), torch.bfloat16, bits, shared=96)
+    table = tensors["page_table"][:1].to(dev)
+    want = attend(dev, tensors | dict(page_table=table.repeat(5, 1)), kw | dict(shared_prefix=96))
+    wide = torch.zeros(10, 8, 128, dtype=torch.bfloat16, device=dev)
+    wide[:, 2:6] = tensors["q"].to(dev)
+    got = attend(dev, tensors | dict(page_table=table.expand(5, -1), q=wide[:, 2:6]), kw | dict(shared_prefix=numpy.int64(96)))
+    assert torch.equal(got, want)
+    expected, bound = oracle.attention(*(tensors | dict(page_table=tensors["page_table"][:1].repeat(5, 1))).values(), **kw)
+    within(got, expected, bound)
+
+
+def test_a_cache_without_pages(dev):
+    """Nothing is there: rows without keys are zero, those that should see some NaN, slots are all outside."""
+    pool = ops().fp8_cache(0, 16, 2, 64, device=dev)
+    k, v = ops().read_fp8_cache(*pool, torch.tensor([0, -1, 5], device=dev))
+    assert k.shape == (3, 2, 64) and not k.any() and not v.any()
+    q = seeded((3, 4, 64), 1).to(dev)
+    offsets, lens = (torch.tensor(x, dtype=torch.int32, device=dev) for x in ([0, 1, 3], [0, 5]))
+    table = torch.full((2, 1), -1, dtype=torch.int32, device=dev)
+    out = ops().paged_attention(q, pool[0], pool[1], table, offsets, lens, k_scales=pool[2], v_scales=pool[3])
+    assert not out[0].any() and bool(out[1:].isnan().all())
 
 
 def test_lengths_out_of_range(dev):
