@@ -66,12 +66,13 @@ __device__ __forceinline__ uint2 encode8(const float* n, const StaticDivisor& d)
         return make_uint2(e4m3_pack2(v[0], v[1]) | e4m3_pack2(v[2], v[3]) << 16, e4m3_pack2(v[4], v[5]) | e4m3_pack2(v[6], v[7]) << 16);
     return make_uint2(encode4(v[0], v[1], v[2], v[3]), encode4(v[4], v[5], v[6], v[7]));
 }
+// (The product of two bf16 values is exact in fp32: one rounding, that of r's product.)
 __device__ __forceinline__ void normed8(const v4i& t, const v4i& w, float r, float more, float* n) {
     float wf[8];
     unpack8(t, n);
     unpack8(w, wf);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) n[i] = n[i] * r * (wf[i] + more);
+    for (int i = 0; i < 8; ++i) n[i] = n[i] * (wf[i] + more) * r;
 }
 
 // Over the workgroup's wavefronts, whose words are in LDS, in their order.

@@ -11,7 +11,7 @@
 // no exchange, and the sum of squares is a few lane shuffles.  The angles are loaded once for the heads of a token that
 // a group goes through.  Bound by memory: every element is read once and written once; 13056 tokens of 8 + 2 heads of 256 in
 // 32.1 us, 4.6 TB/s, where a large copy runs at 5.2; one token 4.5 us, the launch.  Into pages in 8 bits, with two maxima over a head's lanes
-// and conversions besides, 33.9 us, 3.8 TB/s of fewer bytes.
+// and conversions besides, 28.0 us, 4.5 TB/s of fewer bytes (33.9 with groups of queries and of keys in one wavefront).
 #include "fp8_device.h"
 #include "layer_kernels.h"
 #include "quant_device.h"
@@ -88,11 +88,13 @@ __device__ __forceinline__ void write_codes(uint8_t* o, uint8_t* scale, int a, i
     for (int k = 1; k < (1 << lp_log); k <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, k));
     const bool known = m < 0x7F800000u;
     constexpr float most = TYPE == HEAD_BF16 ? 0x1.Ep127f : 61440.0f;
-    m = min(m, __float_as_uint(most));
+    if (__builtin_expect(m > __float_as_uint(most), 0)) {
+        m = __float_as_uint(most);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        x[i] = __builtin_amdgcn_fmed3f(x[i], -most, most);
-        y[i] = __builtin_amdgcn_fmed3f(y[i], -most, most);
+        for (int i = 0; i < V; ++i) {
+            x[i] = __builtin_amdgcn_fmed3f(x[i], -most, most);
+            y[i] = __builtin_amdgcn_fmed3f(y[i], -most, most);
+        }
     }
     if (!active || !write) return;
     const uint32_t power = known ? power_of(m) : 127u;
@@ -102,14 +104,78 @@ __device__ __forceinline__ void write_codes(uint8_t* o, uint8_t* scale, int a, i
     if ((threadIdx.x & ((1 << lp_log) - 1)) == 0) *scale = (uint8_t)power;
 }
 
+// A lane's runs of a head, normed and rotated.  FP8: with as few roundings as fp32 allows, since each of them moves codes over a border now and
+// then: a value times its weight is exact, one product of a rotation goes into a fused add.  (In 64 bits throughout, codes are off a
+// third as often, one or two of 3.3 million, at 39.5 us for 35.)
+template <int TYPE, int V, bool FP8>
+__device__ __forceinline__ void norm_and_turn(const HeadRope& p, const uint16_t* weight, const Run<V>& ra, const Run<V>& rb, int a, int b, bool active, bool turned,
+                                              const float* cs, const float* sn, int lp_log, float* x, float* y) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        x[i] = head_to_f32<TYPE>((ra.w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu);
+        y[i] = head_to_f32<TYPE>((rb.w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu);
+    }
+    if (weight != nullptr) {   // (uniform)
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) ss = __builtin_fmaf(x[i], x[i], __builtin_fmaf(y[i], y[i], ss));
+        for (int m = 1; m < (1 << lp_log); m <<= 1) ss += __shfl_xor(ss, m);
+        const float r = 1.0f / __builtin_sqrtf(ss / (float)p.D + p.eps);
+        Run<V> wa = {}, wb = {};
+        if (active) {
+            wa = load_run<V>(weight + a);
+            wb = load_run<V>(weight + b);
+        }
+        const float more = p.gemma ? 1.0f : 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float u = head_to_f32<TYPE>((wa.w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu) + more;
+            const float v = head_to_f32<TYPE>((wb.w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu) + more;
+            x[i] = FP8 ? x[i] * u * r : x[i] * r * u;
+            y[i] = FP8 ? y[i] * v * r : y[i] * r * v;
+        }
+    }
+    if (turned) {
+        auto turn = [](float u, float c, float w) { return FP8 ? __builtin_fmaf(u, c, w) : u * c + w; };
+        if (p.interleaved) {
+            // pairs (0, 1), (2, 3), ... of the first run, then of the second: angle i of the lane's V
+#pragma unroll
+            for (int i = 0; i < V; i += 2) {
+                const float u = x[i], v = x[i + 1], f = y[i], g = y[i + 1];
+                const float c0 = cs[i >> 1], s0 = sn[i >> 1], c1 = cs[(V + i) >> 1], s1 = sn[(V + i) >> 1];
+                x[i] = turn(u, c0, -(v * s0)); x[i + 1] = turn(v, c0, u * s0);
+                y[i] = turn(f, c1, -(g * s1)); y[i + 1] = turn(g, c1, f * s1);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float u = x[i], v = y[i];
+                x[i] = turn(u, cs[i], -(v * sn[i]));
+                y[i] = turn(v, cs[i], u * sn[i]);
+            }
+        }
+    }
+}
+
 // LP lanes a head (a power of two, at least D / (2 V)); `heads_per_group` heads of one token, neighbours, per group.
 template <int TYPE, int V, bool FP8>
-__global__ __launch_bounds__(256) void head_rope_kernel(const HeadRope p, int lp_log, int heads_per_group, int groups_per_token, int64_t groups) {
+__global__ __launch_bounds__(256) void head_rope_kernel(const HeadRope p, int lp_log, int heads_per_group, int groups_per_token, int64_t groups, int query_groups) {
     const int64_t group = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> lp_log;
     const int c = threadIdx.x & ((1 << lp_log) - 1);
     if (group >= groups) return;   // (a head's lanes leave together)
-    const int t = (int)(group / groups_per_token);
-    const int first = (int)(group - (int64_t)t * groups_per_token) * heads_per_group;
+    int t, nth;
+    if constexpr (FP8) {
+        // The groups of queries alone come first, of all tokens, so that few wavefronts have both kinds of work (13056 tokens of 8 + 2 heads of 256
+        // written and read back: 34.5 us, 38 in the tokens' order).
+        const uint32_t queries = (uint32_t)p.T * (uint32_t)query_groups, g = (uint32_t)group, rest = g < queries ? g : g - queries;
+        const uint32_t of = (uint32_t)(g < queries ? query_groups : groups_per_token - query_groups);
+        t = (int)(rest / of);
+        nth = (int)(rest - (uint32_t)t * of) + (g < queries ? 0 : query_groups);
+    } else {
+        t = (int)(group / groups_per_token);
+        nth = (int)(group - (int64_t)t * groups_per_token);
+    }
+    const int first = nth * heads_per_group;
     const int heads = p.H + 2 * p.KV;
     const int last = first + heads_per_group < heads ? first + heads_per_group : heads;
     const bool active = c * 2 * V < p.D;
@@ -172,49 +238,7 @@ __global__ __launch_bounds__(256) void head_rope_kernel(const HeadRope p, int lp
             continue;
         }
         float x[V], y[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            x[i] = head_to_f32<TYPE>((ra.w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu);
-            y[i] = head_to_f32<TYPE>((rb.w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu);
-        }
-        const uint16_t* weight = h < p.H ? p.q_weight : p.k_weight;
-        if (weight != nullptr) {   // (uniform)
-            float ss = 0.f;
-#pragma unroll
-            for (int i = 0; i < V; ++i) ss = __builtin_fmaf(x[i], x[i], __builtin_fmaf(y[i], y[i], ss));
-            for (int m = 1; m < (1 << lp_log); m <<= 1) ss += __shfl_xor(ss, m);
-            const float r = 1.0f / __builtin_sqrtf(ss / (float)p.D + p.eps);
-            Run<V> wa = {}, wb = {};
-            if (active) {
-                wa = load_run<V>(weight + a);
-                wb = load_run<V>(weight + b);
-            }
-            const float more = p.gemma ? 1.0f : 0.0f;
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                x[i] = x[i] * r * (head_to_f32<TYPE>((wa.w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu) + more);
-                y[i] = y[i] * r * (head_to_f32<TYPE>((wb.w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu) + more);
-            }
-        }
-        if (turned) {
-            if (p.interleaved) {
-                // pairs (0, 1), (2, 3), ... of the first run, then of the second: angle i of the lane's V
-#pragma unroll
-                for (int i = 0; i < V; i += 2) {
-                    const float u = x[i], v = x[i + 1], f = y[i], g = y[i + 1];
-                    const float c0 = cs[i >> 1], s0 = sn[i >> 1], c1 = cs[(V + i) >> 1], s1 = sn[(V + i) >> 1];
-                    x[i] = u * c0 - v * s0; x[i + 1] = v * c0 + u * s0;
-                    y[i] = f * c1 - g * s1; y[i + 1] = g * c1 + f * s1;
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float u = x[i], v = y[i];
-                    x[i] = u * cs[i] - v * sn[i];
-                    y[i] = v * cs[i] + u * sn[i];
-                }
-            }
-        }
+        norm_and_turn<TYPE, V, FP8>(p, h < p.H ? p.q_weight : p.k_weight, ra, rb, a, b, active, turned, cs, sn, lp_log, x, y);
         if constexpr (FP8) {
             if (h >= p.H) {   // (uniform in a head's lanes)
                 const int j = h - p.H;
@@ -251,7 +275,9 @@ hipError_t launch_v(const HeadRope& p, hipStream_t stream) {
     const int per_token = (heads + per_group - 1) / per_group;
     const int64_t groups = (int64_t)p.T * per_token;
     const int64_t threads = groups << lp_log;
-    return enqueue(head_rope_kernel<TYPE, V, FP8>, dim3((uint32_t)((threads + 255) / 256)), dim3(256), stream, p, lp_log, per_group, per_token, groups);
+    if (threads > 0xFFFFFF00ll) return hipErrorInvalidConfiguration;   // (more than a launch has)
+    return enqueue(head_rope_kernel<TYPE, V, FP8>, dim3((uint32_t)((threads + 255) / 256)), dim3(256), stream, p, lp_log, per_group, per_token, groups,
+                   p.H / per_group);
 }
 
 }  // namespace
