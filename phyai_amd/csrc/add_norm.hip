@@ -224,7 +224,10 @@ hipError_t launch_blocks(const AddNorm& p, hipStream_t stream) {
     int chunks = 1;
     if (p.M * threads_of(1) > 4096 * kWave) chunks = threads_of(3) * 3 < threads_of(2) * 2 ? 3 : 2;
     if (lanes <= kWave) chunks = 1;
-    if (const char* forced = tuning_env("PHYAI_LAYER_ADD_NORM")) chunks = atoi(forced);
+    if (const char* forced = tuning_env("PHYAI_LAYER_ADD_NORM")) {   // (what is no number of chunks changes nothing)
+        const int n = atoi(forced);
+        if (n >= 1 && n <= 4) chunks = n;
+    }
     while (threads_of(chunks) > 1024) ++chunks;
     const dim3 threads((uint32_t)threads_of(chunks));
     if (lanes > 4096) return enqueue(add_norm_long_kernel<BLOCKS>, grid, dim3(512), stream, p);

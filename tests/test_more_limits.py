@@ -1,0 +1,30 @@
+"""Host logic of the operators around a cache in 8 bits that decides about a launch: no GPU needed, and with one there is nothing to see
+here (the buffers are the host's)."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from phyai_amd import _lib
+
+ELAUNCH = -4   # phyai_fp8.h: all checks are passed, and there is no device
+
+
+def norm_call(lib, **over):
+    raw = (ctypes.c_char * 65792)()
+    p = (ctypes.addressof(raw) + 255) // 256 * 256
+    at = dict(x=p, ldx=64, res=p + 4096, ldr=64, w=p + 61440, gemma=0, eps=1e-6, M=4, D=64, total=p + 8192, ldt=64, xq=p + 16384, xs=p + 32768, row=1, block=1)
+    for name, value in over.items():
+        at[name] = value if name not in ("total", "xq") or value is None else p + value
+    return lib.phyai_layer_add_rmsnorm_quant(*at.values(), None)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="would be launched on the host's memory")
+@pytest.mark.parametrize("value", ["0", "", "x", "-3", "9", "1", "4"])
+def test_a_forced_number_of_chunks_is_one_that_there_is(monkeypatch, value):
+    """Anything but 1 to 4 is no number of chunks a thread: zero of them was a division by zero."""
+    monkeypatch.setenv("PHYAI_LAYER_ADD_NORM", value)
+    assert norm_call(_lib.load()) == ELAUNCH
