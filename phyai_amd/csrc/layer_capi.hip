@@ -406,7 +406,7 @@ int phyai_layer_add_rmsnorm_quant(const void* x, int64_t ldx, const void* residu
     // (in place is fine: a thread reads what it writes, before; anywhere else rows would be written that others still read)
     for (const void* in : {x, residual}) {
         const int64_t ld = in == x ? ldx : ldr;
-        if (!(in == total && ld == ldt) && overlap(in, ld * 2, D * 2, total, ldt * 2, D * 2, M))
+        if (!(in == total && (ld == ldt || M == 1)) && overlap(in, ld * 2, D * 2, total, ldt * 2, D * 2, M))
             return fail(PHYAI_FP8_EINVAL, "%s: total overlaps an input without being it", fn);
         if (overlap(in, ld * 2, D * 2, xq, D, D, M)) return fail(PHYAI_FP8_EINVAL, "%s: xq overlaps an input", fn);
     }
