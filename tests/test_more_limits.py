@@ -45,3 +45,11 @@ def test_one_row_in_place_has_no_stride(strides):
     assert call(1) == ELAUNCH
     if at["ldx"] != at["ldt"]:
         assert call(2) == -1 and b"total overlaps" in lib.phyai_layer_last_error()
+
+
+@pytest.mark.parametrize("over,what", [(dict(total=16), b"total overlaps an input"), (dict(total=4096 + 128), b"total overlaps an input"),
+                                       (dict(total=0, ldt=72), b"total overlaps an input"), (dict(xq=0), b"xq overlaps an input"),
+                                       (dict(xq=4096), b"xq overlaps an input"), (dict(xq=8192), b"xq overlaps total")])
+def test_overlaps_are_what_is_refused(over, what):
+    lib = _lib.load()
+    assert norm_call(lib, **over) == -1 and what in lib.phyai_layer_last_error(), lib.phyai_layer_last_error()
