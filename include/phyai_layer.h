@@ -101,14 +101,16 @@ int phyai_layer_paged_attention(const void *q, int64_t q_token_stride, int64_t q
  * Since version 2: the same half of a layer over a cache in 8 bits, and batches that share a prefix.
  *
  * A cache in 8 bits holds e4m3fn codes (strides multiples of 16 bytes) and, for each token and head, a byte b in a tensor of
- * its own (any strides): a code stands for code * 2^(b - 127), exactly, in bfloat16; in half precision as far as that
- * reaches.  255: all of the head's elements are NaNs.  head_dim is a multiple of 16.
+ * its own (any strides): a code stands for code * 2^(b - 127), rounded once, to nearest even, to the element type.  bfloat16 holds it
+ * exactly for b from 3 to 246 and half precision from 112 to 134; beyond, large codes are infinite and small ones of the type's
+ * subnormal numbers or zero.  255: all of the head's elements are NaNs.  head_dim is a multiple of 16.
  */
 
 /*
  * phyai_layer_head_rope into such a cache.  b is the smallest with which the head's largest magnitude, in fp32 after norm and
  * rotation, stays within 448 (1 at least), so no code is ever beyond the type; codes are rounded to nearest even from fp32.
- * Finite values end at 1.875 times the type's largest power of two (half precision: 61440).  A head with an infinity or a NaN is written as NaNs.
+ * Finite values end at 1.875 times the type's largest power of two (half precision: 61440), so what is written is never read as
+ * infinite.  A head with an infinity or a NaN is written as NaNs.
  */
 int phyai_layer_head_rope_fp8(const void *qkv, int64_t ld, const void *q_weight, const void *k_weight, const float *cos_sin,
                               int64_t table_rows, const int64_t *positions, void *q_out, void *k_pages, void *v_pages,

@@ -14,7 +14,7 @@
 // f of its own for K (sixteen neighbouring keys, one chunk: sixteen bank groups) and for V (four keys, four chunks).
 //
 // A cache in 8 bits holds e4m3 codes and a power of two for each key and head: code times power is a value of the element type
-// exactly (four significant bits), so its keys go through registers on their way to LDS, where they arrive in 16 bits, and
+// (widen.h), so its keys go through registers on their way to LDS, where they arrive in 16 bits, and
 // everything behind that is the same.
 //
 // The kernels are templates: paged_attention.hip has those of plain 16-bit calls (MODE 0), attention_{bf16,f16,bf16_fp8,f16_fp8}.hip the others.

@@ -1,5 +1,5 @@
-// Keys and values of single tokens out of a paged cache in 8 bits: out[t, h, :] = code * 2^(b - 127) in the element type, which
-// holds such a product exactly (gfx950).  Sixteen codes a thread, one load and two stores; bound by memory, three bytes an element: 13056 tokens
+// Keys and values of single tokens out of a paged cache in 8 bits: out[t, h, :] = code * 2^(b - 127) in the element type (what
+// it holds of that exactly: widen.h; gfx950).  Sixteen codes a thread, one load and two stores; bound by memory, three bytes an element: 13056 tokens
 // of one head of 256 in 6.0 us, 3.3 TB/s with the launch's 2 us in it; one token 1.6 us.
 #include "fp8_device.h"
 #include "layer_kernels.h"

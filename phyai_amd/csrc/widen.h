@@ -1,6 +1,6 @@
 // Codes of a cache in 8 bits as values: e4m3 times the power of two that a token's head has, a byte b that stands for 2^(b - 127)
-// (255: not a number).  Four significant bits times a power are a value of bfloat16 exactly, and of half precision where that
-// reaches.
+// (255: not a number).  Four significant bits times a power are a value of bfloat16 exactly for b from 3 to 246, of half precision from
+// 112 to 134; beyond, the conversion rounds to nearest even, to subnormal numbers and infinities too.
 #pragma once
 
 #include "fp8_device.h"
@@ -10,7 +10,7 @@ namespace phyai {
 
 constexpr uint32_t kNanCodes = 0x7F7F7F7Fu;
 
-// Two codes times a power as two values in a word: one instruction.
+// Two codes times a power as two values in a word: one instruction, which takes the power from the exponent's bits alone: 0.0 is 2^-127.
 template <int TYPE>
 __device__ __forceinline__ uint32_t widen2(uint32_t codes, float power, bool upper) {
     if constexpr (TYPE == HEAD_BF16) {

@@ -1021,7 +1021,8 @@ def qk_norm_rope(qkv: torch.Tensor, cos_sin: torch.Tensor, positions: torch.Tens
 def read_fp8_cache(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor, slots: torch.Tensor, *,
                    dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
     """Keys and values of single tokens of a cache in 8 bits (:func:`fp8_cache`, written by :func:`qk_norm_rope`), ``[T, kv_heads,
-    head_dim]`` each in ``dtype`` (bf16, which holds them exactly, or fp16): what :func:`paged_attention` sees of them.  ``slots``: ``[T]``
+    head_dim]`` each in ``dtype``, bf16 or fp16: what :func:`paged_attention` sees of them, code times power rounded once (nothing to round for
+    powers of 2^-124 to 2^119 in bf16, 2^-15 to 2^7 in fp16).  ``slots``: ``[T]``
     int64, page * page_size + place; one outside the cache reads as zeros."""
     op = "read_fp8_cache"
     got = _native().read_fp8_cache(k_pages, v_pages, k_scales, v_scales, slots, dtype)
