@@ -416,7 +416,7 @@ __device__ __forceinline__ uint32_t without_special(uint32_t w) {
 }
 // A probability of zero times an infinity or a NaN is a NaN.  In a tile that some rows see only part of, such values are
 // taken out of V as it lands (each wavefront looks through the `keys` keys it has copied itself and whatever lies behind them;
-// true if there were any among the keys), and add_special gives them to the rows that see their key after the last tile.
+// true if there were any among the keys), and add_specials gives them to the rows that see their key after the last tile.
 template <int DP, int TYPE, int N>
 __device__ __forceinline__ bool clean_values(uint8_t* v, int keys) {
     bool special = false;
@@ -441,37 +441,87 @@ __device__ __forceinline__ bool clean_values(uint8_t* v, int keys) {
     }
     return __any(special);
 }
-// Keys first .. last - 1, from their pages.  (A page that does not exist has made its scores NaN already.)
-template <int DP, int TYPE, int MODE>
-__device__ __forceinline__ void add_special(State<DP>& st, const Pool& s, int first, int last, int d_end, int lo, int hi) {
+template <int N_>
+struct Unrolled {
+    static constexpr int N = N_;
+};
+// Infinities and NaNs of keys first .. last - 1, from their pages: add(q, e, value) is for value dim 8 q + 4 (lane / 32) + e of the lane's row.
+// (A page that does not exist has made its scores NaN already.)
+template <int DP, int TYPE, int MODE, int UNROLLED, typename Add>
+__device__ __forceinline__ void special_values(const Pool& s, int first, int last, int d_end, int lo, int hi, Add add) {
     const int half = (threadIdx.x & 63) >> 5;
     last = last < s.kv_len ? last : s.kv_len;
 #pragma unroll 1
     for (int j = first; j < last; ++j) {
         const int at = divide(j, s.by_page), page = s.table[at];
-        if (page < 0 || page >= s.n_pages) continue;
+        if (page < 0 || page >= s.n_pages || j < lo || j >= hi) continue;
         const uint8_t* v = s.v + (int64_t)page * s.page_bytes + (int64_t)(j - at * s.page_size) * s.token_bytes;
-        const bool sees = j >= lo && j < hi;
         uint32_t power = 0;
         if constexpr (MODE & MODE_FP8) power = s.v_scale[(int64_t)page * s.scale_page + (int64_t)(j - at * s.page_size) * s.scale_token];
-#pragma unroll
-        for (int b = 0; b < DP / 32; ++b)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int d = 32 * b + 8 * i + 4 * half;
-                uint2 w = make_uint2(0, 0);
-                if (d < d_end && sees) {
-                    if constexpr (MODE & MODE_FP8) {
-                        const uint32_t codes = power == 255 ? kNanCodes : *reinterpret_cast<const uint32_t*>(v + d);
-                        w = make_uint2(widen2<TYPE>(codes, __uint_as_float(power << 23), false), widen2<TYPE>(codes, __uint_as_float(power << 23), true));
-                    } else w = *reinterpret_cast<const uint2*>(v + 2 * d);
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t h = ((e & 2 ? w.y : w.x) >> (16 * (e & 1))) & 0xFFFFu;
-                    if (any_special<TYPE>(h)) st.o[b][4 * i + e] += to_f32<TYPE>(h);
-                }
+#pragma unroll UNROLLED
+        for (int q = 0; q < DP / 8; ++q) {
+            const int d = 8 * q + 4 * half;
+            uint2 w = make_uint2(0, 0);
+            if (d < d_end) {
+                if constexpr (MODE & MODE_FP8) {
+                    const uint32_t codes = power == 255 ? kNanCodes : *reinterpret_cast<const uint32_t*>(v + d);
+                    w = make_uint2(widen2<TYPE>(codes, __uint_as_float(power << 23), false), widen2<TYPE>(codes, __uint_as_float(power << 23), true));
+                } else w = *reinterpret_cast<const uint2*>(v + 2 * d);
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t h = ((e & 2 ? w.y : w.x) >> (16 * (e & 1))) & 0xFFFFu;
+                if (any_special<TYPE>(h)) add(q, e, to_f32<TYPE>(h));
+            }
+        }
+    }
+}
+// O in LDS: a row of it for each of a wavefront's rows, OLD floats apart.
+template <int DP>
+constexpr int OLD = DP + 4;
+template <int DP>
+__device__ __forceinline__ float* row_of_sums(float* sums) { return sums + (threadIdx.x & 31) * OLD<DP> + 4 * ((threadIdx.x & 63) >> 5); }
+template <int DP>
+__device__ __forceinline__ void put_sums(const State<DP>& st, float* row) {
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v4f v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = st.o[b][4 * i + e];
+            *reinterpret_cast<v4f*>(row + 32 * b + 8 * i) = v;
+        }
+}
+template <int DP>
+__device__ __forceinline__ void get_sums(State<DP>& st, const float* row) {
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const v4f v = *reinterpret_cast<const v4f*>(row + 32 * b + 8 * i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) st.o[b][4 * i + e] = v[e];
+        }
+}
+// Those of the blocks of STEP keys from begin up to end that some rows see only part of.  O goes through LDS meanwhile (`sums`: the wavefront's, which nobody
+// reads any more): in registers, an element of O each in the code, their masks spilled up to 270 scalars into vector registers that the loop over
+// the keys wants, and 8 to 24 bytes of scratch in the kernels of 8 bits and 128 dims (at 256, up to 556 with selects for the branches).  16 x 816 tokens
+// of 256 dims in half precision 68.5 to 67.6 us, 2048 over 8192 keys of 128 dims 257 to 252.  64 dims have the registers, and 30.5 us for 29.6 by way of LDS.
+template <int DP, int TYPE, int MODE, int STEP>
+__device__ __forceinline__ void add_specials(State<DP>& st, float* sums, const Pool& s, int begin, int end, int all_lo, int all_hi, int d_end, int lo, int hi) {
+    auto blocks = [&](auto unrolled, auto add) {
+#pragma unroll 1
+        for (int blk = begin; blk < end; ++blk)
+            if (blk * STEP < all_lo || blk * STEP + STEP > all_hi) special_values<DP, TYPE, MODE, decltype(unrolled)::N>(s, blk * STEP, blk * STEP + STEP, d_end, lo, hi, add);
+    };
+    if constexpr (DP == 64) {
+        blocks(Unrolled<DP / 8>(), [&](int q, int e, float v) { st.o[q >> 2][4 * (q & 3) + e] += v; });
+    } else {
+        float* row = row_of_sums<DP>(sums);
+        put_sums<DP>(st, row);
+        blocks(Unrolled<1>(), [&](int q, int e, float v) { row[8 * q + e] += v; });
+        get_sums<DP>(st, row);
     }
 }
 
@@ -773,8 +823,7 @@ template <int DP, int WAVES_OF>
 struct SplitShape {
     static constexpr int WAVES = WAVES_OF;
     static constexpr int STAGE = 2 * 32 * Shape<DP>::ROW;
-    static constexpr int OLD = DP + 4;                            // floats of a row of O in LDS
-    static constexpr int WAVE_BYTES = STAGE > 32 * OLD * 4 ? STAGE : 32 * OLD * 4;
+    static constexpr int WAVE_BYTES = STAGE > 32 * OLD<DP> * 4 ? STAGE : 32 * OLD<DP> * 4;
     static constexpr int LDS = WAVES * (WAVE_BYTES + 512 + 256 + 128);   // and page numbers, maxima and sums, shares
 };
 template <int DP>
@@ -918,24 +967,11 @@ __device__ __forceinline__ void attend_split(const PagedAttention& p, const Plan
             return mine;
         }, Nothing());
     }
-    if (special) {
-#pragma unroll 1
-        for (int blk = begin; blk < end; ++blk)
-            if (blk * 32 < all_lo || blk * 32 + 32 > all_hi) add_special<DP, TYPE, MODE>(st, pool, blk * 32, blk * 32 + 32, p.D, row.lo, row.hi);
-    }
+    if (special) add_specials<DP, TYPE, MODE, 32>(st, reinterpret_cast<float*>(mine), pool, begin, end, all_lo, all_hi, p.D, row.lo, row.hi);
     // the wavefronts' states meet
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     const float l = other_half_sum(st.l);
-    float* o = reinterpret_cast<float*>(mine);
-#pragma unroll
-    for (int b = 0; b < DP / 32; ++b)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v4f v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = st.o[b][4 * i + e];
-            *reinterpret_cast<v4f*>(o + (lane & 31) * X::OLD + 32 * b + 8 * i + 4 * (lane >> 5)) = v;
-        }
+    put_sums<DP>(st, row_of_sums<DP>(reinterpret_cast<float*>(mine)));
     if (lane < 32) {
         const int from = row.lo > begin * 32 ? row.lo : begin * 32, to = row.hi < end * 32 ? row.hi : end * 32;
         ml[wave][lane][0] = st.m == kNone && l == 0.f && from < to ? kLowest : st.m;
@@ -969,7 +1005,7 @@ __device__ __forceinline__ void attend_split(const PagedAttention& p, const Plan
 #pragma unroll
         for (int w = 0; w < X::WAVES; ++w) {
             const float a = weight[w][r];
-            const v4f ow = *reinterpret_cast<const v4f*>(reinterpret_cast<const float*>(lds + w * X::WAVE_BYTES) + r * X::OLD + d);
+            const v4f ow = *reinterpret_cast<const v4f*>(reinterpret_cast<const float*>(lds + w * X::WAVE_BYTES) + r * OLD<DP> + d);
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(ow[e], a, v[e]);
         }
@@ -1196,11 +1232,9 @@ __device__ __forceinline__ void attend_many(const PagedAttention& p, const Plan&
     if (lane == 0) specials[wave] = special ? 1 : 0;
     __syncthreads();
     if ((specials[0] | specials[1] | specials[2] | specials[3]) != 0) {
-#pragma unroll 1
-        for (int step = begin; step < end; ++step) {
-            const int j0 = step * X::STEP;
-            if (j0 < all_lo || j0 + X::STEP > all_hi) add_special<DP, TYPE, MODE>(st, pool, j0, j0 + X::STEP, p.D, row.lo, row.hi);
-        }
+        // (the wavefronts' sums lie in all of LDS but these words)
+        static_assert(X::WAVES * 32 * OLD<DP> * 4 <= 2 * X::STAGE + X::WAVES * 512, "sums reach into the words between wavefronts");
+        add_specials<DP, TYPE, MODE, X::STEP>(st, reinterpret_cast<float*>(lds) + wave * 32 * OLD<DP>, pool, begin, end, all_lo, all_hi, p.D, row.lo, row.hi);
     }
     const float l = other_half_sum(st.l);
     if constexpr (MODE & MODE_MORE) {
