@@ -150,3 +150,30 @@ def test_attention_sees_what_is_read_back(dev, monkeypatch, plan, dtype, d):
         out = ops().paged_attention(q, k, v, steps[:256].view(256, 1).contiguous(), steps, torch.ones(256, dtype=torch.int32, device=dev), k_scales=ks, v_scales=vs)
         off = ~((out == want) | (out.isnan() & want.isnan()))
         assert not off.any(), (int(off.sum()), [(i, part + j, float(out[i, 0, j]), float(want[i, 0, j])) for i, _, j in off.nonzero()[:8].tolist()])
+
+
+@pytest.mark.parametrize("d", [64, 80, 128, 256])
+@pytest.mark.parametrize("bits,dtype", [(8, torch.bfloat16), (16, torch.bfloat16), (16, torch.float16)])
+@pytest.mark.parametrize("plan", ["0 2 0 0 3", "0 2 1 0 2", "0 2 1 1 3", "1 2 0 1 3", "1 1 0 0 0", "0 1 0 0 0"])
+def test_unknown_values_of_shared_and_own_keys(dev, monkeypatch, plan, bits, dtype, d):
+    """NaNs and infinities among shared values and a sequence's own, tokens that stand inside the prefix: they reach the rows that see their key
+    and no other, whichever kernels share the work."""
+    from test_gpu_more_ops import attend, attend_case, within
+
+    monkeypatch.setenv("PHYAI_LAYER_ATTEND_MORE", plan)
+    qs, kvs = [20, 30, 10], [64, 70, 66]
+    tensors, kw = attend_case((qs, kvs, 16, 4, 2, d, True, None, [0, 45, 0], None), dtype, bits, shared=64)
+    want, bound = oracle.attention(*tensors.values(), **kw)
+    table, values = tensors["page_table"], tensors["v_pages"]
+    planted = [(None, 42, 3), (None, 50, d - 1), (1, 66, 17), (2, 64, 40)]     # (whose, key, value dim): the first two of all sequences
+    position = torch.cat([torch.arange(kv - q, kv) for q, kv in zip(qs, kvs)])
+    sequence = torch.repeat_interleave(torch.arange(3), torch.tensor(qs))
+    hit = torch.zeros(60, 4, d, dtype=torch.bool)
+    for n, (b, key, at) in enumerate(planted):
+        values[table[b or 0, key // 16].long(), key % 16, 1, at] = 0x7F if bits == 8 else (float("nan"), float("inf"))[n % 2]
+        rows = (position >= key) | ((sequence == 1) & (key < 45)) if b is None else (position >= key) & (sequence == b)
+        hit[rows, 2:, at] = True                                              # (key head 1: query heads 2 and 3)
+    for shared in (64, 0):
+        out = attend(dev, tensors, kw | dict(shared_prefix=shared)).cpu().double()
+        assert not out[hit].isfinite().any(), shared
+        within(torch.where(hit, 0.0, out), torch.where(hit, 0.0, want), torch.where(hit, 0.0, bound), f"shared {shared}")
