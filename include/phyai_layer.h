@@ -110,7 +110,7 @@ int phyai_layer_paged_attention(const void *q, int64_t q_token_stride, int64_t q
  * phyai_layer_head_rope into such a cache.  b is the smallest with which the head's largest magnitude, in fp32 after norm and
  * rotation, stays within 448 (1 at least), so no code is ever beyond the type; codes are rounded to nearest even from fp32.
  * Finite values end at 1.875 times the type's largest power of two (half precision: 61440), so what is written is never read as
- * infinite.  A head with an infinity or a NaN is written as NaNs.
+ * infinite, in the same type.  A head with an infinity or a NaN is written as NaNs.
  */
 int phyai_layer_head_rope_fp8(const void *qkv, int64_t ld, const void *q_weight, const void *k_weight, const float *cos_sin,
                               int64_t table_rows, const int64_t *positions, void *q_out, void *k_pages, void *v_pages,

@@ -66,7 +66,7 @@ __device__ __forceinline__ uint2 encode8(const float* n, const StaticDivisor& d)
         return make_uint2(e4m3_pack2(v[0], v[1]) | e4m3_pack2(v[2], v[3]) << 16, e4m3_pack2(v[4], v[5]) | e4m3_pack2(v[6], v[7]) << 16);
     return make_uint2(encode4(v[0], v[1], v[2], v[3]), encode4(v[4], v[5], v[6], v[7]));
 }
-// (The product of two bf16 values is exact in fp32: one rounding, that of r's product.)
+// (The product of two bf16 values is exact in fp32: one rounding, that of r's product.  With gemma w + 1 may round as well, and its product with t.)
 __device__ __forceinline__ void normed8(const v4i& t, const v4i& w, float r, float more, float* n) {
     float wf[8];
     unpack8(t, n);

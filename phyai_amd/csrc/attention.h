@@ -262,8 +262,9 @@ struct Feeder {
 
 // The same part of a block for pages in 8 bits, through registers: what was asked for while a block was worked on is widened and
 // put into LDS at its end (32 keys of 128 dims: 32 registers a lane).  The places of 64 keys are looked up at once, as above,
-// their scales with them: 64 sequences of up to 8192 keys of 8 heads of 128 in 171 us, 4.2 TB/s, where 16 bits take 254 at 5.1: what is left is the
-// chain of a wavefront (codes, LDS, products) with eight of them a CU.  Widening costs the many-row kernel what it saves in bytes and more: 2048 tokens over 8192 keys 352 us for 272.
+// their scales with them: 64 sequences of up to 8192 keys of 8 heads of 128 in 165 us, 4.3 TB/s, where the same keys in 16 bits take 267 at 5.3: what is left is the
+// chain of a wavefront (codes, LDS, products) with eight of them a CU.  Widening costs the many-row kernel, in which each workgroup does it again, what it saves in bytes and
+// more: 2048 tokens over 8192 keys 310 us for 255.
 template <int DP, int TYPE, int STEP, int N>
 struct Widener {
     static constexpr int LANES = DP / 16, PER = 64 / LANES, LOADS = N / PER, BLOCKS = 64 / N, ROW = Shape<DP>::ROW;   // lanes of a key, keys of a load
@@ -585,8 +586,8 @@ __device__ __forceinline__ void raise_maximum(State<DP>& st, float mx) {
 // A score s to cap tanh(s / cap) in base 2: with e = 2^(s by), by = 2 log2(e) scale / cap, tanh = 1 - 2 / (e + 1), exact where the
 // power over- or underflows.  Kept is -1 / (e + 1), from which the score (less a maximum) is one multiply-add: times 2 cap log2(e), and cap log2(e)
 // left out, which all scores have in common.  Off by some 2^-22 of cap in all, which is what the score's own rounding is.
-// Four instructions a score, two of them at a quarter of the rate, and not hidden behind the products: 2048 tokens of 32 heads of 128 over 8192
-// keys 390 us for 275, 16 x 816 of 8 heads of 256 100 for 79.
+// Four instructions a score, two of them at half the rate, and not hidden behind the products: 2048 tokens of 32 heads of 128 over 8192
+// keys 354 us for 255, 16 x 816 of 8 heads of 256 98 for 76.
 struct Cap {
     float by, most;
 };
@@ -597,7 +598,9 @@ __device__ __forceinline__ void cap_some(v16f& s, int first, Cap c) {
 }
 // That rounding is 2^-22 of the cap also for scores far below it, which large caps are there to leave alone.  So for those: with y = s by,
 // by = scale / cap, s times the first terms of tanh(y) / y = 1 - y^2 / 3 + ..., the one left out 6e-8 of it at the border, and beyond
-// cap / scale times 1 - 2 / (e^2y + 1).  The result is a score as it was.  Three times the instructions: only in kernels of its own.
+// cap / scale times 1 - 2 / (e^2y + 1).  The result is a score as it was.  Three times the instructions: only in kernels of its own,
+// and only in those for few rows: 64 sequences of up to 8192 keys in 8 bits 210 us where a cap of 50 takes 170, but 2048 tokens over 8192 keys 770 for 396 (16 bits 634 for
+// 354), 16 x 816 of 256 dims 160 for 98, 64 tokens behind 8192 shared keys 94 for 39 without a cap.
 __device__ __forceinline__ void cap_wide(v16f& s, Cap c) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -817,8 +820,8 @@ __device__ __forceinline__ Pool make_pool(const PagedAttention& p, const Tile& t
 // Each wavefront has 32 keys in LDS to itself and waits for nobody until the end: it copies a block, waits, multiplies,
 // copies the next; the others' copies are under way meanwhile (twice as many wavefronts beat two stages for each).  Then the
 // workgroup's states meet in LDS; with more than one workgroup per tile they leave unnormalised sums for
-// attend_join_kernel.  Many sequences: bound by memory, 64 x 8192 keys of 8 heads of 128 in 254 us, 5.1 TB/s.  Few: by the chain of
-// sequence, page numbers, keys (64 bytes a cycle into a CU), products, sums: 50 tokens over 866 keys of 256 dims 15.3 us, 3 to 4 of them the join.
+// attend_join_kernel.  Many sequences: bound by memory, 64 x 8192 keys of 8 heads of 128 in 253 us, 5.1 TB/s.  Few: by the chain of
+// sequence, page numbers, keys (64 bytes a cycle into a CU), products, sums: 50 tokens over 866 keys of 256 dims 14.4 us, 3 to 4 of them the join.
 template <int DP, int WAVES_OF>
 struct SplitShape {
     static constexpr int WAVES = WAVES_OF;
@@ -1087,7 +1090,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const PagedAttention p
 // A step of 64 keys at a time, the next one on its way to LDS meanwhile; a wait for the wavefront's own copies and a barrier a
 // step.  Bound by the issue of instructions: two wavefronts a SIMD, of which each has 130 vector and 86 scalar ones beside 16
 // products for 32 keys when it takes those at a time (four such steps in LDS: 316 us for 2048 tokens of 32 heads of 128
-// dims over 8192 keys, 84 us for 16 x 816 of 8 heads of 256 over 816), and far fewer for 64 (then 270 and 77, now 260 and 68).
+// dims over 8192 keys, 84 us for 16 x 816 of 8 heads of 256 over 816), and far fewer for 64 (then 270 and 77, now 255 and 67).
 template <int DP>
 struct ManyShape {
     static constexpr int WAVES = 4, STEP = 64, MINE = STEP / WAVES, STAGE = 2 * STEP * Shape<DP>::ROW;
@@ -1278,8 +1281,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
 }
 
 // The shared keys for many rows a workgroup, bound by arithmetic, and the sequences' own for few, bound by memory, in one launch: first
-// come the workgroups of the shared ones.  64 single tokens of 32 heads on 8 of 128 dims behind 8192 shared keys, up to 512 of their own: 37 us
-// and 5 for the join, where few rows for both take 67, and 180 without sharing.
+// come the workgroups of the shared ones.  64 single tokens of 32 heads on 8 of 128 dims behind 8192 shared keys, up to 512 of their own: 33 us
+// and 5 for the join, where few rows for both take 64 in all, and 110 without sharing.
 template <int DP, int TYPE, int MODE>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_both_kernel(const PagedAttention p, const Plan g, float* __restrict__ part) {
     using X = SplitShape<DP, 4>;

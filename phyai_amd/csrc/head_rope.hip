@@ -105,7 +105,7 @@ __device__ __forceinline__ void write_codes(uint8_t* o, uint8_t* scale, int a, i
 }
 
 // A lane's runs of a head, normed and rotated.  FP8: with as few roundings as fp32 allows, since each of them moves codes over a border now and
-// then: a value times its weight is exact, one product of a rotation goes into a fused add.  (In 64 bits throughout, codes are off a
+// then: a value times its weight is exact (but for the Gemma form, whose w + 1 has more bits), one product of a rotation goes into a fused add.  (In 64 bits throughout, codes are off a
 // third as often, one or two of 3.3 million, at 39.5 us for 35.)
 template <int TYPE, int V, bool FP8>
 __device__ __forceinline__ void norm_and_turn(const HeadRope& p, const uint16_t* weight, const Run<V>& ra, const Run<V>& rb, int a, int b, bool active, bool turned,

@@ -64,13 +64,14 @@ double together(const Part* parts, int count, int64_t at_once) {
 
 // Calls that are more than plain ones: few rows a workgroup with all its wavefronts or half of them (two of those a CU), or many rows, each
 // with the keys split or not, and shared keys beside the sequences' own, for few rows or many.  The
-// choice with the least expected time; a workgroup takes its start (9 us for few rows, 12 for many: most of it instructions that a cold
-// cache does not have, and three turns of memory) and its blocks of 32 keys a wavefront, or steps of 64, at what they take where the
+// choice with the least expected time; a workgroup takes its start (9 us for few rows, 12 for many, fitted to measured times: three turns of
+// memory, and instructions that a cold cache does not have) and its blocks of 32 keys a wavefront, or steps of 64, at what they take where the
 // CU is full; sums to be joined take 4.5.  Measured, few rows with all wavefronts / half of them / many rows, best number of splits each, 8 bits and
-// 32 heads on 8 of 128 dims unless said: 64 single tokens of 8192 keys 177 / 169 / -, 16 of them 53 / 48, 4 of them 20 / 22, 32 of 400 11 / 14, 256 of
-// 1000 114 / 94; 256 tokens of 1024 20 / 27 / 31, 512 of 512 26 / 19 / 26, 512 of 4096 79 / 71 / 63, 2048 of 8192 625 / 567 / 360; 1000 of 1000 of 64
-// dims 39 / 29 / 38; 16 x 816 of 816 of 256 dims in 16 bits 149 / 124 / 103.  64 tokens behind 8192 shared keys and up to 512 of their
-// own: few and few rows 67, many and few 53, nothing shared 180; 16 of them 28 and 35.
+// 32 heads on 8 of 128 dims unless said, more than one token with a cap but for 4096 keys: 64 single tokens of 8192 keys 165 / 155 / -, 16 of them 48 / 43, 4 of them 18 / 18, 32 of
+// 400 9 / 12, 256 of 1000 101 / 86; 256 tokens of 1024 19 / 26 / 30, 512 of 512 23 / 17 / 25, 512 of 4096 76 / 72 / 61, 2048 of 8192 583 / 530 / 358; 1000 of 1000 of 64
+// dims 40 / 30 / 38; 16 x 816 of 816 of 256 dims in 16 bits 144 / 116 / 98.  64 tokens behind 8192 shared keys and up to 512 of their
+// own in 16 bits: few and few rows 64, many and few 39 (16 shared splits; 43 with 8, 49 with 32), nothing shared 110; 16 of them 25 and 24.
+// The rule's choices there: 166, 48, 17, 12, 87, 19, 17, 74, 383, 40, 99 and 40, 26; late by a third for 32 of 400 and 1000 of 64 dims, by a fifth for 512 of 4096.
 // (few_only: kernels for caps above kWideCap are there for few rows with all wavefronts.)
 // PHYAI_LAYER_ATTEND_MORE = "many splits small shared_many shared_splits" (shared_splits 0: nothing is shared) forces one.
 Plan make_plan_more(int64_t T, int64_t B, int64_t H, int64_t KV, int64_t D, int64_t max_kv, int64_t page_size, int64_t shared, int64_t window, bool few_only) {
