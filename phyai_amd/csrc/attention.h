@@ -442,15 +442,12 @@ __device__ __forceinline__ bool clean_values(uint8_t* v, int keys) {
     }
     return __any(special);
 }
-template <int N_>
-struct Unrolled {
-    static constexpr int N = N_;
-};
 // Infinities and NaNs of keys first .. last - 1, from their pages: add(q, e, value) is for value dim 8 q + 4 (lane / 32) + e of the lane's row.
 // (A page that does not exist has made its scores NaN already.)
-template <int DP, int TYPE, int MODE, int UNROLLED, typename Add>
+template <int DP, int TYPE, int MODE, typename Add>
 __device__ __forceinline__ void special_values(const Pool& s, int first, int last, int d_end, int lo, int hi, Add add) {
     const int half = (threadIdx.x & 63) >> 5;
+    constexpr int AT_ONCE = DP == 64 || (MODE & MODE_FP8) ? 8 : 16;   // loads on their way together (16 of 8 bits: masks spilled at 128 dims)
     last = last < s.kv_len ? last : s.kv_len;
 #pragma unroll 1
     for (int j = first; j < last; ++j) {
@@ -459,20 +456,29 @@ __device__ __forceinline__ void special_values(const Pool& s, int first, int las
         const uint8_t* v = s.v + (int64_t)page * s.page_bytes + (int64_t)(j - at * s.page_size) * s.token_bytes;
         uint32_t power = 0;
         if constexpr (MODE & MODE_FP8) power = s.v_scale[(int64_t)page * s.scale_page + (int64_t)(j - at * s.page_size) * s.scale_token];
-#pragma unroll UNROLLED
-        for (int q = 0; q < DP / 8; ++q) {
-            const int d = 8 * q + 4 * half;
-            uint2 w = make_uint2(0, 0);
-            if (d < d_end) {
-                if constexpr (MODE & MODE_FP8) {
-                    const uint32_t codes = power == 255 ? kNanCodes : *reinterpret_cast<const uint32_t*>(v + d);
-                    w = make_uint2(widen2<TYPE>(codes, __uint_as_float(power << 23), false), widen2<TYPE>(codes, __uint_as_float(power << 23), true));
-                } else w = *reinterpret_cast<const uint2*>(v + 2 * d);
+#pragma unroll 1
+        for (int q0 = 0; q0 < DP / 8; q0 += AT_ONCE) {
+            uint2 w[AT_ONCE];
+#pragma unroll
+            for (int q = 0; q < AT_ONCE; ++q) {
+                const int d = 8 * (q0 + q) + 4 * half;
+                w[q] = make_uint2(0, 0);
+                if (d < d_end) {
+                    if constexpr (MODE & MODE_FP8) w[q].x = *reinterpret_cast<const uint32_t*>(v + d);
+                    else w[q] = *reinterpret_cast<const uint2*>(v + 2 * d);
+                }
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t h = ((e & 2 ? w.y : w.x) >> (16 * (e & 1))) & 0xFFFFu;
-                if (any_special<TYPE>(h)) add(q, e, to_f32<TYPE>(h));
+            for (int q = 0; q < AT_ONCE; ++q) {
+                if constexpr (MODE & MODE_FP8) {
+                    const uint32_t codes = power == 255 && 8 * (q0 + q) + 4 * half < d_end ? kNanCodes : w[q].x;
+                    w[q] = make_uint2(widen2<TYPE>(codes, __uint_as_float(power << 23), false), widen2<TYPE>(codes, __uint_as_float(power << 23), true));
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t h = ((e & 2 ? w[q].y : w[q].x) >> (16 * (e & 1))) & 0xFFFFu;
+                    if (any_special<TYPE>(h)) add(q0 + q, e, to_f32<TYPE>(h));
+                }
             }
         }
     }
@@ -509,19 +515,21 @@ __device__ __forceinline__ void get_sums(State<DP>& st, const float* row) {
 // reads any more): in registers, an element of O each in the code, their masks spilled up to 270 scalars into vector registers that the loop over
 // the keys wants, and 8 to 24 bytes of scratch in the kernels of 8 bits and 128 dims (at 256, up to 556 with selects for the branches).  16 x 816 tokens
 // of 256 dims in half precision 68.5 to 67.6 us, 2048 over 8192 keys of 128 dims 257 to 252.  64 dims have the registers, and 30.5 us for 29.6 by way of LDS.
+// Where there is a NaN in every page: 16 x 816 causal tokens of 256 dims 767 to 635 us, but 2048 over 8192 keys of 128 dims 357 to 389
+// and 64 of up to 8192 keys 296 to 319.
 template <int DP, int TYPE, int MODE, int STEP>
 __device__ __forceinline__ void add_specials(State<DP>& st, float* sums, const Pool& s, int begin, int end, int all_lo, int all_hi, int d_end, int lo, int hi) {
-    auto blocks = [&](auto unrolled, auto add) {
+    auto blocks = [&](auto add) {
 #pragma unroll 1
         for (int blk = begin; blk < end; ++blk)
-            if (blk * STEP < all_lo || blk * STEP + STEP > all_hi) special_values<DP, TYPE, MODE, decltype(unrolled)::N>(s, blk * STEP, blk * STEP + STEP, d_end, lo, hi, add);
+            if (blk * STEP < all_lo || blk * STEP + STEP > all_hi) special_values<DP, TYPE, MODE>(s, blk * STEP, blk * STEP + STEP, d_end, lo, hi, add);
     };
     if constexpr (DP == 64) {
-        blocks(Unrolled<DP / 8>(), [&](int q, int e, float v) { st.o[q >> 2][4 * (q & 3) + e] += v; });
+        blocks([&](int q, int e, float v) { st.o[(q >> 2) & 1][4 * (q & 3) + e] += v; });
     } else {
         float* row = row_of_sums<DP>(sums);
         put_sums<DP>(st, row);
-        blocks(Unrolled<1>(), [&](int q, int e, float v) { row[8 * q + e] += v; });
+        blocks([&](int q, int e, float v) { row[8 * q + e] += v; });
         get_sums<DP>(st, row);
     }
 }
